@@ -30,6 +30,7 @@ from .gemm_op_a4w4 import (  # noqa: E402,F401
     unpack_mxfp8_out_scale,
 )
 from .batched_gemm_op_bf16 import batched_gemm_bf16, batched_gemm_bf16_CK, batched_gemm_bf16_tune  # noqa: E402,F401
+from .block_ops import act_and_mul, gated_residual_norm, gelu_and_mul, gelu_tanh_and_mul, silu_and_mul  # noqa: E402,F401
 from .gemm_op_a8w4 import gemm_a8w4_mxfp8  # noqa: E402,F401
 from .gemm_op_a8w8 import (  # noqa: E402,F401
     flatmm_a8w8_blockscale_asm,

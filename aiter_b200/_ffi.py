@@ -97,6 +97,8 @@ SIGNATURES = {
     "flatmm_a8w8_blockscale_asm": (T, T, T, T, T),
     "gemm_a8w8_blockscale_bpreshuffle_asm": (T, T, T, T, T, T, I, S, I, T),
     "aiter_b200_gemm_a8w8_mxfp8_noalloc": (T, T, T, T, T, I, I),
+    "aiter_b200_gated_residual_norm": (T, T, T, T, T, T, T, T, T, T, F, F, F, I, I, I),
+    "aiter_b200_act_and_mul": (T, T, T, I, I),
 }
 EXPORTS = sorted(
     list(SIGNATURES)

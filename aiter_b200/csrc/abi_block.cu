@@ -1,0 +1,368 @@
+// extern "C" entry points of the operators between two GEMMs (block_ops.cuh): argument checks and launches.
+#include "../../include/aiter_b200.h"
+#include "abi_checks.h"
+#include "block_ops.cuh"
+#include "launch.h"
+
+#include <algorithm>
+#include <string>
+
+using namespace b200;
+
+// defined in abi.cu: stores the message where aiter_get_last_error() finds it
+void aiter_b200_set_last_error(const std::string& msg);
+
+namespace {
+
+template <typename Fn>
+int safe_call(Fn&& fn)
+{
+    try
+    {
+        aiter_b200_set_last_error(std::string());
+        fn();
+        return 0;
+    }
+    catch(const std::exception& e)
+    {
+        aiter_b200_set_last_error(e.what());
+    }
+    catch(...)
+    {
+        aiter_b200_set_last_error("unknown C++ exception");
+    }
+    return -1;
+}
+
+// Makes a device current for a launch and puts the previous one back.
+struct DeviceGuard
+{
+    int prev = 0, cur;
+    explicit DeviceGuard(int device) : cur(device)
+    {
+        B200_CUDA(cudaGetDevice(&prev));
+        if(prev != cur)
+            B200_CUDA(cudaSetDevice(cur));
+    }
+    ~DeviceGuard()
+    {
+        if(prev != cur)
+            cudaSetDevice(prev);
+    }
+};
+
+int float_type(const aiter_tensor_t* t, const char* fn, const char* name)
+{
+    switch(t->dtype_)
+    {
+    case AITER_DTYPE_bf16: return OUT_BF16;
+    case AITER_DTYPE_fp16: return OUT_F16;
+    case AITER_DTYPE_fp32: return OUT_F32;
+    default: fail(fn, ": ", name, " must be bf16, fp16 or fp32 (got ", dtype_name(t->dtype_), ")");
+    }
+}
+int bytes_of(int dt) { return dt == OUT_F32 ? 4 : dt == OUT_E2M1 || dt == OUT_MXFP8 ? 1 : 2; }
+
+// every vector of eight elements of every row starts on a 16-byte boundary
+bool rows_aligned(const void* p, long long ld, int dt) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * bytes_of(dt)) % 16 == 0; }
+
+// A row of [M, n] values, contiguous along n
+RowTensor row_tensor(const aiter_tensor_t* t, const char* fn, const char* name, long long M, long long n)
+{
+    require_tensor(t, fn, name, 2);
+    B200_CHECK(t->shape[0] == M && t->shape[1] == n, fn, ": ", name, " must be [", M, ", ", n, "] (got [", t->shape[0], ", ", t->shape[1], "])");
+    require_rows_contiguous(t, fn, name);
+    return RowTensor{t->ptr, t->strides[0], float_type(t, fn, name)};
+}
+
+// [n] for every row, or [groups, n]: M must be a multiple of groups, row r uses entry r / (M / groups).  `scalar`: [groups, 1] is
+// allowed too (one value an entry).
+RowParam row_param(const aiter_tensor_t* t, const char* fn, const char* name, long long M, long long n, int* scalar = nullptr)
+{
+    if(scalar != nullptr)
+        *scalar = 0;
+    if(t == nullptr)
+        return RowParam{nullptr, 0, OUT_BF16, 1u};
+    require_tensor(t, fn, name, t->ndim == 1 ? 1 : 2);
+    B200_CHECK(t->ptr != nullptr, fn, ": ", name, " has a null data pointer");
+    const int dt       = float_type(t, fn, name);
+    const long long w  = t->shape[t->ndim - 1];
+    const bool one     = scalar != nullptr && t->ndim == 2 && w == 1 && n != 1;
+    B200_CHECK(w == n || one, fn, ": ", name, " must have ", n, " columns (got ", w, ")");
+    if(!one)
+        require_rows_contiguous(t, fn, name);
+    if(scalar != nullptr)
+        *scalar = one;
+    if(t->ndim == 1)
+        return RowParam{t->ptr, 0, dt, 1u};
+    const long long groups = t->shape[0];
+    B200_CHECK(groups >= 1 && M % groups == 0, fn, ": ", name, " has ", groups, " entries, which do not divide ", M, " rows");
+    return RowParam{t->ptr, groups == 1 ? 0 : t->strides[0], dt, static_cast<unsigned>(M / groups)};
+}
+
+struct Span
+{
+    uintptr_t first;
+    long long pitch, width; // bytes between rows, bytes of a row
+    long long rows;
+};
+Span span(const RowTensor& t, long long rows, long long n)
+{
+    const int b = bytes_of(t.dt);
+    return Span{reinterpret_cast<uintptr_t>(t.ptr), t.ld * b, (t.dt == OUT_E2M1 ? n / 2 : n * b), rows};
+}
+// Whether two sets of rows share memory (rows of one pitch may interleave: two column slices of one tensor do not overlap)
+bool overlap(const Span& a, const Span& b)
+{
+    if(a.first + static_cast<uintptr_t>((a.rows - 1) * a.pitch + a.width) <= b.first || b.first + static_cast<uintptr_t>((b.rows - 1) * b.pitch + b.width) <= a.first)
+        return false;
+    if(a.pitch != b.pitch || a.pitch <= 0)
+        return true;
+    const long long d = ((static_cast<long long>(b.first - a.first)) % a.pitch + a.pitch) % a.pitch;
+    return !(d >= a.width && d + b.width <= a.pitch);
+}
+bool same_rows(const RowTensor& a, const RowTensor& b) { return a.ptr == b.ptr && a.ld == b.ld && a.dt == b.dt; }
+
+// The MX output of [M, n] values: data as fp8 [M, n] or fp4x2 / uint8 [M, n / 2], and its scale array
+void mx_output(const aiter_tensor_t* out, const aiter_tensor_t* scales, int layout, const char* fn, long long M, long long n, RowTensor& y, BlockScales& sf)
+{
+    const bool fp4 = out->dtype_ != AITER_DTYPE_fp8;
+    B200_CHECK(n % 32 == 0, fn, ": MX outputs need a multiple of 32 columns (got ", n, ")");
+    B200_CHECK(layout >= 0 && layout <= 2, fn, ": shuffle_scale must be 0 (plain), 1 (e8m0_shuffle) or 2 ((m/32,k/4,32,4))");
+    B200_CHECK(out->shape[0] == M && out->shape[1] == (fp4 ? n / 2 : n), fn, ": out must be [M, ", (fp4 ? "n/2" : "n"), "]");
+    require_rows_contiguous(out, fn, "out");
+    B200_CHECK((reinterpret_cast<uintptr_t>(out->ptr) & 7) == 0 && out->strides[0] % 8 == 0, fn, ": out rows must start on 8-byte boundaries");
+    require_tensor(scales, fn, "scales", 2);
+    B200_CHECK(scales->dtype_ == AITER_DTYPE_fp8_e8m0 || scales->dtype_ == AITER_DTYPE_u8, fn, ": scales must be e8m0 / uint8 (got ", dtype_name(scales->dtype_), ")");
+    require_dense(scales, fn, "scales");
+    const long long kb = n / 32, rows32 = (M + 31) / 32 * 32;
+    if(layout == QSL_E8M0_SHUFFLE)
+        B200_CHECK(scales->shape[0] >= rows32 && scales->shape[1] >= (kb + 7) / 8 * 8 && scales->shape[1] % 8 == 0, fn, ": shuffled scales must be [>= pad32(M), pad8(n/32)]");
+    else if(layout == QSL_M32K4)
+    {
+        B200_CHECK(n % 128 == 0, fn, ": the (m/32,k/4,32,4) scale layout needs n % 128 == 0");
+        B200_CHECK(scales->shape[0] >= rows32 && scales->shape[1] == kb, fn, ": scales must be [pad32(M), n/32]");
+    }
+    else
+        B200_CHECK(scales->shape[0] >= M && scales->shape[1] >= kb, fn, ": scales must be [M, n/32]");
+    B200_CHECK(layout == QSL_PLAIN || (reinterpret_cast<uintptr_t>(scales->ptr) & 7) == 0, fn, ": scales must be 8-byte aligned");
+    y  = RowTensor{out->ptr, out->strides[0], fp4 ? OUT_E2M1 : OUT_MXFP8};
+    sf = BlockScales{static_cast<uint8_t*>(scales->ptr), static_cast<int>(scales->shape[1]), layout};
+}
+bool is_mx(const aiter_tensor_t* out)
+{
+    return out->dtype_ == AITER_DTYPE_fp8 || out->dtype_ == AITER_DTYPE_fp4x2 || out->dtype_ == AITER_DTYPE_u8;
+}
+
+template <typename Params>
+void launch(void (*kernel)(Params), dim3 grid, dim3 block, cudaStream_t stream, const Params& prm)
+{
+    // the set-up of the kernel may run while its predecessor in the stream drains: it waits before its first access
+    cudaLaunchConfig_t lc{};
+    lc.gridDim  = grid;
+    lc.blockDim = block;
+    lc.stream   = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs    = attr;
+    lc.numAttrs = programmatic_launch_enabled() ? 1 : 0;
+    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, prm));
+    count_launch();
+}
+
+constexpr unsigned kLongRow = 16384; // elements of a row that the register kernels hold at most (512 threads x 32)
+
+template <int VEC, int CNT>
+void launch_norm_rows(const NormParams& prm, dim3 grid, dim3 block, cudaStream_t stream)
+{
+    const bool x32 = prm.x.dt == OUT_F32, r32 = prm.res.ptr != nullptr && prm.res.dt == OUT_F32;
+    if(x32 && r32)
+        launch(norm_rows_kernel<VEC, CNT, true, true>, grid, block, stream, prm);
+    else if(x32)
+        launch(norm_rows_kernel<VEC, CNT, true, false>, grid, block, stream, prm);
+    else if(r32)
+        launch(norm_rows_kernel<VEC, CNT, false, true>, grid, block, stream, prm);
+    else
+        launch(norm_rows_kernel<VEC, CNT, false, false>, grid, block, stream, prm);
+}
+
+void launch_norm(const NormParams& prm, bool aligned, int sms, cudaStream_t stream)
+{
+    const unsigned n = prm.n;
+    if(n > kLongRow)
+    {
+        if(aligned)
+            launch(norm_long_kernel<8>, dim3(prm.M), dim3(512), stream, prm);
+        else
+            launch(norm_long_kernel<1>, dim3(prm.M), dim3(512), stream, prm);
+        return;
+    }
+    const unsigned per = aligned ? 8 : 1; // elements of a vector
+    const unsigned vecs = (n + per - 1) / per;
+    auto shape = [&](unsigned cnt) {
+        const unsigned t = ((vecs + cnt - 1) / cnt + 31) / 32 * 32;
+        const unsigned r = t == 32 ? 4 : 1; // a warp a row: four rows a CTA
+        return std::make_pair(dim3((prm.M + r - 1) / r), dim3(t, r));
+    };
+    if(!aligned)
+    {
+        // one element at a time: 8 or 32 a thread
+        const unsigned cnt = vecs > 2048 ? 32 : 8;
+        auto [grid, block] = shape(cnt);
+        if(cnt == 8)
+            launch_norm_rows<1, 8>(prm, grid, block, stream);
+        else
+            launch_norm_rows<1, 32>(prm, grid, block, stream);
+        return;
+    }
+    // one vector a thread where there are few rows (the shortest chain), up to four where the machine is full
+    const bool few     = prm.M <= 2u * static_cast<unsigned>(sms);
+    const unsigned cnt = vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1;
+    auto [grid, block] = shape(cnt);
+    if(cnt == 1)
+        launch_norm_rows<8, 1>(prm, grid, block, stream);
+    else if(cnt == 2)
+        launch_norm_rows<8, 2>(prm, grid, block, stream);
+    else
+        launch_norm_rows<8, 4>(prm, grid, block, stream);
+}
+
+template <int VEC, bool X32>
+void launch_act_mul(const ActMulParams& prm, cudaStream_t stream)
+{
+    constexpr int U                = VEC == 1 ? 8 : 2;
+    const unsigned long long total = static_cast<unsigned long long>(prm.M) * prm.row_vecs;
+    const unsigned long long ctas  = (total + 256 * U - 1) / (256 * U);
+    B200_CHECK(ctas < (1ull << 31), "act_and_mul: too many elements");
+    launch(act_mul_kernel<VEC, X32, U>, dim3(static_cast<unsigned>(ctas)), dim3(256), stream, prm);
+}
+
+} // namespace
+
+extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_t* scales, aiter_tensor_t* residual_out, aiter_tensor_t* x,
+                                              aiter_tensor_t* residual, aiter_tensor_t* weight, aiter_tensor_t* bias, aiter_tensor_t* gate,
+                                              aiter_tensor_t* post_weight, aiter_tensor_t* post_bias, float residual_scale,
+                                              float weight_offset, float eps, int norm, int post_norm, int shuffle_scale, void* stream)
+{
+    return safe_call([&] {
+        const char* fn = "aiter_b200_gated_residual_norm";
+        require_tensor(x, fn, "x", 2);
+        require_tensor(out, fn, "out", 2);
+        const long long M = x->shape[0], n = x->shape[1];
+        B200_CHECK(n > 0, fn, ": x must have at least one column");
+        B200_CHECK(M < (1LL << 31) && n < (1LL << 31), fn, ": dimension too large");
+        B200_CHECK(norm == 0 || norm == 1, fn, ": norm must be 0 (rms) or 1 (layer), got ", norm);
+        B200_CHECK(post_norm != 0 || (post_weight == nullptr && post_bias == nullptr), fn, ": post_weight and post_bias go with the first norm only");
+        NormParams prm{};
+        prm.x = row_tensor(x, fn, "x", M, n);
+        if(residual != nullptr)
+            prm.res = row_tensor(residual, fn, "residual", M, n);
+        if(residual_out != nullptr)
+            prm.h = row_tensor(residual_out, fn, "residual_out", M, n);
+        prm.weight      = row_param(weight, fn, "weight", M, n);
+        prm.bias        = row_param(bias, fn, "bias", M, n);
+        prm.gate        = row_param(gate, fn, "gate", M, n, &prm.gate_scalar);
+        prm.post_weight = row_param(post_weight, fn, "post_weight", M, n);
+        prm.post_bias   = row_param(post_bias, fn, "post_bias", M, n);
+        if(is_mx(out))
+            mx_output(out, scales, shuffle_scale, fn, M, n, prm.y, prm.sf);
+        else
+        {
+            B200_CHECK(scales == nullptr, fn, ": scales go with an MX output only");
+            prm.y = row_tensor(out, fn, "out", M, n);
+        }
+        for(const aiter_tensor_t* t : {out, scales, residual_out, residual, weight, bias, gate, post_weight, post_bias})
+            require_same_device(x, t, fn, "an argument");
+        if(M == 0)
+            return;
+        // written rows share no memory with one another or with what other rows read; a tensor may be updated in place
+        const Span sx = span(prm.x, M, n), sy = span(prm.y, M, n);
+        B200_CHECK((prm.y.dt <= OUT_F32 && same_rows(prm.y, prm.x)) || !overlap(sx, sy), fn, ": out overlaps x");
+        if(residual != nullptr)
+            B200_CHECK((prm.y.dt <= OUT_F32 && same_rows(prm.y, prm.res)) || !overlap(span(prm.res, M, n), sy), fn, ": out overlaps residual");
+        if(residual_out != nullptr)
+        {
+            const Span sh = span(prm.h, M, n);
+            B200_CHECK(!overlap(sh, sy), fn, ": residual_out overlaps out");
+            B200_CHECK(same_rows(prm.h, prm.x) || !overlap(sx, sh), fn, ": residual_out overlaps x");
+            B200_CHECK(residual == nullptr || same_rows(prm.h, prm.res) || !overlap(span(prm.res, M, n), sh), fn, ": residual_out overlaps residual");
+        }
+        prm.post          = post_norm != 0;
+        prm.layer         = norm;
+        prm.res_scale     = residual_scale;
+        prm.weight_offset = weight_offset;
+        prm.eps           = eps;
+        prm.inv_n         = 1.0f / static_cast<float>(n);
+        prm.M             = static_cast<unsigned>(M);
+        prm.n             = static_cast<unsigned>(n);
+        bool aligned = n % 8 == 0 && rows_aligned(prm.x.ptr, prm.x.ld, prm.x.dt) && (prm.res.ptr == nullptr || rows_aligned(prm.res.ptr, prm.res.ld, prm.res.dt)) &&
+                       (prm.h.ptr == nullptr || rows_aligned(prm.h.ptr, prm.h.ld, prm.h.dt)) && (prm.y.dt > OUT_F32 || rows_aligned(prm.y.ptr, prm.y.ld, prm.y.dt));
+        for(const RowParam* p : {&prm.weight, &prm.bias, &prm.post_weight, &prm.post_bias})
+            aligned = aligned && (p->ptr == nullptr || rows_aligned(p->ptr, p->ld, p->dt));
+        aligned = aligned && (prm.gate.ptr == nullptr || prm.gate_scalar || rows_aligned(prm.gate.ptr, prm.gate.ld, prm.gate.dt));
+        B200_CHECK(aligned || prm.y.dt <= OUT_F32, fn, ": with an MX output every row of every argument must start on a 16-byte boundary");
+        const int sms = device_sm_count(x->device_id);
+        DeviceGuard guard(x->device_id);
+        launch_norm(prm, aligned, sms, static_cast<cudaStream_t>(stream));
+    });
+}
+
+extern "C" int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* scales, aiter_tensor_t* input, int activation, int shuffle_scale, void* stream)
+{
+    return safe_call([&] {
+        const char* fn = "aiter_b200_act_and_mul";
+        require_tensor(input, fn, "input", 2);
+        require_tensor(out, fn, "out", 2);
+        const long long M = input->shape[0], n2 = input->shape[1], n = n2 / 2;
+        B200_CHECK(n2 > 0 && n2 % 2 == 0, fn, ": input must have an even number of columns (got ", n2, ")");
+        B200_CHECK(M < (1LL << 31) && n2 < (1LL << 31), fn, ": dimension too large");
+        B200_CHECK(activation > ACT_NONE && activation < ACT_COUNT, fn, ": activation must be 1 (relu), 2 (silu), 3 (gelu) or 4 (gelu_tanh), got ", activation);
+        const RowTensor in = row_tensor(input, fn, "input", M, n2);
+        RowTensor y{};
+        ActMulParams prm{};
+        if(is_mx(out))
+            mx_output(out, scales, shuffle_scale, fn, M, n, y, prm.sf);
+        else
+        {
+            B200_CHECK(scales == nullptr, fn, ": scales go with an MX output only");
+            y = row_tensor(out, fn, "out", M, n);
+        }
+        require_same_device(input, out, fn, "out");
+        require_same_device(input, scales, fn, "scales");
+        if(M == 0)
+            return;
+        B200_CHECK((y.dt <= OUT_F32 && same_rows(y, in)) || !overlap(span(in, M, n2), span(y, M, n)), fn, ": out overlaps the input (only the gate half may be overwritten in place)");
+        prm.in     = in.ptr;
+        prm.in_ld  = in.ld;
+        prm.in_dt  = in.dt;
+        prm.out    = y.ptr;
+        prm.out_ld = y.ld;
+        prm.out_dt = y.dt;
+        prm.act    = activation;
+        prm.M      = static_cast<unsigned>(M);
+        prm.n      = static_cast<unsigned>(n);
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const bool in_vec    = n % 8 == 0 && rows_aligned(in.ptr, in.ld, in.dt);
+        const bool x32       = in.dt == OUT_F32;
+        B200_CHECK(in_vec || y.dt <= OUT_F32, fn, ": with an MX output the input's rows must start on 16-byte boundaries");
+        DeviceGuard guard(input->device_id);
+        if(y.dt > OUT_F32)
+        {
+            const unsigned long long tiles = static_cast<unsigned long long>((M + 31) / 32) * ((n / 32 + 7) / 8);
+            B200_CHECK(tiles < (1ull << 31), fn, ": too many elements");
+            const dim3 grid(static_cast<unsigned>(tiles)), block(256);
+            if(y.dt == OUT_E2M1)
+                x32 ? launch(act_mul_mx_kernel<true, true>, grid, block, s, prm) : launch(act_mul_mx_kernel<false, true>, grid, block, s, prm);
+            else
+                x32 ? launch(act_mul_mx_kernel<true, false>, grid, block, s, prm) : launch(act_mul_mx_kernel<false, false>, grid, block, s, prm);
+            return;
+        }
+        const bool vec = in_vec && rows_aligned(y.ptr, y.ld, y.dt);
+        prm.row_vecs   = static_cast<unsigned>(vec ? n / 8 : n);
+        if(vec)
+            x32 ? launch_act_mul<8, true>(prm, s) : launch_act_mul<8, false>(prm, s);
+        else
+            x32 ? launch_act_mul<1, true>(prm, s) : launch_act_mul<1, false>(prm, s);
+    });
+}

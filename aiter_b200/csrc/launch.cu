@@ -537,6 +537,8 @@ static bool pdl_disabled()
     return off;
 }
 
+bool programmatic_launch_enabled() { return !pdl_disabled(); }
+
 // Raise the dynamic shared-memory limit once per device for one kernel; `attr_done` is the caller's
 // per-instantiation flag array (caller holds g_mutex).
 template <typename Kernel>

@@ -150,5 +150,6 @@ void set_wait_control(int device, unsigned long long limit_ns, int withhold_scal
 unsigned long long launch_count();
 void count_launch(); // kernels launched outside launch.cu report themselves here
 int device_sm_count(int device);
+bool programmatic_launch_enabled(); // launches carry the programmatic-serialization attribute
 
 } // namespace b200

@@ -210,6 +210,26 @@ AITER_B200_API int dynamic_per_group_scaled_quant(aiter_tensor_t* out, aiter_ten
                                                   int group_size, int shuffle_scale, aiter_tensor_t* num_rows,
                                                   int num_rows_factor, void* stream);
 
+/* ---- what stands between two GEMMs of a transformer block, one launch each.  No counterpart of this form in the reference
+ * (its closest: rmsnorm2d_fwd_with_add / layernorm2d_fwd_with_add, silu_and_mul / gelu_and_mul / gelu_tanh_and_mul).
+ *   u = x, or with post_norm != 0  norm(x) * post_weight + post_bias
+ *   h = residual_scale * residual + gate * u      -> residual_out (NULL: not stored; may be residual or x itself)
+ *   y = norm(h) * (weight_offset + weight) + bias -> out
+ * norm 0: v * rsqrt(mean v^2 + eps); 1: (v - mean v) * rsqrt(var v + eps).  x, residual, residual_out [M, n], bf16 / fp16 / fp32
+ * each, any row stride.  residual, weight, bias, gate, post_weight, post_bias may be NULL; parameters are [n], or [groups, n] with
+ * groups dividing M (row r uses entry r / (M / groups)); the gate may also be [groups, 1].
+ * out: [M, n] bf16 / fp16 / fp32 (scales NULL), or an MX operand: fp8 [M, n] or fp4x2 / uint8 [M, n / 2] with n % 32 == 0 and
+ * e8m0 scales laid out by shuffle_scale as in dynamic_per_group_scaled_quant; then every row starts on a 16-byte boundary. */
+AITER_B200_API int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_t* scales, aiter_tensor_t* residual_out,
+                                                  aiter_tensor_t* x, aiter_tensor_t* residual, aiter_tensor_t* weight,
+                                                  aiter_tensor_t* bias, aiter_tensor_t* gate, aiter_tensor_t* post_weight,
+                                                  aiter_tensor_t* post_bias, float residual_scale, float weight_offset, float eps,
+                                                  int norm, int post_norm, int shuffle_scale, void* stream);
+/* out[:, j] = act(input[:, j]) * input[:, n + j] for input [M, 2n] bf16 / fp16 / fp32.  activation: 1 relu, 2 silu, 3 gelu (erf),
+ * 4 gelu_tanh.  out and scales as above; out may be the gate half of input itself (same type). */
+AITER_B200_API int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* scales, aiter_tensor_t* input, int activation,
+                                          int shuffle_scale, void* stream);
+
 /* ---- library state ---- */
 /* Copies the 4-word device status record of `device` (0 = healthy; non-zero = a bounded wait
  * inside a kernel expired: code, block, split, iteration) and clears it.  Synchronises the device.

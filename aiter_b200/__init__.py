@@ -43,6 +43,7 @@ from .gemm_op_a8w8 import (  # noqa: E402,F401
     gemm_a8w8_mxfp8_noalloc,
 )
 from .gemm_op_a16w16 import gemm_a16w16_asm, gemm_a16w16_opus, opus_gemm, opus_gemm_a16w16_tune  # noqa: E402,F401
+from .gemm_op_fused import gemm_a16w16_fused, gemm_a4w4_fused, gemm_a8w8_mxfp8_fused  # noqa: E402,F401
 from .quant import (  # noqa: E402,F401
     dynamic_per_group_scaled_quant,
     get_hip_quant,

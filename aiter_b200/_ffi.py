@@ -10,9 +10,11 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
+from .dtypes import _torch_to_aiter_dtype as _DTYPE_IDS
 from .dtypes import aiter_dtype_id
 
 # AITER_B200_LIBRARY points at another build of the library (comparing two builds on one machine)
@@ -97,6 +99,9 @@ SIGNATURES = {
     "flatmm_a8w8_blockscale_asm": (T, T, T, T, T),
     "gemm_a8w8_blockscale_bpreshuffle_asm": (T, T, T, T, T, T, I, S, I, T),
     "aiter_b200_gemm_a8w8_mxfp8_noalloc": (T, T, T, T, T, I, I),
+    "aiter_b200_gemm_a16w16_fused": (T, T, T, T, T, I, I, S),
+    "aiter_b200_gemm_a8w8_mxfp8_fused": (T, T, T, T, T, T, T, I, I, S),
+    "aiter_b200_gemm_a4w4_fused": (T, T, T, T, T, T, T, I, I, S),
     "aiter_b200_gated_residual_norm": (T, T, T, T, T, T, T, T, T, T, F, F, F, I, I, I),
     "aiter_b200_act_and_mul": (T, T, T, I, I),
 }
@@ -109,24 +114,44 @@ EXPORTS = sorted(
 )
 
 
-def _convert(kind, value, keep):
-    if kind == T:
-        if value is None:
-            return None
-        at = torch_to_aiter(value)
-        keep.append(at)
-        return ctypes.byref(at)
-    if kind == I:
-        return ctypes.c_int(-1 if value is None else int(value))
-    if kind == F:
-        return ctypes.c_float(float(value))
-    if kind == S:
-        return None if value is None else ctypes.c_char_p(str(value).encode())
-    raise TypeError(kind)
+# aiter_tensor_t of an n-dimensional tensor as one packed byte string: filling the ctypes structure field by field took
+# 3.7 us a tensor, half of a small call's host time; this takes 1.5
+_PACKERS = [struct.Struct(f"@NNi4x{n}q{64 - 8 * n}x{n}q{64 - 8 * n}xii").pack for n in range(9)]
+assert all(len(_PACKERS[n](*([0] * (2 * n + 5)))) == 160 for n in range(9)), "aiter_tensor_t layout drifted from include/aiter_b200.h"
 
 
+def _pack_tensor(t):
+    if t is None:
+        return None
+    shape = t.shape
+    ndim = len(shape)
+    assert ndim <= 8, f"aiter_tensor_t supports at most 8 dims, got {ndim}"
+    dtype = _DTYPE_IDS.get(t.dtype)
+    return _PACKERS[ndim](t.data_ptr(), t.numel(), ndim, *shape, *t.stride(), aiter_dtype_id(t.dtype) if dtype is None else dtype,
+                          t.get_device() if t.is_cuda else -1)
+
+
+def _int(value):
+    return -1 if value is None else int(value)
+
+
+def _str(value):
+    return None if value is None else str(value).encode()
+
+
+_CONVERT = {T: (_pack_tensor, ctypes.c_char_p), I: (_int, ctypes.c_int), S: (_str, ctypes.c_char_p), F: (float, ctypes.c_float)}
 _FUNCS = {}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _bind(name: str):
+    """The library function with its argument types, and how each Python argument is converted (tensors travel as the bytes of
+    their descriptor, which the call reads before it returns)."""
+    kinds = SIGNATURES[name]
+    fn = getattr(_lib, name)
+    fn.argtypes = [_CONVERT[k][1] for k in kinds] + [ctypes.c_void_p]
+    _FUNCS[name] = bound = (fn, [_CONVERT[k][0] for k in kinds])
+    return bound
 
 
 # AITER_LOG_MORE=2 logs every call that crosses the C ABI with its arguments (tensors as shape / dtype / device), as
@@ -142,26 +167,18 @@ def _describe(a):
 
 def call(name: str, *args):
     """Call an entry point on the current CUDA stream of the first tensor's device."""
-    kinds = SIGNATURES[name]
-    assert len(args) == len(kinds), f"{name} takes {len(kinds)} arguments, got {len(args)}"
+    fn, convert = _FUNCS.get(name) or _bind(name)
+    assert len(args) == len(convert), f"{name} takes {len(convert)} arguments, got {len(args)}"
     if AITER_LOG_MORE == 2:
         import logging
 
         logging.getLogger("aiter").info("calling %s(%s)", name, ", ".join(_describe(a) for a in args))
-    keep = []
-    cargs = [_convert(k, a, keep) for k, a in zip(kinds, args)]
-    dev = next((a.device for a in args if isinstance(a, torch.Tensor) and a.is_cuda), None)
-    if dev is None:
-        stream = 0
-    elif _raw_stream is not None:
-        stream = _raw_stream(dev.index if dev.index is not None else torch.cuda.current_device())
-    else:
-        stream = torch.cuda.current_stream(dev).cuda_stream
-    fn = _FUNCS.get(name)
-    if fn is None:
-        fn = _FUNCS[name] = getattr(_lib, name)
-    rc = fn(*cargs, ctypes.c_void_p(stream))
-    if rc != 0:
+    stream = None
+    for a in args:
+        if isinstance(a, torch.Tensor) and a.is_cuda:
+            stream = _raw_stream(a.get_device()) if _raw_stream is not None else torch.cuda.current_stream(a.device).cuda_stream
+            break
+    if fn(*[c(a) for c, a in zip(convert, args)], stream) != 0:
         msg = _lib.aiter_get_last_error()
         raise RuntimeError(f"{name} failed: {msg.decode() if msg else 'unknown error'}")
 

@@ -4,7 +4,7 @@ instead of 16-bit values.  The reference's closest forms: aiter/ops/rmsnorm.py, 
 from __future__ import annotations
 
 import torch
-from torch import Tensor
+from torch import Tensor, empty
 
 from . import _ffi, dtypes
 
@@ -24,19 +24,17 @@ def _mx_out(fn: str, m: int, n: int, quant_dtype, shuffle, device):
     if n % 32 != 0:
         raise ValueError(f"{fn}: an MX output needs a multiple of 32 columns, got {n}")
     if quant_dtype == dtypes.fp4x2:
-        y = torch.empty((m, n // 2), dtype=torch.uint8, device=device).view(dtypes.fp4x2)
+        y = empty(m, n // 2, dtype=dtypes.fp4x2, device=device)
     elif quant_dtype == dtypes.fp8:
-        y = torch.empty((m, n), dtype=dtypes.fp8, device=device)
+        y = empty(m, n, dtype=dtypes.fp8, device=device)
     else:
         raise ValueError(f"{fn}: unsupported quant_dtype {quant_dtype}, expected one of (dtypes.fp4x2, dtypes.fp8)")
     kb = n // 32
     if shuffle == 2:
-        shape = ((m + 31) // 32 * 32, kb)
+        m = (m + 31) // 32 * 32
     elif shuffle:
-        shape = ((m + 255) // 256 * 256, (kb + 7) // 8 * 8)
-    else:
-        shape = (m, kb)
-    return y, torch.empty(shape, dtype=dtypes.fp8_e8m0, device=device)
+        m, kb = (m + 255) // 256 * 256, (kb + 7) // 8 * 8
+    return y, empty(m, kb, dtype=dtypes.fp8_e8m0, device=device)
 
 
 def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -76,7 +74,7 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
     elif copies_x:
         h, h2 = x, None
     else:
-        h = torch.empty(x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
+        h = empty(*x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
         h2 = h if h.dim() == 2 else h.view(-1, n)
     scale, layout = None, 0
     if quant_dtype is not None:
@@ -85,7 +83,7 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
         y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
     else:
-        y = torch.empty((m, n), dtype=x.dtype if otype is None else otype, device=x.device)
+        y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
     _ffi.call("aiter_b200_gated_residual_norm", y, scale, h2, x2, r2, weight, bias, gate, post_weight, post_bias, residual_scale,
               weight_offset, eps, _NORMS[norm], post, layout)
     if x.dim() != 2:
@@ -113,7 +111,7 @@ def act_and_mul(x: Tensor, activation: str = "silu", otype: torch.dtype | None =
         y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
     else:
-        y = torch.empty((m, n), dtype=x.dtype if otype is None else otype, device=x.device)
+        y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
     _ffi.call("aiter_b200_act_and_mul", y, scale, x2, act, layout)
     if x.dim() != 2:
         y = y.view(*x.shape[:-1], y.shape[-1])

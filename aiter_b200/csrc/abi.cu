@@ -1,6 +1,7 @@
 // extern "C" entry points: argument checking, aiter_tensor_t -> GemmProblem, error bridge.
 #include "../../include/aiter_b200.h"
 #include "abi_checks.h"
+#include "activation.cuh"
 #include "gemm_common.cuh"
 #include "launch.h"
 #include "quant_mx.cuh"
@@ -62,10 +63,62 @@ static void apply_config(GemmProblem& p, const char* kernelName, int log2_splitk
         B200_CHECK(parse_config_name(kernelName, p.cfg), fn, ": not find kernel ", kernelName);
 }
 
+// Fused epilogue: out = act(A B^T + bias) + residual
+struct FusedArgs
+{
+    const aiter_tensor_t* bias;
+    const aiter_tensor_t* residual;
+    int activation;
+};
+
+static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_tensor_t* out, const FusedArgs& f, const char* fn)
+{
+    const long long M = p.M, N = p.N;
+    require_tensor(out, fn, "out", 2);
+    B200_CHECK(out->shape[0] == M && out->shape[1] == N, fn, ": out must be [", M, ", ", N, "] (got [", out->shape[0], ", ", out->shape[1], "])");
+    require_rows_contiguous(out, fn, "out");
+    p.out_mode = plain_out_mode(out->dtype_);
+    B200_CHECK(p.out_mode >= 0, fn, ": out must be bf16, fp16 or fp32 (got ", dtype_name(out->dtype_), ")");
+    B200_CHECK(f.activation >= ACT_NONE && f.activation < ACT_COUNT, fn, ": activation must be 0 (none), 1 (relu), 2 (silu), 3 (gelu) or 4 (gelu_tanh), got ", f.activation);
+    require_same_device(first, out, fn, "out");
+    p.out        = out->ptr;
+    p.ldo        = M == 1 ? (N + 7) / 8 * 8 : out->strides[0]; // (one row: any pitch, and one that allows a tensor map)
+    p.fused      = true;
+    p.activation = f.activation;
+    if(f.bias != nullptr)
+    {
+        require_tensor(f.bias, fn, "bias", 1);
+        B200_CHECK(f.bias->shape[0] == N, fn, ": bias must be [", N, "] (got [", f.bias->shape[0], "])");
+        require_rows_contiguous(f.bias, fn, "bias");
+        require_same_device(first, f.bias, fn, "bias");
+        p.fused_bias      = f.bias->ptr;
+        p.fused_bias_mode = plain_out_mode(f.bias->dtype_);
+        B200_CHECK(p.fused_bias_mode >= 0, fn, ": bias must be bf16, fp16 or fp32 (got ", dtype_name(f.bias->dtype_), ")");
+    }
+    if(f.residual != nullptr)
+    {
+        const aiter_tensor_t* r = f.residual;
+        require_tensor(r, fn, "residual", 2);
+        B200_CHECK(r->shape[0] == M && r->shape[1] == N, fn, ": residual must be [", M, ", ", N, "] (got [", r->shape[0], ", ", r->shape[1], "])");
+        require_rows_contiguous(r, fn, "residual");
+        require_same_device(first, r, fn, "residual");
+        p.residual      = r->ptr;
+        p.residual_ld   = M == 1 ? (N + 7) / 8 * 8 : r->strides[0];
+        p.residual_mode = plain_out_mode(r->dtype_);
+        B200_CHECK(p.residual_mode >= 0, fn, ": residual must be bf16, fp16 or fp32 (got ", dtype_name(r->dtype_), ")");
+        // every value is read by the thread that writes it: the very same matrix may be updated in place, nothing else may overlap
+        const int rb = p.residual_mode == OUT_F32 ? 4 : 2, ob = p.out_mode == OUT_F32 ? 4 : 2;
+        const bool same = r->ptr == out->ptr && p.residual_ld == p.ldo && p.residual_mode == p.out_mode;
+        B200_CHECK(M == 0 || same ||
+                       !overlap(Span{reinterpret_cast<uintptr_t>(r->ptr), p.residual_ld * rb, N * rb, M}, Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}),
+                   fn, ": out overlaps residual");
+    }
+}
+
 // ------------------------------------------------------------------------------------------- MXFP4
 static void run_mxfp4(const char* fn, aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* A_scale,
                       aiter_tensor_t* B_scale, aiter_tensor_t* out, aiter_tensor_t* bias, float alpha, float beta,
-                      int a_mode, int b_mode, int wire, const KernelConfig& cfg, void* stream)
+                      int a_mode, int b_mode, int wire, const KernelConfig& cfg, void* stream, const FusedArgs* fused = nullptr)
 {
     require_tensor(A, fn, "A", 2);
     require_tensor(B, fn, "B", 2);
@@ -87,7 +140,14 @@ static void run_mxfp4(const char* fn, aiter_tensor_t* A, aiter_tensor_t* B, aite
     p.wgt    = Operand{B->ptr, N, Kb, Kb, b_mode};
     p.act_sf = scale_operand(A_scale, wire, fn, "A_scale");
     p.wgt_sf = scale_operand(B_scale, wire, fn, "B_scale");
-    set_out(p, out, fn, M, N);
+    if(fused != nullptr)
+    {
+        set_fused(p, A, out, *fused, fn);
+        for(const aiter_tensor_t* t : {B, A_scale, B_scale})
+            require_same_device(A, t, fn, "an operand");
+    }
+    else
+        set_out(p, out, fn, M, N);
     if(bias != nullptr)
     {
         B200_CHECK(bias->dtype_ == AITER_DTYPE_fp32 && static_cast<long long>(bias->numel_) == N, fn,
@@ -239,10 +299,11 @@ extern "C" int nvfp4_gemm_asm(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor
 
 // ------------------------------------------------------------------------------------------- MXFP8
 static void run_mxfp8(const char* fn, int b_is_fp4, aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* ScaleA,
-                      aiter_tensor_t* ScaleB, aiter_tensor_t* out, const char* kernelName, int a_preshuffle, void* stream)
+                      aiter_tensor_t* ScaleB, aiter_tensor_t* out, const char* kernelName, int a_preshuffle, void* stream,
+                      const FusedArgs* fused = nullptr)
 {
     require_tensor(out, fn, "out", 2);
-    B200_CHECK(out->dtype_ == AITER_DTYPE_bf16, fn, " only supports BFloat16 output");
+    B200_CHECK(fused != nullptr || out->dtype_ == AITER_DTYPE_bf16, fn, " only supports BFloat16 output");
     B200_CHECK(a_preshuffle == 0 || a_preshuffle == 1, fn, " a_preshuffle must be 0 or 1");
     require_tensor(A, fn, "A", 2);
     require_tensor(B, fn, "B", 2);
@@ -259,7 +320,14 @@ static void run_mxfp8(const char* fn, int b_is_fp4, aiter_tensor_t* A, aiter_ten
     p.wgt    = Operand{B->ptr, N, b_is_fp4 ? K / 2 : K, b_is_fp4 ? K / 2 : K, OPM_TILE16};
     p.act_sf = scale_operand(ScaleA, SFW_G1250, fn, "ScaleA");
     p.wgt_sf = scale_operand(ScaleB, SFW_G1250, fn, "ScaleB");
-    set_out(p, out, fn, M, N);
+    if(fused != nullptr)
+    {
+        set_fused(p, A, out, *fused, fn);
+        for(const aiter_tensor_t* t : {B, ScaleA, ScaleB})
+            require_same_device(A, t, fn, "an operand");
+    }
+    else
+        set_out(p, out, fn, M, N);
     p.device = A->device_id;
     p.stream = static_cast<cudaStream_t>(stream);
     apply_config(p, kernelName, -1, fn);
@@ -431,7 +499,7 @@ extern "C" int gemm_a8w8_blockscale_bpreshuffle_asm(aiter_tensor_t* A, aiter_ten
 
 // ------------------------------------------------------------------------------------------- bf16
 static void run_bf16(const char* fn, const aiter_tensor_t* A, const aiter_tensor_t* B, const aiter_tensor_t* out,
-                     const aiter_tensor_t* bias, int bpreshuffle, const KernelConfig& cfg, void* stream)
+                     const aiter_tensor_t* bias, int bpreshuffle, const KernelConfig& cfg, void* stream, const FusedArgs* fused = nullptr)
 {
     // A [.., M, K], B [.., N, K], out [.., M, N]; a leading batch dimension (3-D form) becomes one more tile coordinate
     // of the same launch
@@ -486,10 +554,53 @@ static void run_bf16(const char* fn, const aiter_tensor_t* A, const aiter_tensor
     }
     p.alpha  = 1.f;
     p.beta   = 1.f;
+    if(fused != nullptr)
+    {
+        set_fused(p, A, out, *fused, fn);
+        require_same_device(A, B, fn, "B");
+    }
     p.device = A->device_id;
     p.stream = static_cast<cudaStream_t>(stream);
     p.cfg    = cfg;
     launch_gemm(p);
+}
+
+extern "C" int aiter_b200_gemm_a16w16_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* bias, aiter_tensor_t* residual,
+                                            aiter_tensor_t* out, int activation, int bpreshuffle, const char* kernelName, void* stream)
+{
+    return safe_call([&] {
+        const char* fn = "aiter_b200_gemm_a16w16_fused";
+        require_tensor(A, fn, "A", 2);
+        require_tensor(B, fn, "B", 2);
+        require_tensor(out, fn, "out", 2);
+        GemmProblem tmp;
+        apply_config(tmp, kernelName, -1, fn);
+        const FusedArgs f{bias, residual, activation};
+        run_bf16(fn, A, B, out, nullptr, bpreshuffle, tmp.cfg, stream, &f);
+    });
+}
+
+extern "C" int aiter_b200_gemm_a8w8_mxfp8_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* ScaleA, aiter_tensor_t* ScaleB,
+                                                aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
+                                                int a_preshuffle, const char* kernelName, void* stream)
+{
+    return safe_call([&] {
+        const FusedArgs f{bias, residual, activation};
+        run_mxfp8("aiter_b200_gemm_a8w8_mxfp8_fused", 0, A, B, ScaleA, ScaleB, out, kernelName, a_preshuffle, stream, &f);
+    });
+}
+
+extern "C" int aiter_b200_gemm_a4w4_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* A_scale, aiter_tensor_t* B_scale,
+                                          aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
+                                          int bpreshuffle, const char* kernelName, void* stream)
+{
+    return safe_call([&] {
+        const char* fn = "aiter_b200_gemm_a4w4_fused";
+        GemmProblem tmp;
+        apply_config(tmp, kernelName, -1, fn);
+        const FusedArgs f{bias, residual, activation};
+        run_mxfp4(fn, A, B, A_scale, B_scale, out, nullptr, 1.f, 0.f, OPM_ROWMAJOR, bpreshuffle ? OPM_TILE16 : OPM_ROWMAJOR, SFW_E8M0_SHUFFLE, tmp.cfg, stream, &f);
+    });
 }
 
 extern "C" int gemm_a16w16_asm(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* out, aiter_tensor_t* semaphore,

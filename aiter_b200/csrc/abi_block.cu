@@ -100,26 +100,10 @@ RowParam row_param(const aiter_tensor_t* t, const char* fn, const char* name, lo
     return RowParam{t->ptr, groups == 1 ? 0 : t->strides[0], dt, static_cast<unsigned>(M / groups)};
 }
 
-struct Span
-{
-    uintptr_t first;
-    long long pitch, width; // bytes between rows, bytes of a row
-    long long rows;
-};
 Span span(const RowTensor& t, long long rows, long long n)
 {
     const int b = bytes_of(t.dt);
     return Span{reinterpret_cast<uintptr_t>(t.ptr), t.ld * b, (t.dt == OUT_E2M1 ? n / 2 : n * b), rows};
-}
-// Whether two sets of rows share memory (rows of one pitch may interleave: two column slices of one tensor do not overlap)
-bool overlap(const Span& a, const Span& b)
-{
-    if(a.first + static_cast<uintptr_t>((a.rows - 1) * a.pitch + a.width) <= b.first || b.first + static_cast<uintptr_t>((b.rows - 1) * b.pitch + b.width) <= a.first)
-        return false;
-    if(a.pitch != b.pitch || a.pitch <= 0)
-        return true;
-    const long long d = ((static_cast<long long>(b.first - a.first)) % a.pitch + a.pitch) % a.pitch;
-    return !(d >= a.width && d + b.width <= a.pitch);
 }
 bool same_rows(const RowTensor& a, const RowTensor& b) { return a.ptr == b.ptr && a.ld == b.ld && a.dt == b.dt; }
 

@@ -50,6 +50,24 @@ inline void require_dense(const aiter_tensor_t* t, const char* fn, const char* n
     }
 }
 
+// The memory of a matrix: rows of `width` bytes, `pitch` bytes apart
+struct Span
+{
+    uintptr_t first;
+    long long pitch, width;
+    long long rows;
+};
+// Whether two matrices share memory (rows of one pitch may interleave: two column slices of one tensor do not overlap)
+inline bool overlap(const Span& a, const Span& b)
+{
+    if(a.first + static_cast<uintptr_t>((a.rows - 1) * a.pitch + a.width) <= b.first || b.first + static_cast<uintptr_t>((b.rows - 1) * b.pitch + b.width) <= a.first)
+        return false;
+    if(a.pitch != b.pitch || a.pitch <= 0)
+        return true;
+    const long long d = ((static_cast<long long>(b.first - a.first)) % a.pitch + a.pitch) % a.pitch;
+    return !(d >= a.width && d + b.width <= a.pitch);
+}
+
 inline ScaleOperand scale_operand(const aiter_tensor_t* s, int wire, const char* fn, const char* name)
 {
     require_tensor(s, fn, name, 2);

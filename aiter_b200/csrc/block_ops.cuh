@@ -119,19 +119,20 @@ __device__ __forceinline__ void unpack(const Raw<VEC, B32>& r, int dt, float (&v
             v[i] = dec16((r.w[VEC == 1 ? 0 : i >> 1] >> (16 * (i & 1))) & 0xFFFFu, OUT_F16);
     }
 }
-// parameters: the type is looked at here (they are few, and in L1 after the first rows)
+// parameters: the type is looked at here (they are few, and in L1 after the first rows).  Plain loads: a gate or a modulation may
+// come from the kernel just before, which this one overlaps up to its dependency wait.
 template <int VEC>
 __device__ __forceinline__ void ld_param(const void* base, int dt, size_t at, float (&v)[VEC])
 {
     if(VEC == 1)
-        v[0] = dt == OUT_F32 ? __ldg(static_cast<const float*>(base) + at) : dec16(__ldg(static_cast<const uint16_t*>(base) + at), dt);
+        v[0] = dt == OUT_F32 ? static_cast<const float*>(base)[at] : dec16(static_cast<const uint16_t*>(base)[at], dt);
     else if(dt == OUT_F32)
     {
         const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
 #pragma unroll
         for(int i = 0; i < VEC / 4; ++i)
         {
-            const float4 t = __ldg(p + i);
+            const float4 t = p[i];
             v[VEC == 1 ? 0 : 4 * i]     = t.x;
             v[VEC == 1 ? 0 : 4 * i + 1] = t.y;
             v[VEC == 1 ? 0 : 4 * i + 2] = t.z;
@@ -140,7 +141,7 @@ __device__ __forceinline__ void ld_param(const void* base, int dt, size_t at, fl
     }
     else
     {
-        const uint4 t = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+        const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
         Raw<8, false> r;
         r.w[0] = t.x, r.w[1] = t.y, r.w[2] = t.z, r.w[3] = t.w;
         float f[8];

@@ -20,6 +20,7 @@
 //        6 raw-scale producer.  Every barrier wait is bounded (bounded_wait).
 #pragma once
 #include "gemm_common.cuh"
+#include "epilogue.cuh"
 
 namespace b200 {
 
@@ -58,11 +59,11 @@ __host__ __device__ constexpr int decode_sf_unit(int kind) { return kind == KIND
 // (the mixed kind, e4m3 activations x packed e2m1 weights, is MXF8 once the scale warps have widened the weight tile to
 // e4m3 in shared memory: exact, every e2m1 value is an e4m3 value)
 
-template <int KIND, int SFW>
+template <int KIND, int SFW, int EPI>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                    const __grid_constant__ CUtensorMap map_sfp, const __grid_constant__ CUtensorMap map_sfq,
-                   const __grid_constant__ CUtensorMap map_out, const DecodeParams prm)
+                   const __grid_constant__ CUtensorMap map_out, const DecodeParams prm, const __grid_constant__ EpilogueParams<EPI> epi)
 {
     constexpr bool kScaled = (KIND != KIND_BF16);
     constexpr bool kMixed  = (KIND == KIND_MXF8F4);
@@ -322,6 +323,25 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         const int p_local    = quarter * 32 + lane;
         const uint32_t tlane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         bool ok = true;
+        // (fused epilogue) this thread's bias and the residual of its first 16 rows: under way before the K loop ends
+        float bias0 = 0.f;
+        uint32_t res0[16];
+        if constexpr(EPI != 0)
+        {
+            const int p0 = row_p0 + p_local;
+            if(p0 < prm.rows_p && (csplit == 1 || static_cast<uint32_t>(p_local) / per == zrank))
+            {
+                if(epi.bias != nullptr)
+                    bias0 = load_elem(epi.bias, epi.bias_mode, p0);
+                if(epi.res != nullptr)
+                {
+#pragma unroll
+                    for(int j = 0; j < 16; ++j)
+                        if(row_q0 + j < prm.rows_q)
+                            res0[j] = load_elem_raw(epi.res, epi.res_mode, static_cast<size_t>(row_q0 + j) * epi.res_ld + p0);
+                }
+            }
+        }
         if(kScaled)
         {
             const int q_groups = (bn + 31) / 32; // 1 to 4 groups of 32 activation rows (the weights always stage 4)
@@ -607,6 +627,12 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             if(ok && mine)
             {
                 const int p = row_p0 + p_local;
+                auto out16  = [&](float x) -> uint16_t {
+                    if constexpr(EPI != 0)
+                        return cvt_out16(x, epi.out_mode == OUT_F16);
+                    else
+                        return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+                };
                 if(prm.bias != nullptr)
                 {
                     const float b = (p < prm.rows_p) ? prm.beta * load_bias(prm.bias, prm.bias_is_bf16, p) : 0.f;
@@ -622,7 +648,47 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                         if(j < bw)
                             v[j] *= prm.alpha;
                 }
-                if(prm.tma_store)
+                if constexpr(EPI != 0)
+                {
+                    if(epi.bias != nullptr)
+                    {
+#pragma unroll
+                        for(int j = 0; j < 64; ++j)
+                            v[j] += bias0;
+                    }
+                    activate(v, epi.act);
+                    if(epi.res != nullptr && p < prm.rows_p)
+                    {
+#pragma unroll
+                        for(int j = 0; j < 64; ++j)
+                            if(j < bw && row_q0 + c0 + j < prm.rows_q)
+                            {
+                                if(j < 16 && h == 0)
+                                    v[j] += raw_to_f32(res0[j & 15], epi.res_mode);
+                                else
+                                    v[j] += load_elem(epi.res, epi.res_mode, static_cast<size_t>(row_q0 + c0 + j) * epi.res_ld + p);
+                            }
+                    }
+                }
+                if(EPI != 0 && prm.tma_store == 2)
+                {
+                    // fp32 output: [row m][32 floats], 8 KB a warp (tiles of at most 64 rows)
+                    float* buf = reinterpret_cast<float*>(smem_gen + static_cast<uint32_t>(warp - 2) * 8192u);
+#pragma unroll
+                    for(int j = 0; j < 64; ++j)
+                        if(j < bw)
+                            buf[j * 32 + lane] = v[j];
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    const int p_warp0 = row_p0 + quarter * 32;
+                    if(lane == 0 && p_warp0 < prm.rows_p)
+                    {
+                        tma_store_2d(&map_out, smem_base + static_cast<uint32_t>(warp - 2) * 8192u, p_warp0 * 4, row_q0);
+                        bulk_commit_group();
+                        bulk_wait_group_read<0>();
+                    }
+                }
+                else if(prm.tma_store)
                 {
                     // this warp's 32 output columns x bw rows, staged as [row m][32 x bf16] in a retired operand stage (every
                     // tile load has landed and been consumed once the accumulator is complete; a buffer per warp and chunk)
@@ -632,7 +698,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 #pragma unroll
                     for(int j = 0; j < 64; ++j)
                         if(j < bw)
-                            reinterpret_cast<__nv_bfloat16*>(buf)[j * 32 + lane] = __float2bfloat16_rn(v[j]);
+                            reinterpret_cast<uint16_t*>(buf)[j * 32 + lane] = out16(v[j]);
                     fence_proxy_async_smem();
                     __syncwarp();
                     const int p_warp0 = row_p0 + quarter * 32;
@@ -651,7 +717,13 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 #pragma unroll
                     for(int j = 0; j < 64; ++j)
                         if(j < bw && row_q0 + c0 + j < prm.rows_q)
-                            prm.out[static_cast<size_t>(row_q0 + c0 + j) * prm.ldo + p] = __float2bfloat16_rn(v[j]);
+                        {
+                            const size_t at = static_cast<size_t>(row_q0 + c0 + j) * prm.ldo + p;
+                            if constexpr(EPI != 0)
+                                store_out(prm.out, at, v[j], epi.out_mode);
+                            else
+                                prm.out[at] = __float2bfloat16_rn(v[j]);
+                        }
                 }
             }
             } // chunks of 64 columns

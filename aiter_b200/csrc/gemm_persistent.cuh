@@ -33,6 +33,7 @@
 //   acc_empty[a]  leader: all epilogue warps of all CTAs have drained accumulator a
 #pragma once
 #include "gemm_common.cuh"
+#include "epilogue.cuh"
 
 namespace b200 {
 
@@ -150,11 +151,11 @@ struct WorkIter
     bool valid;
 };
 
-template <int KIND, int SFW, int CG>
+template <int KIND, int SFW, int CG, int EPI>
 __global__ void __launch_bounds__(kPersistentThreads, 1)
 gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_sfp, const __grid_constant__ CUtensorMap map_sfq,
-                       const __grid_constant__ CUtensorMap map_out, const PersistentParams prm)
+                       const __grid_constant__ CUtensorMap map_out, const PersistentParams prm, const __grid_constant__ EpilogueParams<EPI> epi)
 {
     constexpr bool kScaled = (KIND != KIND_BF16);
     constexpr bool kMixed  = (KIND == KIND_MXF8F4);
@@ -209,6 +210,9 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
 
     if(threadIdx.x == 0)
     {
+        if constexpr(EPI != 0)
+            for(int i = 0; i < 8; ++i) // the residual tiles of the fused epilogue: two per epilogue warp
+                mbar_init(smem_base + L.total + 8u * i, 1);
         for(int s = 0; s < S; ++s)
         {
             // one expect_tx arrival per operand producer and one arrival per scale warp, of every CTA of the pair
@@ -834,7 +838,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         const uint32_t tlane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const int chunk      = bn < 32 ? 16 : 32;
         const int n_chunks   = bn / chunk;
-        const bool split     = (splits > 1);
+        const bool split     = EPI == 0 && (splits > 1); // (the fused epilogue splits K in clusters only)
         const uint32_t acc_empty_remote = (CG == 2) ? map_to_cta(acc_empty_bar(0), 0) : 0u;
         const bool vec_ok = (!prm.transposed_out) && ((prm.ldo & (prm.out_mode == OUT_F32 ? 3 : 7)) == 0) && ((reinterpret_cast<uintptr_t>(prm.out) & 15) == 0) &&
                             ((prm.out_batch_stride & 7) == 0);
@@ -846,6 +850,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         const uint32_t epi_s = smem_base + L.epi_off + (warp - 6) * epi_warp_bytes;
         int ebuf             = 0;
         uint32_t wbuf        = 0; // wide stores: which of the two 4 KB buffers comes next (0 when there is only one)
+        FusedStore fused;         // (fused epilogue) this warp's place in its ring of two slots
         if(use_tma && lane == 0)
             tma_prefetch_desc(&map_out);
         uint32_t epi_phase = 0;
@@ -940,6 +945,10 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                                 static_cast<size_t>(w.b) * static_cast<size_t>(prm.out_batch_stride) * (prm.out_mode == OUT_F32 ? 4u : 2u);
             const void* const bias_b = prm.bias == nullptr ? nullptr
                                        : static_cast<const uint8_t*>(prm.bias) + static_cast<size_t>(w.b) * static_cast<size_t>(prm.bias_batch_stride) * (prm.bias_is_bf16 ? 2u : 4u);
+            if constexpr(EPI != 0)
+                if(prm.tma_store == 3)
+                    fused_begin(fused, epi, (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32, row_q0, bn, epi_s_fused(smem_base, L.epi_off, warp - 6, epi),
+                                smem_base + L.total + 16u * (warp - 6), lane);
             ok = bounded_wait(acc_full_bar(a), (uc / prm.n_acc) & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, uc);
             ok = __all_sync(0xffffffffu, ok);
             if(!ok)
@@ -1064,6 +1073,34 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                         for(int j = 0; j < 32; ++j)
                             v[j] *= prm.alpha;
                     }
+                    if constexpr(EPI != 0)
+                    {
+                        if(epi.bias != nullptr)
+                        {
+                            if(prm.bias_on_q)
+                                add_row<32>(v, epi.bias, epi.bias_mode, q_first, min(chunk, prm.rows_q - q_first), epi.bias_vec != 0);
+                            else
+                            {
+                                const float b = p < prm.rows_p ? load_elem(epi.bias, epi.bias_mode, p) : 0.f;
+#pragma unroll
+                                for(int j = 0; j < 32; ++j)
+                                    v[j] += b;
+                            }
+                        }
+                        activate(v, epi.act);
+                        if(epi.res != nullptr && p < prm.rows_p)
+                        {
+                            if(!prm.transposed_out)
+                                add_row<32>(v, epi.res, epi.res_mode, static_cast<size_t>(p) * epi.res_ld + q_first, min(chunk, prm.rows_q - q_first), epi.res_vec != 0);
+                            else
+                            {
+#pragma unroll
+                                for(int j = 0; j < 32; ++j)
+                                    if(j < chunk && q_first + j < prm.rows_q)
+                                        v[j] += load_elem(epi.res, epi.res_mode, static_cast<size_t>(q_first + j) * epi.res_ld + p);
+                            }
+                        }
+                    }
                     if(use_tma)
                     {
                         if(lane == 0)
@@ -1156,7 +1193,22 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                         }
                     }
                 };
-                if(prm.out_mode >= OUT_E2M1)
+                if(EPI != 0 && prm.tma_store == 3)
+                {
+                    // Fused epilogue with tile loads of the residual and tile stores (row-major output): 64 or 32 columns a step
+                    if constexpr(EPI != 0)
+                    {
+                        const int p_warp0 = (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32;
+                        const uint32_t slots = epi_s_fused(smem_base, L.epi_off, warp - 6, epi);
+                        uint8_t* slots_gen   = smem_gen + (slots - smem_base);
+                        const uint32_t rbars = smem_base + L.total + 16u * (warp - 6);
+                        if(epi.step == 64)
+                            ok = fused_tile<64>(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, slots, slots_gen, rbars, abort_f, lane, uc, release_acc);
+                        else
+                            ok = fused_tile<32>(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, slots, slots_gen, rbars, abort_f, lane, uc, release_acc);
+                    }
+                }
+                else if(EPI == 0 && prm.out_mode >= OUT_E2M1)
                 {
                     // Re-quantising epilogue (row-major output, no K split, tile width a multiple of 128): the thread's row
                     // goes out 128 columns at a time.  e4m3 + UE8M0: the block's maximum first (one pass over the TMEM
@@ -1252,7 +1304,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                     }
                     release_acc();
                 }
-                else if(!split && prm.tma_store == 2)
+                else if(EPI == 0 && !split && prm.tma_store == 2)
                 {
                     // Wide path (row-major output, tile width a multiple of 64): 64 columns per step, so that the
                     // one warp per scheduler that runs this code has long runs of independent instructions: one
@@ -1411,6 +1463,13 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         // before anything ordered after the grid runs), and waiting would add the store's full latency to the kernel's tail
         if(use_tma && lane == 0)
             bulk_wait_group_read<0>();
+        if constexpr(EPI != 0)
+            if(*abort_f && epi.res_tma != 0 && lane == 0)
+            {
+                // residual tiles still in flight land before this CTA's shared memory is released (bounded, as the producers')
+                const uint64_t t0 = global_timer_ns();
+                while(global_timer_ns() - t0 < 200000ull) {}
+            }
         B200_TRACE(if(warp == 6 && lane == 0) stamp(62);)
         B200_TRACE(if(lane == 0) stamp(43 + (warp - 6));)
         tc_fence_before_sync();

@@ -162,6 +162,16 @@ struct DeviceState
 };
 
 static std::mutex g_mutex;
+// Held from a re-layout pass to the launch of the GEMM that reads its buffer: another host thread on the same stream must not
+// put its own pass in between.
+static std::mutex g_prepass_mutex;
+
+static bool is_capturing(cudaStream_t stream)
+{
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaStreamIsCapturing(stream, &cap);
+    return cap != cudaStreamCaptureStatusNone;
+}
 static std::map<int, DeviceState> g_devices;
 static std::atomic<unsigned long long> g_launches{0};
 
@@ -554,11 +564,12 @@ static void raise_smem_limit(Kernel kernel, bool (&attr_done)[64])
     }
 }
 
-template <int KIND, int SFW, int CG>
+template <int KIND, int SFW, int CG, int EPI>
 static void launch_persistent(int ctas, size_t smem, cudaStream_t stream, const CUtensorMap& mp, const CUtensorMap& mq,
-                              const CUtensorMap& msp, const CUtensorMap& msq, const CUtensorMap& mo, const PersistentParams& prm)
+                              const CUtensorMap& msp, const CUtensorMap& msq, const CUtensorMap& mo, const PersistentParams& prm,
+                              const EpilogueParams<EPI>& epi)
 {
-    auto kernel = gemm_persistent_kernel<KIND, SFW, CG>;
+    auto kernel = gemm_persistent_kernel<KIND, SFW, CG, EPI>;
     static bool attr_done[64] = {};
     raise_smem_limit(kernel, attr_done);
     cudaLaunchConfig_t lc{};
@@ -577,19 +588,19 @@ static void launch_persistent(int ctas, size_t smem, cudaStream_t stream, const 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs    = attr;
     lc.numAttrs = pdl_disabled() ? 1 : 2;
-    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, mp, mq, msp, msq, mo, prm));
+    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, mp, mq, msp, msq, mo, prm, epi));
     g_launches.fetch_add(1);
 }
 
-template <int KIND, int SFW>
+template <int KIND, int SFW, int EPI = 0>
 static void launch_persistent_cg(int cg, int ctas, size_t smem, cudaStream_t stream, const CUtensorMap& mp,
                                  const CUtensorMap& mq, const CUtensorMap& msp, const CUtensorMap& msq,
-                                 const CUtensorMap& mo, const PersistentParams& prm)
+                                 const CUtensorMap& mo, const PersistentParams& prm, const EpilogueParams<EPI>& epi = {})
 {
     if(cg == 2)
-        launch_persistent<KIND, SFW, 2>(ctas, smem, stream, mp, mq, msp, msq, mo, prm);
+        launch_persistent<KIND, SFW, 2, EPI>(ctas, smem, stream, mp, mq, msp, msq, mo, prm, epi);
     else
-        launch_persistent<KIND, SFW, 1>(ctas, smem, stream, mp, mq, msp, msq, mo, prm);
+        launch_persistent<KIND, SFW, 1, EPI>(ctas, smem, stream, mp, mq, msp, msq, mo, prm, epi);
 }
 
 static bool cluster_split_disabled()
@@ -706,6 +717,8 @@ static bool decode_mixed_disabled()
     return off;
 }
 
+constexpr int kFusedBarrierBytes = 128; // the residual barriers behind the persistent kernel's shared memory (fused epilogue)
+
 constexpr uint32_t kDecodeBarrierBytes = 256; // the decode kernel's barriers and flags (gemm_decode.cuh)
 
 struct DecodeLayout
@@ -739,11 +752,12 @@ static DecodeLayout make_decode_layout(int bn, int stages, int csplit, int scale
     return L;
 }
 
-template <int KIND, int SFW>
+template <int KIND, int SFW, int EPI = 0>
 static void launch_decode_instance(int ctas, int tiles_q, int csplit, size_t smem, cudaStream_t stream, const CUtensorMap& mp, const CUtensorMap& mq,
-                                   const CUtensorMap& msp, const CUtensorMap& msq, const CUtensorMap& mo, const DecodeParams& prm)
+                                   const CUtensorMap& msp, const CUtensorMap& msq, const CUtensorMap& mo, const DecodeParams& prm,
+                                   const EpilogueParams<EPI>& epi = {})
 {
-    auto kernel = gemm_decode_kernel<KIND, SFW>;
+    auto kernel = gemm_decode_kernel<KIND, SFW, EPI>;
     static bool attr_done[64] = {};
     {
         int dev = 0;
@@ -766,8 +780,26 @@ static void launch_decode_instance(int ctas, int tiles_q, int csplit, size_t sme
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs    = attr;
     lc.numAttrs = pdl_disabled() ? 1 : 2;
-    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, mp, mq, msp, msq, mo, prm));
+    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, mp, mq, msp, msq, mo, prm, epi));
     g_launches.fetch_add(1);
+}
+
+// What both kernels need of a fused epilogue; the residual's tensor map is filled in by the persistent launch.
+static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
+{
+    EpilogueParams<1> e{};
+    e.bias      = prob.fused_bias;
+    e.bias_mode = prob.fused_bias_mode;
+    e.bias_vec  = (reinterpret_cast<uintptr_t>(prob.fused_bias) & 15) == 0;
+    e.res       = prob.residual;
+    e.res_ld    = prob.residual_ld;
+    e.res_mode  = prob.residual_mode;
+    e.res_vec   = (reinterpret_cast<uintptr_t>(prob.residual) & 15) == 0 && (prob.residual_ld * (prob.residual_mode == OUT_F32 ? 4 : 2)) % 16 == 0;
+    e.act       = prob.activation;
+    e.out_mode  = prob.out_mode;
+    e.step      = 64;
+    e.slot_bytes = 4096;
+    return e;
 }
 
 // Launches the decode kernel if the problem and configuration fit it; returns false otherwise (the persistent kernel
@@ -781,7 +813,7 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
     const int tiles_q = static_cast<int>((prob.M + cfg.bn - 1) / std::max(cfg.bn, 1));
     if(decode_kernel_disabled() || !cfg.swap || cfg.cg != 1 || cfg.bn > 128 || cfg.bn % 16 != 0 || (cfg.bn > 64 && cfg.bn != 128) ||
        (tiles_q > 1 && (cfg.bn < 64 || tiles_q * cfg.bn > 256)) || (cfg.bn == 128 && named_stages > 4) || prob.scratch != nullptr ||
-       prob.out_mode != OUT_BF16 || prob.batch > 1 || prob.noscale)
+       (prob.out_mode != OUT_BF16 && !(prob.fused && prob.out_mode <= OUT_F32)) || prob.batch > 1 || prob.noscale)
         return false;
     const bool mixed = (kkind == KIND_MXF8F4);
     if(mixed && decode_mixed_disabled())
@@ -891,8 +923,16 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
         cols <<= 1;
     prm.tmem_cols = cols;
     CUtensorMap mo = mp;
-    prm.tma_store  = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % 8 == 0) ? 1 : 0;
-    if(prm.tma_store)
+    const bool out32 = (prob.out_mode == OUT_F32); // (fused epilogue only)
+    prm.tma_store  = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % (out32 ? 4 : 8) == 0) && (!out32 || bn <= 64) ? (out32 ? 2 : 1) : 0;
+    if(prm.tma_store == 2)
+    {
+        const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 4, static_cast<cuuint64_t>(prob.M)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * 4};
+        const cuuint32_t box[2]     = {128u, static_cast<cuuint32_t>(bn)};
+        mo = encode_map(prob.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "output");
+    }
+    else if(prm.tma_store)
     {
         // bf16 [M][N] seen as bytes; a warp's box is its 32 output columns by the tile's bn rows
         const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 2, static_cast<cuuint64_t>(prob.M)};
@@ -903,7 +943,19 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
     const int tiles_p = static_cast<int>((P.rows + kTileP - 1) / kTileP);
     const int ctas    = tiles_p * csplit;
     const size_t smem = L.total + 1024;
-    if(kkind == KIND_BF16)
+    if(prob.fused)
+    {
+        const EpilogueParams<1> epi = epilogue_params(prob);
+        if(kkind == KIND_BF16)
+            launch_decode_instance<KIND_BF16, SFW_NONE, 1>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
+            launch_decode_instance<KIND_MXF8, SFW_G1250, 1>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else if(kkind == KIND_MXF4 && sfw == SFW_E8M0_SHUFFLE)
+            launch_decode_instance<KIND_MXF4, SFW_E8M0_SHUFFLE, 1>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else
+            fail("no fused decode kernel for kind ", kkind, " with scale layout ", sfw);
+    }
+    else if(kkind == KIND_BF16)
         launch_decode_instance<KIND_BF16, SFW_NONE>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm);
     else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
         launch_decode_instance<KIND_MXF8, SFW_G1250>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm);
@@ -935,8 +987,10 @@ void launch_gemm(const GemmProblem& prob)
         return; // no activation rows: nothing to compute, the (empty) output is already complete
     if(prob.kind == PK_MXFP4 && prob.M >= kScalePrepassMinM && prob.scratch == nullptr && prob.act_sf.wire == SFW_E8M0_SHUFFLE &&
        prob.wgt_sf.wire == SFW_E8M0_SHUFFLE && prob.K % 256 == 0 && prob.K >= (tall_problem(prob.M, prob.N) ? 1024 : kScalePrepassMinK) &&
-       !relay_prepass_disabled())
+       !relay_prepass_disabled() && !(prob.fused && is_capturing(prob.stream)))
     {
+        // (the fused epilogue stays off the shared buffer inside a capture: two graphs captured on one stream would both hold it)
+        std::lock_guard<std::mutex> prepass(g_prepass_mutex);
         int prev_dev = 0;
         B200_CUDA(cudaGetDevice(&prev_dev));
         if(prev_dev != prob.device)
@@ -1005,6 +1059,7 @@ void launch_gemm(const GemmProblem& prob)
     if(prob.kind == PK_MXF8F4 && prob.M >= kWidenPrepassMinM && prob.scratch == nullptr && prob.wgt.mode == OPM_TILE16 &&
        prob.N % 16 == 0 && prob.K % 64 == 0 && !widen_prepass_disabled())
     {
+        std::lock_guard<std::mutex> prepass(g_prepass_mutex);
         int prev_dev = 0;
         B200_CUDA(cudaGetDevice(&prev_dev));
         if(prev_dev != prob.device)
@@ -1121,6 +1176,9 @@ static void launch_gemm_locked(const GemmProblem& prob)
     B200_CHECK(prob.batch == 1 || (prob.kind == PK_BF16 && prob.act.mode == OPM_BATCHED && prob.wgt.mode == OPM_BATCHED),
                "internal: batched launches are built for row-major bf16 operands");
     choose_config(prob.kind, prob.M, prob.N, prob.K, st.sm_count, cfg);
+    // the fused epilogue splits K inside a cluster only: no partial sums in memory that two captured graphs would share
+    if(prob.fused && !(cfg.swap && cfg.cg == 1))
+        cfg.log2_splitk = 0;
     B200_CHECK(cfg.log2_splitk >= 0 && cfg.log2_splitk <= 8, "log2 of the K split must be between 0 and 8 (got ", cfg.log2_splitk, ")");
     {
         bool ok = false;
@@ -1158,18 +1216,36 @@ static void launch_gemm_locked(const GemmProblem& prob)
     // the output leaves through shared memory and TMA tile stores when its pitch and base allow a tensor map
     const bool tma_store = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % 8 == 0) && (cfg.swap || cfg.bn >= 32) &&
                            (prob.out_mode == OUT_BF16 || prob.out_mode == OUT_F16) && prob.batch == 1;
+    // fused epilogue through its slots: row-major output and residual whose pitches and bases allow tensor maps
+    EpilogueParams<1> epi = epilogue_params(prob);
+    const bool slots      = prob.fused && !cfg.swap && cfg.bn % 64 == 0 && prob.batch == 1 && (reinterpret_cast<uintptr_t>(prob.out) & 15) == 0 &&
+                       (prob.ldo * (prob.out_mode == OUT_F32 ? 4 : 2)) % 16 == 0 && (prob.residual == nullptr || epi.res_vec);
+    int epi_units = tma_store ? 1 : 0;
+    if(slots)
+    {
+        epi.res_tma        = prob.residual != nullptr;
+        const bool wide    = prob.out_mode == OUT_F32 || (epi.res_tma && prob.residual_mode == OUT_F32);
+        const bool unequal = epi.res_tma && (prob.out_mode == OUT_F32) != (prob.residual_mode == OUT_F32);
+        epi.step       = wide ? 32 : 64;
+        epi.slot_bytes = unequal ? 8192 : 4096;
+        epi.out_off    = unequal ? 4096 : 0;
+        epi_units      = unequal ? 4 : 2;
+    }
     // Decode shapes: the K split runs across the CTAs of a thread-block cluster, one output tile per cluster; the
     // partial accumulators meet in the first CTA's shared memory instead of a global workspace.
     int csplit = 1;
     // (only with the weights on the 128-row slot: for row-major tiles, whose partial tiles are wide, it was measured two to
     // five times slower than the workspace split)
+    const int smem_limit = st.smem_optin - (prob.fused ? kFusedBarrierBytes : 0);
     if(cfg.swap && cg == 1 && splits > 1 && splits <= 8 && prob.scratch == nullptr && !cluster_split_disabled() &&
-       max_stages(cfg.bn, cg, st.smem_optin, f4_operand, sf_unit, tma_store, splits) >= 4)
+       max_stages(cfg.bn, cg, smem_limit, f4_operand, sf_unit, tma_store, splits) >= 4)
     {
         csplit = splits;
         splits = 1;
     }
-    const int max_st = max_stages(cfg.bn, cg, st.smem_optin, f4_operand, sf_unit, tma_store, csplit);
+    if(prob.fused)
+        splits = 1;
+    const int max_st = max_stages(cfg.bn, cg, smem_limit, f4_operand, sf_unit, epi_units, csplit);
     B200_CHECK(max_st >= 2, "tile ", 128 * cg, "x", cfg.bn, " does not fit in shared memory");
     int stages = cfg.stages <= 0 ? max_st : std::min(cfg.stages, max_st);
 
@@ -1319,10 +1395,16 @@ static void launch_gemm_locked(const GemmProblem& prob)
     prm.tma_store          = tma_store ? (wide_store ? 2 : 1) : 0;
     // the wide stores get a second staging buffer where that costs no pipeline stage
     prm.epi_bufs = tma_store ? 1 : 0;
-    if(wide_store && static_cast<int>(make_persistent_smem(cfg.bn, cg, stages, f4_operand, sf_unit, 2, csplit).total) + 1024 <= st.smem_optin)
+    if(prob.fused)
+    {
+        // (3: the slot path; otherwise 32 columns per store, or plain stores)
+        prm.tma_store = slots ? 3 : (tma_store ? 1 : 0);
+        prm.epi_bufs  = epi_units;
+    }
+    else if(wide_store && static_cast<int>(make_persistent_smem(cfg.bn, cg, stages, f4_operand, sf_unit, 2, csplit).total) + 1024 <= st.smem_optin)
         prm.epi_bufs = 2;
     const PersistentSmem L = make_persistent_smem(cfg.bn, cg, stages, f4_operand, sf_unit, prm.epi_bufs, csplit);
-    const size_t smem      = L.total + 1024;
+    const size_t smem      = L.total + 1024 + (prob.fused ? kFusedBarrierBytes : 0);
     // Tile order.  When the Q operand (the weights of a tall problem) is much larger than what L2 keeps beside the
     // streaming P operand and the output, walk it in panels of about 32 MB.
     prm.panel_q = 0;
@@ -1339,18 +1421,46 @@ static void launch_gemm_locked(const GemmProblem& prob)
         }
     }
     CUtensorMap mo         = mp;
-    if(tma_store)
+    if(slots)
+    {
+        // 32 rows of one step; rows of 128 bytes, or 64 where 32 columns of a 16-bit type meet a 32-bit one
+        auto rows_map = [&](const void* base, long long ld, int mode, const char* what) {
+            const int esize             = mode == OUT_F32 ? 4 : 2;
+            const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * esize, static_cast<cuuint64_t>(prob.M)};
+            const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esize};
+            const cuuint32_t box[2]     = {static_cast<cuuint32_t>(epi.step * esize), 32u};
+            return encode_map(base, 2, dims, strides, box, box[0] == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, what);
+        };
+        mo = rows_map(prob.out, prob.ldo, prob.out_mode, "output");
+        if(epi.res_tma)
+            epi.map_res = rows_map(prob.residual, prob.residual_ld, prob.residual_mode, "residual");
+    }
+    else if(tma_store)
     {
         // bf16 [M][N] seen as bytes; one box = 32 values of the fast dimension by 32 rows (or the tile's chunk of rows
         // when the 128-row slot holds the weights and the store is transposed)
         const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 2, static_cast<cuuint64_t>(prob.M)};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * 2};
-        const cuuint32_t box[2]     = {wide_store ? 128u : 64u, static_cast<cuuint32_t>(cfg.swap ? (cfg.bn < 32 ? 16 : 32) : 32)};
+        const bool wide_box         = wide_store && !prob.fused;
+        const cuuint32_t box[2]     = {wide_box ? 128u : 64u, static_cast<cuuint32_t>(cfg.swap ? (cfg.bn < 32 ? 16 : 32) : 32)};
         mo = encode_map(prob.out, 2, dims, strides, box,
-                        cfg.swap ? CU_TENSOR_MAP_SWIZZLE_NONE : (wide_store ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B), "output");
+                        cfg.swap ? CU_TENSOR_MAP_SWIZZLE_NONE : (wide_box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B), "output");
     }
     const int ctas         = clusters * cg * csplit;
-    if(kkind == KIND_BF16)
+    if(prob.fused)
+    {
+        if(kkind == KIND_BF16)
+            launch_persistent_cg<KIND_BF16, SFW_NONE, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
+            launch_persistent_cg<KIND_MXF8, SFW_G1250, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else if(kkind == KIND_MXF4 && sfw == SFW_E8M0_SHUFFLE)
+            launch_persistent_cg<KIND_MXF4, SFW_E8M0_SHUFFLE, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else if(kkind == KIND_MXF4 && sfw == SFW_G1250)
+            launch_persistent_cg<KIND_MXF4, SFW_G1250, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+        else
+            fail("no fused kernel instance for kind ", kkind, " with scale layout ", sfw);
+    }
+    else if(kkind == KIND_BF16)
         launch_persistent_cg<KIND_BF16, SFW_NONE>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm);
     else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
         launch_persistent_cg<KIND_MXF8, SFW_G1250>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm);

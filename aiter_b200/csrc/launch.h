@@ -98,6 +98,14 @@ struct GemmProblem
     const void* bias = nullptr; // indexed by n
     int bias_is_bf16 = 0;
     float alpha = 1.f, beta = 1.f;
+    // fused epilogue: out = act(alpha A B^T + fused_bias) + residual
+    bool fused = false;
+    int activation = 0;               // Activation
+    const void* fused_bias = nullptr; // indexed by n; fused_bias_mode: OutMode of its type
+    int fused_bias_mode = 0;
+    const void* residual = nullptr;   // [M, N], residual_ld elements between rows, OutMode of its type
+    long long residual_ld = 0;
+    int residual_mode = 0;
     int device = 0;
     cudaStream_t stream = nullptr;
     KernelConfig cfg;

@@ -210,6 +210,21 @@ AITER_B200_API int dynamic_per_group_scaled_quant(aiter_tensor_t* out, aiter_ten
                                                   int group_size, int shuffle_scale, aiter_tensor_t* num_rows,
                                                   int num_rows_factor, void* stream);
 
+/* ---- GEMMs with a fused epilogue: out = act(A B^T + bias) + residual, fp32 up to one rounding at the end.  No counterpart of this
+ * form in the reference (its Triton gemm_a16w16 takes a bias and an activation).  Operands as for gemm_a16w16_asm,
+ * mxfp8_mxfp8_gemm_asm and gemm_a4w4_asm.  bias [N] and residual [M, N]: bf16 / fp16 / fp32 or NULL; out [M, N] bf16 / fp16 /
+ * fp32; out may be residual itself (same type and strides), else they must not overlap.  activation: 0 none, 1 relu, 2 silu,
+ * 3 gelu (erf), 4 gelu_tanh.  No per-stream workspace is used inside a stream capture. */
+AITER_B200_API int aiter_b200_gemm_a16w16_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* bias, aiter_tensor_t* residual,
+                                                aiter_tensor_t* out, int activation, int bpreshuffle, const char* kernelName,
+                                                void* stream);
+AITER_B200_API int aiter_b200_gemm_a8w8_mxfp8_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* ScaleA, aiter_tensor_t* ScaleB,
+                                                    aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
+                                                    int a_preshuffle, const char* kernelName, void* stream);
+AITER_B200_API int aiter_b200_gemm_a4w4_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* A_scale, aiter_tensor_t* B_scale,
+                                              aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
+                                              int bpreshuffle, const char* kernelName, void* stream);
+
 /* ---- what stands between two GEMMs of a transformer block, one launch each.  No counterpart of this form in the reference
  * (its closest: rmsnorm2d_fwd_with_add / layernorm2d_fwd_with_add, silu_and_mul / gelu_and_mul / gelu_tanh_and_mul).
  *   u = x, or with post_norm != 0  norm(x) * post_weight + post_bias

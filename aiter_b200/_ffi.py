@@ -70,6 +70,7 @@ _lib.aiter_get_last_error.restype = ctypes.c_char_p
 _lib.aiter_b200_kernel_list.restype = ctypes.c_char_p
 _lib.aiter_b200_heuristic_name.restype = ctypes.c_char_p
 _lib.aiter_b200_launch_count.restype = ctypes.c_ulonglong
+_lib.aiter_b200_gemm_a4w4_fused_workspace.restype = ctypes.c_longlong
 assert _lib.aiter_ctypes_abi_version() == 2
 
 T, I, S, F = "tensor", "int", "str", "float"
@@ -101,7 +102,7 @@ SIGNATURES = {
     "aiter_b200_gemm_a8w8_mxfp8_noalloc": (T, T, T, T, T, I, I),
     "aiter_b200_gemm_a16w16_fused": (T, T, T, T, T, I, I, S),
     "aiter_b200_gemm_a8w8_mxfp8_fused": (T, T, T, T, T, T, T, I, I, S),
-    "aiter_b200_gemm_a4w4_fused": (T, T, T, T, T, T, T, I, I, S),
+    "aiter_b200_gemm_a4w4_fused": (T, T, T, T, T, T, T, T, I, I, S),
     "aiter_b200_gated_residual_norm": (T, T, T, T, T, T, T, T, T, T, F, F, F, I, I, I),
     "aiter_b200_act_and_mul": (T, T, T, I, I),
 }
@@ -110,7 +111,7 @@ EXPORTS = sorted(
     + ["getPaddedM", "aiter_ctypes_abi_version", "aiter_get_last_error", "aiter_clear_last_error",
        "opus_gemm_workspace_init", "aiter_b200_device_status", "aiter_b200_kernel_list",
        "aiter_b200_heuristic_name", "aiter_b200_launch_count", "aiter_b200_noalloc_status",
-       "aiter_b200_debug_wait_control"]
+       "aiter_b200_debug_wait_control", "aiter_b200_gemm_a4w4_fused_workspace"]
 )
 
 
@@ -215,6 +216,10 @@ def debug_wait_control(device: int = 0, limit_ns: int = 1_000_000_000, withhold_
     if rc != 0:
         msg = _lib.aiter_get_last_error()
         raise RuntimeError(f"aiter_b200_debug_wait_control failed: {msg.decode() if msg else ''}")
+
+
+def fused_workspace_bytes(M: int, N: int, K: int) -> int:
+    return int(_lib.aiter_b200_gemm_a4w4_fused_workspace(int(M), int(N), int(K)))
 
 
 def kernel_list() -> str:

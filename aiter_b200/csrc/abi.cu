@@ -69,6 +69,7 @@ struct FusedArgs
     const aiter_tensor_t* bias;
     const aiter_tensor_t* residual;
     int activation;
+    const aiter_tensor_t* workspace = nullptr; // dense bytes
 };
 
 static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_tensor_t* out, const FusedArgs& f, const char* fn)
@@ -85,6 +86,16 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
     p.ldo        = M == 1 ? (N + 7) / 8 * 8 : out->strides[0]; // (one row: any pitch, and one that allows a tensor map)
     p.fused      = true;
     p.activation = f.activation;
+    if(f.workspace != nullptr)
+    {
+        require_tensor(f.workspace, fn, "workspace", 1);
+        B200_CHECK(is_byte_dtype(f.workspace->dtype_), fn, ": workspace must be a uint8 tensor");
+        require_rows_contiguous(f.workspace, fn, "workspace");
+        require_same_device(first, f.workspace, fn, "workspace");
+        B200_CHECK((reinterpret_cast<uintptr_t>(f.workspace->ptr) & 15) == 0, fn, ": workspace must be 16-byte aligned");
+        p.workspace       = f.workspace->ptr;
+        p.workspace_bytes = f.workspace->numel_;
+    }
     if(f.bias != nullptr)
     {
         require_tensor(f.bias, fn, "bias", 1);
@@ -591,17 +602,19 @@ extern "C" int aiter_b200_gemm_a8w8_mxfp8_fused(aiter_tensor_t* A, aiter_tensor_
 }
 
 extern "C" int aiter_b200_gemm_a4w4_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* A_scale, aiter_tensor_t* B_scale,
-                                          aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
-                                          int bpreshuffle, const char* kernelName, void* stream)
+                                          aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, aiter_tensor_t* workspace,
+                                          int activation, int bpreshuffle, const char* kernelName, void* stream)
 {
     return safe_call([&] {
         const char* fn = "aiter_b200_gemm_a4w4_fused";
         GemmProblem tmp;
         apply_config(tmp, kernelName, -1, fn);
-        const FusedArgs f{bias, residual, activation};
+        const FusedArgs f{bias, residual, activation, workspace};
         run_mxfp4(fn, A, B, A_scale, B_scale, out, nullptr, 1.f, 0.f, OPM_ROWMAJOR, bpreshuffle ? OPM_TILE16 : OPM_ROWMAJOR, SFW_E8M0_SHUFFLE, tmp.cfg, stream, &f);
     });
 }
+
+extern "C" long long aiter_b200_gemm_a4w4_fused_workspace(int M, int N, int K) { return static_cast<long long>(fused_workspace_bytes(M, N, K)); }
 
 extern "C" int gemm_a16w16_asm(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* out, aiter_tensor_t* semaphore,
                                aiter_tensor_t* bias, int splitK, const char* kernelName, int bpreshuffle, void* stream)

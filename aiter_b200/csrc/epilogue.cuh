@@ -1,10 +1,12 @@
 // Fused GEMM epilogue: out = act(A B^T + bias) + residual on the fp32 accumulator, rounded once.
 //
-// Row-major output tiles (activations on the 128-row slot) leave in steps of 64 columns (32 where a 32-bit type is
-// involved).  Every epilogue warp owns two slots in shared memory: the residual's tile of a step is loaded into a slot by
-// TMA, read by the lanes (one row each, 128-byte swizzle), the finished row is written back into the same slot and leaves
-// as a TMA tile store.  The loads of a tile's first two steps are issued before the accumulator is waited for and the
-// remaining steps are prefetched into L2, so with a second accumulator the residual costs its bytes and no latency.
+// Row-major output tiles (activations on the 128-row slot) leave in steps of 32 columns, and EIGHT warps share them, two per
+// TMEM lane quarter on alternating steps: an activation costs about 20 issue slots a value, a scheduler runs one warp of a
+// quarter, and the accumulator of an MX tile 256 columns wide has no second one to hide behind.  Every epilogue warp owns two
+// slots in shared memory: the residual's tile of a step is loaded into a slot by TMA, read by the lanes (one row each,
+// swizzled), the finished rows are written back into the same slot and leave as a TMA tile store.  The loads of a warp's first
+// two steps and its bias values are requested before the accumulator is waited for and the remaining residual tiles are
+// prefetched into L2.
 #pragma once
 #include "activation.cuh"
 #include "gemm_common.cuh"
@@ -21,7 +23,6 @@ struct alignas(64) EpilogueParams<1>
     CUtensorMap map_res;
     const void* bias; // [N]
     int bias_mode;    // OutMode of the bias' type
-    int bias_vec;     // 16-byte loads of 8 (4 for fp32) consecutive values are aligned
     const void* res;  // [M, N]
     long long res_ld;
     int res_mode;
@@ -29,10 +30,13 @@ struct alignas(64) EpilogueParams<1>
     int res_tma;      // residual tiles come through map_res
     int act;
     int out_mode;
-    int step;             // columns per step of the slot path
-    uint32_t slot_bytes;  // 4096, or 8192 where residual and output differ in size (the output then has the upper half)
-    uint32_t out_off;
+    uint32_t slot_bytes;  // 32 rows x 32 columns of the wider of residual and output: 2048 or 4096
 };
+
+constexpr int kFusedStep      = 32;
+constexpr int kFusedWarps     = 8;
+constexpr int kFusedBarBytes  = 16 * kFusedWarps;       // two residual barriers per epilogue warp
+constexpr int kFusedBiasBytes = 4 * 128 * kFusedWarps;  // a warp's bias values of one tile (at most 128 columns), fp32
 
 // (plain loads throughout: the residual may be the output itself, and it or the bias may come from the kernel just before, which
 // this one may overlap up to its dependency wait - the read-only path is for memory that nothing writes meanwhile)
@@ -61,138 +65,119 @@ __device__ __forceinline__ void add16x2(float& a, float& b, uint32_t w, bool f16
         b += __uint_as_float(w & 0xFFFF0000u);
     }
 }
-// v[0 .. N) += N consecutive elements from `at`, of which `valid` exist.
-template <int N>
-__device__ __forceinline__ void add_row(float (&v)[N], const void* base, int mode, size_t at, int valid, bool vec)
+// What an epilogue warp needs of the slot path: `seq` counts its steps over all tiles (slot = seq & 1).
+struct FusedWarp
 {
-    if(vec && valid >= N)
-    {
-        if(mode == OUT_F32)
-        {
-#pragma unroll
-            for(int i = 0; i < N; i += 4)
-            {
-                const float4 t = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + i);
-                v[i] += t.x;
-                v[i + 1] += t.y;
-                v[i + 2] += t.z;
-                v[i + 3] += t.w;
-            }
-        }
-        else
-        {
-#pragma unroll
-            for(int i = 0; i < N; i += 8)
-            {
-                const uint4 t = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at + i);
-                add16x2(v[i], v[i + 1], t.x, mode == OUT_F16);
-                add16x2(v[i + 2], v[i + 3], t.y, mode == OUT_F16);
-                add16x2(v[i + 4], v[i + 5], t.z, mode == OUT_F16);
-                add16x2(v[i + 6], v[i + 7], t.w, mode == OUT_F16);
-            }
-        }
-    }
-    else
-    {
-#pragma unroll
-        for(int i = 0; i < N; ++i)
-            if(i < valid)
-                v[i] += mode == OUT_F32 ? static_cast<const float*>(base)[at + i] : raw_to_f32(static_cast<const uint16_t*>(base)[at + i], mode);
-    }
-}
-
-// A warp's position in its ring: the number of steps done so far over all tiles (slot = seq & 1).
-struct FusedStore
-{
-    uint32_t seq = 0;
+    uint32_t seq;
+    uint32_t slots, rbars;  // shared-memory addresses of the two slots and their barriers
+    uint8_t* slots_gen;
+    float* bias;            // this warp's bias values of the current tile
+    int group;              // 0 or 1: the steps it takes
 };
 
-__device__ __forceinline__ uint32_t epi_s_fused(uint32_t smem_base, uint32_t epi_off, int w, const EpilogueParams<1>& epi)
+__device__ __forceinline__ void fused_load(const FusedWarp& f, const EpilogueParams<1>& epi, uint32_t seq, int row0, int col0)
 {
-    return smem_base + epi_off + static_cast<uint32_t>(w) * 2u * epi.slot_bytes;
+    const uint32_t esize = epi.res_mode == OUT_F32 ? 4u : 2u;
+    const uint32_t bar   = f.rbars + 8u * (seq & 1);
+    mbar_arrive_expect_tx(bar, 32u * kFusedStep * esize);
+    tma_load_2d(f.slots + (seq & 1) * epi.slot_bytes, &epi.map_res, bar, col0 * static_cast<int>(esize), row0);
 }
 
-// residual bytes of one step: 32 rows of step columns
-__device__ __forceinline__ uint32_t fused_res_bytes(const EpilogueParams<1>& epi) { return 32u * static_cast<uint32_t>(epi.step) * (epi.res_mode == OUT_F32 ? 4u : 2u); }
-
-__device__ __forceinline__ void fused_load(const EpilogueParams<1>& epi, uint32_t seq, int row0, int col0, uint32_t slots, uint32_t rbars)
+// Before the accumulator of a tile is waited for.  row0, col0: first row of the warp's 32, first column of the tile.
+__device__ __forceinline__ void fused_begin(const FusedWarp& f, const EpilogueParams<1>& epi, int row0, int col0, int bn, int rows_q, int lane)
 {
-    const uint32_t bar = rbars + 8u * (seq & 1);
-    mbar_arrive_expect_tx(bar, fused_res_bytes(epi));
-    tma_load_2d(slots + (seq & 1) * epi.slot_bytes, &epi.map_res, bar, col0 * (epi.res_mode == OUT_F32 ? 4 : 2), row0);
+    const int steps = bn / kFusedStep;
+    if(epi.bias != nullptr)
+    {
+        for(int c = f.group; c < steps; c += 2)
+        {
+            const int q                            = col0 + c * kFusedStep + lane;
+            f.bias[(c >> 1) * kFusedStep + lane] = q < rows_q ? load_elem(epi.bias, epi.bias_mode, q) : 0.f;
+        }
+    }
+    if(epi.res_tma != 0 && lane == 0)
+    {
+        bulk_wait_group_read<0>(); // the slots' last stores have been read
+        uint32_t seq = f.seq;
+        for(int c = f.group, i = 0; c < steps; c += 2, ++i)
+        {
+            if(i < 2)
+                fused_load(f, epi, seq++, row0, col0 + c * kFusedStep);
+            else
+                tma_prefetch_l2_2d(&epi.map_res, (col0 + c * kFusedStep) * (epi.res_mode == OUT_F32 ? 4 : 2), row0);
+        }
+    }
+    __syncwarp();
 }
 
-// Before the accumulator of a tile is waited for: its first two residual tiles are requested (the slots' previous stores have
-// been read by then) and the others brought into L2.
-__device__ __forceinline__ void fused_begin(const FusedStore& f, const EpilogueParams<1>& epi, int row0, int col0, int bn, uint32_t slots, uint32_t rbars, int lane)
+// One warp's share of a tile.  Returns false when a wait ran out.
+template <typename Params, typename Release>
+__device__ __forceinline__ bool fused_tile(FusedWarp& f, const EpilogueParams<1>& epi, const Params& prm, const CUtensorMap* map_out, uint32_t tacc, int row0, int col0,
+                                           int bn, volatile uint32_t* abort_f, int lane, int uc, Release&& release_acc)
 {
-    if(epi.res_tma == 0 || lane != 0)
-        return;
-    bulk_wait_group_read<0>();
-    const int steps = bn / epi.step;
-    fused_load(epi, f.seq, row0, col0, slots, rbars);
-    if(steps > 1)
-        fused_load(epi, f.seq + 1, row0, col0 + epi.step, slots, rbars);
-    for(int i = 2; i < steps; ++i)
-        tma_prefetch_l2_2d(&epi.map_res, (col0 + i * epi.step) * (epi.res_mode == OUT_F32 ? 4 : 2), row0);
-}
-
-// One warp's 32 rows of a tile.  row0 / col0: first row and column of the warp's part.  Returns false when a wait ran out.
-template <int STEP, typename Params, typename Release>
-__device__ __forceinline__ bool fused_tile(FusedStore& f, const EpilogueParams<1>& epi, const Params& prm, const CUtensorMap* map_out, uint32_t tacc, int row0, int col0,
-                                           int bn, uint32_t slots, uint8_t* slots_gen, uint32_t rbars, volatile uint32_t* abort_f, int lane, int uc, Release&& release_acc)
-{
-    const int steps      = bn / STEP;
-    const bool out32     = epi.out_mode == OUT_F32;
-    const bool out_f16   = epi.out_mode == OUT_F16;
-    const int out_esize  = out32 ? 4 : 2;
-    for(int c = 0; c < steps; ++c, ++f.seq)
+    constexpr int STEP = kFusedStep;
+    const int steps    = bn / STEP;
+    const bool out32   = epi.out_mode == OUT_F32;
+    const bool out_f16 = epi.out_mode == OUT_F16;
+    if(f.group >= steps)
+        release_acc();
+    for(int c = f.group; c < steps; c += 2, ++f.seq)
     {
         float v[STEP];
         {
             uint32_t r[STEP];
-            if constexpr(STEP == 64)
-                tmem_ld_x64(tacc + c * 64, r);
-            else
-                tmem_ld_x32(tacc + c * 32, r);
+            tmem_ld_x32(tacc + c * STEP, r);
             tmem_ld_wait();
 #pragma unroll
             for(int j = 0; j < STEP; ++j)
                 v[j] = __uint_as_float(r[j]);
         }
-        if(c == steps - 1)
-            release_acc(); // every column of this accumulator is in registers now
+        if(c + 2 >= steps)
+            release_acc(); // every column that this warp reads is in registers now
         const int q_first = col0 + c * STEP;
         if(lane == 0)
         {
             if(epi.res_tma == 0)
                 bulk_wait_group_read<1>(); // the store that last used this slot has read it
-            else if(c > 0 && c + 1 < steps)
+            else if(c >= 2 && c + 2 < steps)
             {
                 // the previous step's store has read its slot: the residual tile of the next step goes there
                 bulk_wait_group_read<0>();
-                fused_load(epi, f.seq + 1, row0, q_first + STEP, slots, rbars);
+                fused_load(f, epi, f.seq + 1, row0, q_first + 2 * STEP);
             }
         }
         if(epi.bias != nullptr)
-            add_row<STEP>(v, epi.bias, epi.bias_mode, q_first, prm.rows_q - q_first, epi.bias_vec != 0);
+        {
+            const float4* b = reinterpret_cast<const float4*>(f.bias + (c >> 1) * STEP);
+#pragma unroll
+            for(int j = 0; j < STEP / 4; ++j)
+            {
+                const float4 t = b[j];
+                v[4 * j] += t.x;
+                v[4 * j + 1] += t.y;
+                v[4 * j + 2] += t.z;
+                v[4 * j + 3] += t.w;
+            }
+        }
         activate(v, epi.act);
         __syncwarp();
-        const uint32_t off = (f.seq & 1) * epi.slot_bytes;
+        uint8_t* slot = f.slots_gen + (f.seq & 1) * epi.slot_bytes;
+        // a lane's row: 128 bytes of fp32, or 64 of a 16-bit type, in 16-byte pieces swizzled against bank conflicts
+        uint8_t* row128 = slot + lane * 128;
+        uint8_t* row64  = slot + lane * 64;
+        const int x128 = lane & 7, x64 = (lane >> 1) & 3;
         if(epi.res_tma != 0)
         {
-            bool ok = bounded_wait(rbars + 8u * (f.seq & 1), (f.seq >> 1) & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, 0x4000 + uc);
+            bool ok = bounded_wait(f.rbars + 8u * (f.seq & 1), (f.seq >> 1) & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, 0x4000 + uc);
             ok      = __all_sync(0xffffffffu, ok);
             if(!ok)
                 return false;
-            const uint8_t* tile = slots_gen + off;
             if(epi.res_mode == OUT_F32)
             {
-                // 32 floats = 128 bytes a row (STEP is 32 whenever a 32-bit type is involved)
 #pragma unroll
                 for(int j = 0; j < STEP / 4; ++j)
                 {
-                    const float4 t = *reinterpret_cast<const float4*>(tile + lane * 128 + ((j ^ (lane & 7)) * 16));
+                    const float4 t = *reinterpret_cast<const float4*>(row128 + ((j ^ x128) * 16));
                     v[4 * j] += t.x;
                     v[4 * j + 1] += t.y;
                     v[4 * j + 2] += t.z;
@@ -204,40 +189,119 @@ __device__ __forceinline__ bool fused_tile(FusedStore& f, const EpilogueParams<1
 #pragma unroll
                 for(int j = 0; j < STEP / 8; ++j)
                 {
-                    const uint32_t at = STEP == 64 ? lane * 128 + ((j ^ (lane & 7)) * 16) : lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16);
-                    const uint4 t     = *reinterpret_cast<const uint4*>(tile + at);
+                    const uint4 t = *reinterpret_cast<const uint4*>(row64 + ((j ^ x64) * 16));
                     add16x2(v[8 * j], v[8 * j + 1], t.x, epi.res_mode == OUT_F16);
                     add16x2(v[8 * j + 2], v[8 * j + 3], t.y, epi.res_mode == OUT_F16);
                     add16x2(v[8 * j + 4], v[8 * j + 5], t.z, epi.res_mode == OUT_F16);
                     add16x2(v[8 * j + 6], v[8 * j + 7], t.w, epi.res_mode == OUT_F16);
                 }
             }
+            __syncwarp(); // (types of different sizes: a row of one covers rows of the other)
         }
-        // a lane overwrites only the row it has read; rows of different lanes do not overlap in either type
-        uint8_t* dst = slots_gen + off + epi.out_off;
         if(out32)
         {
 #pragma unroll
             for(int j = 0; j < STEP / 4; ++j)
-                *reinterpret_cast<float4*>(dst + lane * 128 + ((j ^ (lane & 7)) * 16)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                *reinterpret_cast<float4*>(row128 + ((j ^ x128) * 16)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
         }
         else
         {
 #pragma unroll
             for(int j = 0; j < STEP / 8; ++j)
-            {
-                const uint32_t at = STEP == 64 ? lane * 128 + ((j ^ (lane & 7)) * 16) : lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16);
-                *reinterpret_cast<uint4*>(dst + at) = make_uint4(pack_out16x2(v[8 * j], v[8 * j + 1], out_f16), pack_out16x2(v[8 * j + 2], v[8 * j + 3], out_f16),
-                                                                 pack_out16x2(v[8 * j + 4], v[8 * j + 5], out_f16), pack_out16x2(v[8 * j + 6], v[8 * j + 7], out_f16));
-            }
+                *reinterpret_cast<uint4*>(row64 + ((j ^ x64) * 16)) = make_uint4(pack_out16x2(v[8 * j], v[8 * j + 1], out_f16), pack_out16x2(v[8 * j + 2], v[8 * j + 3], out_f16),
+                                                                                  pack_out16x2(v[8 * j + 4], v[8 * j + 5], out_f16), pack_out16x2(v[8 * j + 6], v[8 * j + 7], out_f16));
         }
         fence_proxy_async_smem();
         __syncwarp();
         if(lane == 0 && row0 < prm.rows_p && q_first < prm.rows_q) // partly outside: the store clips
         {
-            tma_store_2d(map_out, slots + off + epi.out_off, q_first * out_esize, row0);
+            tma_store_2d(map_out, f.slots + (f.seq & 1) * epi.slot_bytes, q_first * (out32 ? 4 : 2), row0);
             bulk_commit_group();
         }
+    }
+    return true;
+}
+
+// Outputs or residuals whose rows allow no tile copies, and tiles with the weights on the 128-row slot (few rows, a K split over a
+// cluster, or rows that start on odd addresses: there the lanes run along the output's columns and plain accesses coalesce).
+// Sixteen columns of the accumulator at a time, alternating between the two warps of a quarter.  red / red_stride: the other K
+// slices' partial sums of this thread's row.
+template <typename Params, typename Release>
+__device__ __forceinline__ bool fused_plain_tile(const EpilogueParams<1>& epi, const Params& prm, uint32_t tacc, int p, int col0, int bn, int group, int csplit,
+                                                 const float* red, size_t red_stride, uint32_t red_bar, volatile uint32_t* abort_f, int uc, Release&& release_acc)
+{
+    const int groups = bn / 16;
+    const bool row_in = p < prm.rows_p, transposed = prm.transposed_out != 0;
+    const size_t res_step = transposed ? static_cast<size_t>(epi.res_ld) : 1u;
+    const float bias_p    = (epi.bias != nullptr && transposed && row_in) ? load_elem(epi.bias, epi.bias_mode, p) : 0.f;
+    if(group >= groups)
+        release_acc();
+#pragma unroll 1
+    for(int c = group; c < groups; c += 2)
+    {
+        const int q_first = col0 + c * 16;
+        const int valid   = row_in ? min(16, prm.rows_q - q_first) : 0;
+        uint32_t raw[16];
+        if(epi.res != nullptr)
+        {
+            const size_t at = transposed ? static_cast<size_t>(q_first) * epi.res_ld + p : static_cast<size_t>(p) * epi.res_ld + q_first;
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                raw[j] = j < valid ? load_elem_raw(epi.res, epi.res_mode, at + j * res_step) : 0u;
+        }
+        float v[16];
+        {
+            uint32_t r[16];
+            tmem_ld_x16_at(tacc + c * 16, r);
+            tmem_ld_wait();
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                v[j] = __uint_as_float(r[j]);
+        }
+        if(c + 2 >= groups)
+            release_acc(); // every column that this warp reads is in registers now
+        if(csplit > 1)
+        {
+            if(c == group)
+            {
+                bool ok = bounded_wait(red_bar, uc & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, 0x3000 + uc);
+                ok      = __all_sync(0xffffffffu, ok);
+                if(!ok)
+                    return false;
+            }
+            for(int z = 0; z < csplit - 1; ++z)
+            {
+                const float4* row = reinterpret_cast<const float4*>(red + z * red_stride + c * 16);
+#pragma unroll
+                for(int j = 0; j < 16; j += 4)
+                {
+                    const float4 t = row[j / 4];
+                    v[j] += t.x;
+                    v[j + 1] += t.y;
+                    v[j + 2] += t.z;
+                    v[j + 3] += t.w;
+                }
+            }
+        }
+        if(epi.bias != nullptr)
+        {
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                v[j] += transposed ? bias_p : (j < valid ? load_elem(epi.bias, epi.bias_mode, q_first + j) : 0.f);
+        }
+        activate(v, epi.act);
+        if(epi.res != nullptr)
+        {
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                v[j] += raw_to_f32(raw[j], epi.res_mode);
+        }
+        const size_t at       = transposed ? static_cast<size_t>(q_first) * prm.ldo + p : static_cast<size_t>(p) * prm.ldo + q_first;
+        const size_t out_step = transposed ? static_cast<size_t>(prm.ldo) : 1u;
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            if(j < valid)
+                store_out(prm.out, at + j * out_step, v[j], epi.out_mode);
     }
     return true;
 }

@@ -59,6 +59,142 @@ __host__ __device__ constexpr int decode_sf_unit(int kind) { return kind == KIND
 // (the mixed kind, e4m3 activations x packed e2m1 weights, is MXF8 once the scale warps have widened the weight tile to
 // e4m3 in shared memory: exact, every e2m1 value is an e4m3 value)
 
+// ---- fused epilogue (out = act(acc + bias) + residual): the thread holds one weight row = one output column, bn activation rows.
+// It goes over them 16 at a time in a rolled loop - a few KB of code whatever bn is, and no more activations than the tile has
+// rows (all 64 at once, unrolled, cost a one-row call 2 us of instruction fetches and 1 us of arithmetic on rows that do not
+// exist) - with the next 16 residual values in flight while these are finished.
+struct DecodeFused
+{
+    int p;
+    bool mine;         // this thread finishes column p (it exists, and its K slice owns it)
+    float bias;
+    uint32_t res[16];  // raw residual values of the next 16 rows
+};
+__device__ __forceinline__ void decode_load_residual(DecodeFused& f, const EpilogueParams<1>& epi, int row0, int rows)
+{
+    if(epi.res == nullptr)
+        return;
+#pragma unroll
+    for(int j = 0; j < 16; ++j)
+        f.res[j] = (f.mine && row0 + j < rows) ? load_elem_raw(epi.res, epi.res_mode, static_cast<size_t>(row0 + j) * epi.res_ld + f.p) : 0u;
+}
+__device__ __forceinline__ void decode_load_residual(const DecodeFused&, const EpilogueParams<0>&, int, int) {}
+
+__device__ __forceinline__ void decode_fused_epilogue(DecodeFused& f, const EpilogueParams<1>& epi, const DecodeParams& prm, const CUtensorMap* map_out, uint8_t* smem_gen,
+                                                      uint32_t smem_base, uint32_t red_bar, uint32_t tlane, int p_local, int p_warp0, int row_q0, uint32_t zrank,
+                                                      uint32_t per, volatile uint32_t* abort_f, int w, int lane)
+{
+    const int bn = prm.bn, csplit = prm.csplit;
+    const uint32_t owner = csplit > 1 ? static_cast<uint32_t>(p_local) / per : 0u;
+    const uint32_t prow  = static_cast<uint32_t>(p_local) - owner * per;
+    const bool owns      = csplit == 1 || owner == zrank; // (the same for the whole warp: slices own whole warps' rows)
+    if(!owns)
+    {
+        // partial sums to the CTA that owns this row: [source slice][row][bn floats], counted on its red barrier
+        const uint32_t src     = zrank < owner ? zrank : zrank - 1u;
+        const uint32_t dst_row = map_to_cta(smem_base + prm.red_off, owner) + (src * per + prow) * static_cast<uint32_t>(bn) * 4u;
+        const uint32_t dst_bar = map_to_cta(red_bar, owner);
+#pragma unroll 1
+        for(int c = 0; c < bn; c += 16)
+        {
+            uint32_t r[16];
+            tmem_ld_x16_at(tlane + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for(int j = 0; j < 16; j += 4)
+                st_async_v4(dst_row + static_cast<uint32_t>(c + j) * 4u, r[j], r[j + 1], r[j + 2], r[j + 3], dst_bar);
+        }
+        return;
+    }
+    if(csplit > 1)
+    {
+        bool ok = bounded_wait(red_bar, 0, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, 0x3000);
+        ok      = __all_sync(0xffffffffu, ok);
+        if(!ok)
+            return;
+    }
+    const bool out32    = epi.out_mode == OUT_F32;
+    // two staging buffers of 16 rows x 32 columns per warp in a retired operand stage (every tile load has landed and been consumed
+    // once the accumulator is complete)
+    const uint32_t buf0 = static_cast<uint32_t>(w) * 4096u;
+    uint32_t flip       = 0;
+    const int rows      = min(bn, prm.rows_q - row_q0);
+#pragma unroll 1
+    for(int c = 0; c < rows; c += 16)
+    {
+        float v[16];
+        {
+            uint32_t r[16];
+            tmem_ld_x16_at(tlane + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                v[j] = __uint_as_float(r[j]);
+        }
+        for(int z = 0; z < csplit - 1; ++z)
+        {
+            const float4* row = reinterpret_cast<const float4*>(smem_gen + prm.red_off) + (static_cast<size_t>(z * per + prow) * bn + c) / 4;
+#pragma unroll
+            for(int j = 0; j < 16; j += 4)
+            {
+                const float4 t = row[j / 4];
+                v[j] += t.x;
+                v[j + 1] += t.y;
+                v[j + 2] += t.z;
+                v[j + 3] += t.w;
+            }
+        }
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            v[j] += f.bias;
+        activate(v, epi.act);
+        if(epi.res != nullptr)
+        {
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                v[j] += raw_to_f32(f.res[j], epi.res_mode);
+            if(c + 16 < rows)
+                decode_load_residual(f, epi, row_q0 + c + 16, prm.rows_q);
+        }
+        if(prm.tma_store)
+        {
+            if(lane == 0)
+                bulk_wait_group_read<1>(); // the store before the last one, from this buffer, has read it
+            __syncwarp();
+            uint8_t* buf = smem_gen + buf0 + flip;
+            if(out32)
+            {
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                    reinterpret_cast<float*>(buf)[j * 32 + lane] = v[j];
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                    reinterpret_cast<uint16_t*>(buf)[j * 32 + lane] = cvt_out16(v[j], epi.out_mode == OUT_F16);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if(lane == 0 && p_warp0 < prm.rows_p)
+            {
+                tma_store_2d(map_out, smem_base + buf0 + flip, p_warp0 * (out32 ? 4 : 2), row_q0 + c);
+                bulk_commit_group();
+            }
+            flip ^= 2048u;
+        }
+        else if(f.p < prm.rows_p)
+        {
+#pragma unroll
+            for(int j = 0; j < 16; ++j)
+                if(c + j < rows)
+                    store_out(prm.out, static_cast<size_t>(row_q0 + c + j) * prm.ldo + f.p, v[j], epi.out_mode);
+        }
+    }
+    if(prm.tma_store && lane == 0)
+        bulk_wait_group_read<0>(); // the stores have read their source before the CTA retires
+}
+
 template <int KIND, int SFW, int EPI>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
@@ -324,23 +460,14 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         const uint32_t tlane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         bool ok = true;
         // (fused epilogue) this thread's bias and the residual of its first 16 rows: under way before the K loop ends
-        float bias0 = 0.f;
-        uint32_t res0[16];
+        DecodeFused fused{};
         if constexpr(EPI != 0)
         {
-            const int p0 = row_p0 + p_local;
-            if(p0 < prm.rows_p && (csplit == 1 || static_cast<uint32_t>(p_local) / per == zrank))
-            {
-                if(epi.bias != nullptr)
-                    bias0 = load_elem(epi.bias, epi.bias_mode, p0);
-                if(epi.res != nullptr)
-                {
-#pragma unroll
-                    for(int j = 0; j < 16; ++j)
-                        if(row_q0 + j < prm.rows_q)
-                            res0[j] = load_elem_raw(epi.res, epi.res_mode, static_cast<size_t>(row_q0 + j) * epi.res_ld + p0);
-                }
-            }
+            fused.p    = row_p0 + p_local;
+            fused.mine = fused.p < prm.rows_p && (csplit == 1 || static_cast<uint32_t>(p_local) / per == zrank);
+            if(fused.mine && epi.bias != nullptr)
+                fused.bias = load_elem(epi.bias, epi.bias_mode, fused.p);
+            decode_load_residual(fused, epi, row_q0, prm.rows_q);
         }
         if(kScaled)
         {
@@ -545,7 +672,16 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             ok = __all_sync(0xffffffffu, ok);
         }
         B200_TRACE(if(lane == 0) stamp(38 + (warp - 2));)
-        if(ok)
+        if constexpr(EPI != 0)
+        {
+            if(ok)
+            {
+                tc_fence_after_sync();
+                decode_fused_epilogue(fused, epi, prm, &map_out, smem_gen, smem_base, red_bar, tlane, p_local, row_p0 + quarter * 32, row_q0, zrank, per, abort_f,
+                                      warp - 2, lane);
+            }
+        }
+        else if(ok)
         {
             tc_fence_after_sync();
             // the thread's row goes out in chunks of at most 64 columns (one chunk unless bn = 128)
@@ -627,12 +763,6 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             if(ok && mine)
             {
                 const int p = row_p0 + p_local;
-                auto out16  = [&](float x) -> uint16_t {
-                    if constexpr(EPI != 0)
-                        return cvt_out16(x, epi.out_mode == OUT_F16);
-                    else
-                        return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-                };
                 if(prm.bias != nullptr)
                 {
                     const float b = (p < prm.rows_p) ? prm.beta * load_bias(prm.bias, prm.bias_is_bf16, p) : 0.f;
@@ -648,47 +778,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                         if(j < bw)
                             v[j] *= prm.alpha;
                 }
-                if constexpr(EPI != 0)
-                {
-                    if(epi.bias != nullptr)
-                    {
-#pragma unroll
-                        for(int j = 0; j < 64; ++j)
-                            v[j] += bias0;
-                    }
-                    activate(v, epi.act);
-                    if(epi.res != nullptr && p < prm.rows_p)
-                    {
-#pragma unroll
-                        for(int j = 0; j < 64; ++j)
-                            if(j < bw && row_q0 + c0 + j < prm.rows_q)
-                            {
-                                if(j < 16 && h == 0)
-                                    v[j] += raw_to_f32(res0[j & 15], epi.res_mode);
-                                else
-                                    v[j] += load_elem(epi.res, epi.res_mode, static_cast<size_t>(row_q0 + c0 + j) * epi.res_ld + p);
-                            }
-                    }
-                }
-                if(EPI != 0 && prm.tma_store == 2)
-                {
-                    // fp32 output: [row m][32 floats], 8 KB a warp (tiles of at most 64 rows)
-                    float* buf = reinterpret_cast<float*>(smem_gen + static_cast<uint32_t>(warp - 2) * 8192u);
-#pragma unroll
-                    for(int j = 0; j < 64; ++j)
-                        if(j < bw)
-                            buf[j * 32 + lane] = v[j];
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    const int p_warp0 = row_p0 + quarter * 32;
-                    if(lane == 0 && p_warp0 < prm.rows_p)
-                    {
-                        tma_store_2d(&map_out, smem_base + static_cast<uint32_t>(warp - 2) * 8192u, p_warp0 * 4, row_q0);
-                        bulk_commit_group();
-                        bulk_wait_group_read<0>();
-                    }
-                }
-                else if(prm.tma_store)
+                if(prm.tma_store)
                 {
                     // this warp's 32 output columns x bw rows, staged as [row m][32 x bf16] in a retired operand stage (every
                     // tile load has landed and been consumed once the accumulator is complete; a buffer per warp and chunk)
@@ -698,7 +788,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 #pragma unroll
                     for(int j = 0; j < 64; ++j)
                         if(j < bw)
-                            reinterpret_cast<uint16_t*>(buf)[j * 32 + lane] = out16(v[j]);
+                            reinterpret_cast<__nv_bfloat16*>(buf)[j * 32 + lane] = __float2bfloat16_rn(v[j]);
                     fence_proxy_async_smem();
                     __syncwarp();
                     const int p_warp0 = row_p0 + quarter * 32;
@@ -717,13 +807,7 @@ gemm_decode_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 #pragma unroll
                     for(int j = 0; j < 64; ++j)
                         if(j < bw && row_q0 + c0 + j < prm.rows_q)
-                        {
-                            const size_t at = static_cast<size_t>(row_q0 + c0 + j) * prm.ldo + p;
-                            if constexpr(EPI != 0)
-                                store_out(prm.out, at, v[j], epi.out_mode);
-                            else
-                                prm.out[at] = __float2bfloat16_rn(v[j]);
-                        }
+                            prm.out[static_cast<size_t>(row_q0 + c0 + j) * prm.ldo + p] = __float2bfloat16_rn(v[j]);
                 }
             }
             } // chunks of 64 columns

@@ -37,7 +37,8 @@
 
 namespace b200 {
 
-constexpr int kPersistentThreads = 384;
+constexpr int kPersistentThreads = 384; // (512 with the fused epilogue: four more epilogue warps, 12..15)
+__host__ __device__ constexpr int persistent_threads(int epi) { return epi ? 512 : kPersistentThreads; }
 constexpr int kMaxAcc            = 2;
 
 struct PersistentParams
@@ -152,7 +153,7 @@ struct WorkIter
 };
 
 template <int KIND, int SFW, int CG, int EPI>
-__global__ void __launch_bounds__(kPersistentThreads, 1)
+__global__ void __launch_bounds__(persistent_threads(EPI), 1)
 gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_sfp, const __grid_constant__ CUtensorMap map_sfq,
                        const __grid_constant__ CUtensorMap map_out, const PersistentParams prm, const __grid_constant__ EpilogueParams<EPI> epi)
@@ -211,7 +212,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
     if(threadIdx.x == 0)
     {
         if constexpr(EPI != 0)
-            for(int i = 0; i < 8; ++i) // the residual tiles of the fused epilogue: two per epilogue warp
+            for(int i = 0; i < 2 * kFusedWarps; ++i) // the residual tiles of the fused epilogue: two per epilogue warp
                 mbar_init(smem_base + L.total + 8u * i, 1);
         for(int s = 0; s < S; ++s)
         {
@@ -226,7 +227,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         for(int a = 0; a < kMaxAcc; ++a)
         {
             mbar_init(acc_full_bar(a), 1);
-            mbar_init(acc_empty_bar(a), 4 * CG);
+            mbar_init(acc_empty_bar(a), (EPI ? kFusedWarps : 4) * CG);
         }
         mbar_init(epi_bar, 4);
         mbar_init(drain_bar, 1);
@@ -845,12 +846,24 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         // Output staging: every epilogue warp owns two 2 KB buffers (32 rows x 64 bytes) and stores them with its
         // own TMA tile stores, so the warps never wait for one another and global memory sees whole 64-byte runs.
         const bool use_tma   = prm.tma_store != 0;
+        // (fused epilogue) eight epilogue warps, 6..9 and 12..15: those of one TMEM lane quarter take alternate steps
+        const int epi_warp  = warp < 10 ? warp - 6 : warp - 8;
+        const int c_first   = EPI ? epi_warp >> 2 : 0;
+        const int c_step    = EPI ? 2 : 1;
         const uint32_t epi_warp_bytes = prm.epi_bufs == 2 ? 8192u : 4096u;
-        uint8_t* epi_gen     = smem_gen + L.epi_off + (warp - 6) * epi_warp_bytes;
-        const uint32_t epi_s = smem_base + L.epi_off + (warp - 6) * epi_warp_bytes;
+        uint8_t* epi_gen     = smem_gen + L.epi_off + epi_warp * epi_warp_bytes;
+        const uint32_t epi_s = smem_base + L.epi_off + epi_warp * epi_warp_bytes;
         int ebuf             = 0;
         uint32_t wbuf        = 0; // wide stores: which of the two 4 KB buffers comes next (0 when there is only one)
-        FusedStore fused;         // (fused epilogue) this warp's place in its ring of two slots
+        FusedWarp fused{};
+        if constexpr(EPI != 0)
+        {
+            fused.slots     = smem_base + L.epi_off + static_cast<uint32_t>(epi_warp) * 2u * epi.slot_bytes;
+            fused.slots_gen = smem_gen + L.epi_off + static_cast<uint32_t>(epi_warp) * 2u * epi.slot_bytes;
+            fused.rbars     = smem_base + L.total + 16u * epi_warp;
+            fused.bias      = reinterpret_cast<float*>(smem_gen + L.total + kFusedBarBytes) + 128 * epi_warp;
+            fused.group     = epi_warp >> 2;
+        }
         if(use_tma && lane == 0)
             tma_prefetch_desc(&map_out);
         uint32_t epi_phase = 0;
@@ -947,8 +960,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                                        : static_cast<const uint8_t*>(prm.bias) + static_cast<size_t>(w.b) * static_cast<size_t>(prm.bias_batch_stride) * (prm.bias_is_bf16 ? 2u : 4u);
             if constexpr(EPI != 0)
                 if(prm.tma_store == 3)
-                    fused_begin(fused, epi, (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32, row_q0, bn, epi_s_fused(smem_base, L.epi_off, warp - 6, epi),
-                                smem_base + L.total + 16u * (warp - 6), lane);
+                    fused_begin(fused, epi, (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32, row_q0, bn, prm.rows_q, lane);
             ok = bounded_wait(acc_full_bar(a), (uc / prm.n_acc) & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, uc);
             ok = __all_sync(0xffffffffu, ok);
             if(!ok)
@@ -987,7 +999,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                 const uint32_t src    = zrank < owner ? zrank : zrank - 1u; // this slice's place among the owner's sources
                 const uint32_t dst_row = map_to_cta(smem_base + L.red_off, owner) + (src * per + prow) * static_cast<uint32_t>(bn) * 4u;
                 const uint32_t dst_bar = map_to_cta(red_bar, owner);
-                for(int c = 0; c < n_chunks; ++c)
+                for(int c = c_first; c < n_chunks; c += c_step)
                 {
                     uint32_t r[32];
                     if(chunk == 32)
@@ -1072,34 +1084,6 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
 #pragma unroll
                         for(int j = 0; j < 32; ++j)
                             v[j] *= prm.alpha;
-                    }
-                    if constexpr(EPI != 0)
-                    {
-                        if(epi.bias != nullptr)
-                        {
-                            if(prm.bias_on_q)
-                                add_row<32>(v, epi.bias, epi.bias_mode, q_first, min(chunk, prm.rows_q - q_first), epi.bias_vec != 0);
-                            else
-                            {
-                                const float b = p < prm.rows_p ? load_elem(epi.bias, epi.bias_mode, p) : 0.f;
-#pragma unroll
-                                for(int j = 0; j < 32; ++j)
-                                    v[j] += b;
-                            }
-                        }
-                        activate(v, epi.act);
-                        if(epi.res != nullptr && p < prm.rows_p)
-                        {
-                            if(!prm.transposed_out)
-                                add_row<32>(v, epi.res, epi.res_mode, static_cast<size_t>(p) * epi.res_ld + q_first, min(chunk, prm.rows_q - q_first), epi.res_vec != 0);
-                            else
-                            {
-#pragma unroll
-                                for(int j = 0; j < 32; ++j)
-                                    if(j < chunk && q_first + j < prm.rows_q)
-                                        v[j] += load_elem(epi.res, epi.res_mode, static_cast<size_t>(q_first + j) * epi.res_ld + p);
-                            }
-                        }
                     }
                     if(use_tma)
                     {
@@ -1193,22 +1177,18 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                         }
                     }
                 };
-                if(EPI != 0 && prm.tma_store == 3)
+                if constexpr(EPI != 0)
                 {
-                    // Fused epilogue with tile loads of the residual and tile stores (row-major output): 64 or 32 columns a step
-                    if constexpr(EPI != 0)
+                    const int p_warp0 = (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32;
+                    if(prm.tma_store == 3)
+                        ok = fused_tile(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, abort_f, lane, uc, release_acc);
+                    else
                     {
-                        const int p_warp0 = (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32;
-                        const uint32_t slots = epi_s_fused(smem_base, L.epi_off, warp - 6, epi);
-                        uint8_t* slots_gen   = smem_gen + (slots - smem_base);
-                        const uint32_t rbars = smem_base + L.total + 16u * (warp - 6);
-                        if(epi.step == 64)
-                            ok = fused_tile<64>(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, slots, slots_gen, rbars, abort_f, lane, uc, release_acc);
-                        else
-                            ok = fused_tile<32>(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, slots, slots_gen, rbars, abort_f, lane, uc, release_acc);
+                        const float* red = reinterpret_cast<const float*>(smem_gen + L.red_off) + static_cast<size_t>(prow) * bn;
+                        ok = fused_plain_tile(epi, prm, tacc, p, row_q0, bn, c_first, csplit, red, static_cast<size_t>(per) * bn, red_bar, abort_f, uc, release_acc);
                     }
                 }
-                else if(EPI == 0 && prm.out_mode >= OUT_E2M1)
+                else if(prm.out_mode >= OUT_E2M1)
                 {
                     // Re-quantising epilogue (row-major output, no K split, tile width a multiple of 128): the thread's row
                     // goes out 128 columns at a time.  e4m3 + UE8M0: the block's maximum first (one pass over the TMEM
@@ -1304,7 +1284,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                     }
                     release_acc();
                 }
-                else if(EPI == 0 && !split && prm.tma_store == 2)
+                else if(!split && prm.tma_store == 2)
                 {
                     // Wide path (row-major output, tile width a multiple of 64): 64 columns per step, so that the
                     // one warp per scheduler that runs this code has long runs of independent instructions: one

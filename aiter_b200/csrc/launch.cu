@@ -162,16 +162,6 @@ struct DeviceState
 };
 
 static std::mutex g_mutex;
-// Held from a re-layout pass to the launch of the GEMM that reads its buffer: another host thread on the same stream must not
-// put its own pass in between.
-static std::mutex g_prepass_mutex;
-
-static bool is_capturing(cudaStream_t stream)
-{
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    cudaStreamIsCapturing(stream, &cap);
-    return cap != cudaStreamCaptureStatusNone;
-}
 static std::map<int, DeviceState> g_devices;
 static std::atomic<unsigned long long> g_launches{0};
 
@@ -574,7 +564,7 @@ static void launch_persistent(int ctas, size_t smem, cudaStream_t stream, const 
     raise_smem_limit(kernel, attr_done);
     cudaLaunchConfig_t lc{};
     lc.gridDim          = dim3(ctas, 1, 1);
-    lc.blockDim         = dim3(kPersistentThreads, 1, 1);
+    lc.blockDim         = dim3(persistent_threads(EPI), 1, 1);
     lc.dynamicSmemBytes = smem;
     lc.stream           = stream;
     cudaLaunchAttribute attr[2];
@@ -717,7 +707,7 @@ static bool decode_mixed_disabled()
     return off;
 }
 
-constexpr int kFusedBarrierBytes = 128; // the residual barriers behind the persistent kernel's shared memory (fused epilogue)
+constexpr int kFusedExtraBytes = kFusedBarBytes + kFusedBiasBytes; // behind the persistent kernel's shared memory (fused epilogue)
 
 constexpr uint32_t kDecodeBarrierBytes = 256; // the decode kernel's barriers and flags (gemm_decode.cuh)
 
@@ -790,15 +780,13 @@ static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
     EpilogueParams<1> e{};
     e.bias      = prob.fused_bias;
     e.bias_mode = prob.fused_bias_mode;
-    e.bias_vec  = (reinterpret_cast<uintptr_t>(prob.fused_bias) & 15) == 0;
     e.res       = prob.residual;
     e.res_ld    = prob.residual_ld;
     e.res_mode  = prob.residual_mode;
     e.res_vec   = (reinterpret_cast<uintptr_t>(prob.residual) & 15) == 0 && (prob.residual_ld * (prob.residual_mode == OUT_F32 ? 4 : 2)) % 16 == 0;
     e.act       = prob.activation;
     e.out_mode  = prob.out_mode;
-    e.step      = 64;
-    e.slot_bytes = 4096;
+    e.slot_bytes = 2048;
     return e;
 }
 
@@ -924,12 +912,14 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
     prm.tmem_cols = cols;
     CUtensorMap mo = mp;
     const bool out32 = (prob.out_mode == OUT_F32); // (fused epilogue only)
-    prm.tma_store  = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % (out32 ? 4 : 8) == 0) && (!out32 || bn <= 64) ? (out32 ? 2 : 1) : 0;
-    if(prm.tma_store == 2)
+    prm.tma_store  = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % (out32 ? 4 : 8) == 0) ? 1 : 0;
+    if(prm.tma_store && prob.fused)
     {
-        const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 4, static_cast<cuuint64_t>(prob.M)};
-        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * 4};
-        const cuuint32_t box[2]     = {128u, static_cast<cuuint32_t>(bn)};
+        // 16 rows of a warp's 32 columns per store
+        const int esize             = out32 ? 4 : 2;
+        const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * esize, static_cast<cuuint64_t>(prob.M)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * esize};
+        const cuuint32_t box[2]     = {static_cast<cuuint32_t>(32 * esize), 16u};
         mo = encode_map(prob.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "output");
     }
     else if(prm.tma_store)
@@ -981,16 +971,58 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
 // threshold, inside stream capture without a buffer, or with caller-provided scratch the in-kernel path runs.
 constexpr long long kWidenPrepassMinM = 512;
 
+// Output and residual whose rows allow tile copies
+static bool fused_rows_aligned(const GemmProblem& prob)
+{
+    auto ok = [](const void* p, long long ld, int mode) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (mode == OUT_F32 ? 4 : 2)) % 16 == 0; };
+    return ok(prob.out, prob.ldo, prob.out_mode) && (prob.residual == nullptr || ok(prob.residual, prob.residual_ld, prob.residual_mode));
+}
+
+// What the fused epilogue prefers where choose_config would take something else; fields that the caller has set stay.
+static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConfig& cfg)
+{
+    if(cfg.swap >= 0 || cfg.bn > 0 || cfg.cg > 0)
+        return;
+    const long long M = prob.M, N = prob.N;
+    const long long tiles_p = (N + kTileP - 1) / kTileP;
+    if(M <= 64)
+        return;
+    if(M <= 256 && prob.kind != PK_BF16)
+        return;
+    if(M <= 256)
+    {
+        // tiles of 64 rows (128 where those do not fit the machine at once) on the few-rows kernel, K split inside a cluster
+        cfg.swap = 1;
+        cfg.cg   = 1;
+        cfg.bn   = tiles_p * ((M + 63) / 64) <= 2LL * num_sms ? 64 : 128;
+        return;
+    }
+    if(!fused_rows_aligned(prob))
+    {
+        // rows on odd addresses: the weights on the 128-row slot, so that the lanes run along a row of the output
+        cfg.swap = 1;
+        cfg.cg   = 1;
+        cfg.bn   = 256;
+        while(cfg.bn > 64 && tiles_p * ((M + cfg.bn - 1) / cfg.bn) < num_sms)
+            cfg.bn >>= 1;
+    }
+}
+
+size_t fused_workspace_bytes(long long M, long long N, long long K)
+{
+    if(M < kScalePrepassMinM || K % 256 != 0 || K < (tall_problem(M, N) ? 1024 : kScalePrepassMinK) || relay_prepass_disabled())
+        return 0;
+    return static_cast<size_t>((M + 31) / 32 + (N + 31) / 32) * 32 * static_cast<size_t>(K / 32);
+}
+
 void launch_gemm(const GemmProblem& prob)
 {
     if(prob.M == 0 && prob.N > 0 && prob.K > 0)
         return; // no activation rows: nothing to compute, the (empty) output is already complete
     if(prob.kind == PK_MXFP4 && prob.M >= kScalePrepassMinM && prob.scratch == nullptr && prob.act_sf.wire == SFW_E8M0_SHUFFLE &&
        prob.wgt_sf.wire == SFW_E8M0_SHUFFLE && prob.K % 256 == 0 && prob.K >= (tall_problem(prob.M, prob.N) ? 1024 : kScalePrepassMinK) &&
-       !relay_prepass_disabled() && !(prob.fused && is_capturing(prob.stream)))
+       !relay_prepass_disabled() && (!prob.fused || prob.workspace != nullptr))
     {
-        // (the fused epilogue stays off the shared buffer inside a capture: two graphs captured on one stream would both hold it)
-        std::lock_guard<std::mutex> prepass(g_prepass_mutex);
         int prev_dev = 0;
         B200_CUDA(cudaGetDevice(&prev_dev));
         if(prev_dev != prob.device)
@@ -1016,8 +1048,8 @@ void launch_gemm(const GemmProblem& prob)
             DeviceState& st    = device_state(prob.device);
             StreamWorkspace& w = st.ws[prob.stream];
             const size_t bytes = static_cast<size_t>(ga + gw) * 32 * kblocks;
-            bool usable        = w.relaid_bytes >= bytes;
-            if(!usable)
+            bool usable        = prob.fused ? prob.workspace_bytes >= bytes : w.relaid_bytes >= bytes;
+            if(!usable && !prob.fused)
             {
                 cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
                 cudaStreamIsCapturing(prob.stream, &cap);
@@ -1033,7 +1065,7 @@ void launch_gemm(const GemmProblem& prob)
             }
             if(usable)
             {
-                relaid = static_cast<uint32_t*>(w.relaid);
+                relaid = static_cast<uint32_t*>(prob.fused ? prob.workspace : w.relaid);
                 auto run = [&](const ScaleOperand& sf, uint32_t* dst, long long groups) {
                     const long long total = groups * (kblocks / 4) * 32;
                     const int blocks      = static_cast<int>(std::min<long long>((total + 255) / 256, 148LL * 16));
@@ -1059,7 +1091,6 @@ void launch_gemm(const GemmProblem& prob)
     if(prob.kind == PK_MXF8F4 && prob.M >= kWidenPrepassMinM && prob.scratch == nullptr && prob.wgt.mode == OPM_TILE16 &&
        prob.N % 16 == 0 && prob.K % 64 == 0 && !widen_prepass_disabled())
     {
-        std::lock_guard<std::mutex> prepass(g_prepass_mutex);
         int prev_dev = 0;
         B200_CUDA(cudaGetDevice(&prev_dev));
         if(prev_dev != prob.device)
@@ -1175,6 +1206,8 @@ static void launch_gemm_locked(const GemmProblem& prob)
     }
     B200_CHECK(prob.batch == 1 || (prob.kind == PK_BF16 && prob.act.mode == OPM_BATCHED && prob.wgt.mode == OPM_BATCHED),
                "internal: batched launches are built for row-major bf16 operands");
+    if(prob.fused)
+        choose_fused_config(prob, st.sm_count, cfg);
     choose_config(prob.kind, prob.M, prob.N, prob.K, st.sm_count, cfg);
     // the fused epilogue splits K inside a cluster only: no partial sums in memory that two captured graphs would share
     if(prob.fused && !(cfg.swap && cfg.cg == 1))
@@ -1218,27 +1251,24 @@ static void launch_gemm_locked(const GemmProblem& prob)
                            (prob.out_mode == OUT_BF16 || prob.out_mode == OUT_F16) && prob.batch == 1;
     // fused epilogue through its slots: row-major output and residual whose pitches and bases allow tensor maps
     EpilogueParams<1> epi = epilogue_params(prob);
-    const bool slots      = prob.fused && !cfg.swap && cfg.bn % 64 == 0 && prob.batch == 1 && (reinterpret_cast<uintptr_t>(prob.out) & 15) == 0 &&
+    const bool slots      = prob.fused && !cfg.swap && cfg.bn % kFusedStep == 0 && prob.batch == 1 && (reinterpret_cast<uintptr_t>(prob.out) & 15) == 0 &&
                        (prob.ldo * (prob.out_mode == OUT_F32 ? 4 : 2)) % 16 == 0 && (prob.residual == nullptr || epi.res_vec);
-    int epi_units = tma_store ? 1 : 0;
+    int epi_units = tma_store && !prob.fused ? 1 : 0; // staging areas of 16 KB
     if(slots)
     {
         epi.res_tma        = prob.residual != nullptr;
         const bool wide    = prob.out_mode == OUT_F32 || (epi.res_tma && prob.residual_mode == OUT_F32);
-        const bool unequal = epi.res_tma && (prob.out_mode == OUT_F32) != (prob.residual_mode == OUT_F32);
-        epi.step       = wide ? 32 : 64;
-        epi.slot_bytes = unequal ? 8192 : 4096;
-        epi.out_off    = unequal ? 4096 : 0;
-        epi_units      = unequal ? 4 : 2;
+        epi.slot_bytes     = wide ? 4096 : 2048;
+        epi_units          = static_cast<int>(2u * kFusedWarps * epi.slot_bytes / kEpiStageBytes);
     }
     // Decode shapes: the K split runs across the CTAs of a thread-block cluster, one output tile per cluster; the
     // partial accumulators meet in the first CTA's shared memory instead of a global workspace.
     int csplit = 1;
     // (only with the weights on the 128-row slot: for row-major tiles, whose partial tiles are wide, it was measured two to
     // five times slower than the workspace split)
-    const int smem_limit = st.smem_optin - (prob.fused ? kFusedBarrierBytes : 0);
+    const int smem_limit = st.smem_optin - (prob.fused ? kFusedExtraBytes : 0);
     if(cfg.swap && cg == 1 && splits > 1 && splits <= 8 && prob.scratch == nullptr && !cluster_split_disabled() &&
-       max_stages(cfg.bn, cg, smem_limit, f4_operand, sf_unit, tma_store, splits) >= 4)
+       max_stages(cfg.bn, cg, smem_limit, f4_operand, sf_unit, epi_units, splits) >= 4)
     {
         csplit = splits;
         splits = 1;
@@ -1397,14 +1427,14 @@ static void launch_gemm_locked(const GemmProblem& prob)
     prm.epi_bufs = tma_store ? 1 : 0;
     if(prob.fused)
     {
-        // (3: the slot path; otherwise 32 columns per store, or plain stores)
-        prm.tma_store = slots ? 3 : (tma_store ? 1 : 0);
+        // (3: the slot path; otherwise plain stores)
+        prm.tma_store = slots ? 3 : 0;
         prm.epi_bufs  = epi_units;
     }
     else if(wide_store && static_cast<int>(make_persistent_smem(cfg.bn, cg, stages, f4_operand, sf_unit, 2, csplit).total) + 1024 <= st.smem_optin)
         prm.epi_bufs = 2;
     const PersistentSmem L = make_persistent_smem(cfg.bn, cg, stages, f4_operand, sf_unit, prm.epi_bufs, csplit);
-    const size_t smem      = L.total + 1024 + (prob.fused ? kFusedBarrierBytes : 0);
+    const size_t smem      = L.total + 1024 + (prob.fused ? kFusedExtraBytes : 0);
     // Tile order.  When the Q operand (the weights of a tall problem) is much larger than what L2 keeps beside the
     // streaming P operand and the output, walk it in panels of about 32 MB.
     prm.panel_q = 0;
@@ -1423,28 +1453,27 @@ static void launch_gemm_locked(const GemmProblem& prob)
     CUtensorMap mo         = mp;
     if(slots)
     {
-        // 32 rows of one step; rows of 128 bytes, or 64 where 32 columns of a 16-bit type meet a 32-bit one
+        // 32 rows of one step: rows of 128 bytes for fp32, 64 for the 16-bit types
         auto rows_map = [&](const void* base, long long ld, int mode, const char* what) {
             const int esize             = mode == OUT_F32 ? 4 : 2;
             const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * esize, static_cast<cuuint64_t>(prob.M)};
             const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esize};
-            const cuuint32_t box[2]     = {static_cast<cuuint32_t>(epi.step * esize), 32u};
+            const cuuint32_t box[2]     = {static_cast<cuuint32_t>(kFusedStep * esize), 32u};
             return encode_map(base, 2, dims, strides, box, box[0] == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, what);
         };
         mo = rows_map(prob.out, prob.ldo, prob.out_mode, "output");
         if(epi.res_tma)
             epi.map_res = rows_map(prob.residual, prob.residual_ld, prob.residual_mode, "residual");
     }
-    else if(tma_store)
+    else if(tma_store && !prob.fused)
     {
         // bf16 [M][N] seen as bytes; one box = 32 values of the fast dimension by 32 rows (or the tile's chunk of rows
         // when the 128-row slot holds the weights and the store is transposed)
         const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 2, static_cast<cuuint64_t>(prob.M)};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * 2};
-        const bool wide_box         = wide_store && !prob.fused;
-        const cuuint32_t box[2]     = {wide_box ? 128u : 64u, static_cast<cuuint32_t>(cfg.swap ? (cfg.bn < 32 ? 16 : 32) : 32)};
+        const cuuint32_t box[2]     = {wide_store ? 128u : 64u, static_cast<cuuint32_t>(cfg.swap ? (cfg.bn < 32 ? 16 : 32) : 32)};
         mo = encode_map(prob.out, 2, dims, strides, box,
-                        cfg.swap ? CU_TENSOR_MAP_SWIZZLE_NONE : (wide_box ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B), "output");
+                        cfg.swap ? CU_TENSOR_MAP_SWIZZLE_NONE : (wide_store ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B), "output");
     }
     const int ctas         = clusters * cg * csplit;
     if(prob.fused)

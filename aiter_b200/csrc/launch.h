@@ -106,6 +106,8 @@ struct GemmProblem
     const void* residual = nullptr;   // [M, N], residual_ld elements between rows, OutMode of its type
     long long residual_ld = 0;
     int residual_mode = 0;
+    void* workspace = nullptr;        // the caller's, for the re-laid scales of tall MXFP4 problems (fused_workspace_bytes)
+    size_t workspace_bytes = 0;
     int device = 0;
     cudaStream_t stream = nullptr;
     KernelConfig cfg;
@@ -122,6 +124,8 @@ bool config_from_id(int kernel_id, KernelConfig& cfg);
 const char* kernel_menu_text();
 
 void launch_gemm(const GemmProblem& prob);
+// Bytes of workspace with which a fused MXFP4 GEMM of this size runs fastest (0: none needed)
+size_t fused_workspace_bytes(long long M, long long N, long long K);
 
 // FP8 x FP8 with fp32 scales per 128-wide K block (x_scale[m][kb] at x_scale + m*xs_stride_m + kb*xs_stride_k,
 // w_scale [ceil(N/128)][K/128] dense), bf16 output.

@@ -67,6 +67,11 @@ def gemm_a4w4_fused(A: Tensor, B: Tensor, A_scale: Tensor, B_scale: Tensor, bias
     n = B.shape[0]
     _check_residual(fn, A, n, residual)
     a2 = A if A.dim() == 2 else A.reshape(-1, A.shape[-1])
-    o2, result = _out(fn, A, a2.shape[0], n, otype, out)
-    _ffi.call("aiter_b200_gemm_a4w4_fused", a2, B, A_scale, B_scale, bias, _rows(residual, n), o2, act, bool(bpreshuffle), kernelName or None)
+    m = a2.shape[0]
+    o2, result = _out(fn, A, m, n, otype, out)
+    # tall problems re-lay the block scales once per call, in memory of this call's own (two captured graphs share none)
+    nbytes = _ffi.fused_workspace_bytes(m, n, 2 * a2.shape[1]) if m >= 1024 else 0
+    workspace = empty(nbytes, dtype=torch.uint8, device=A.device) if nbytes else None
+    _ffi.call("aiter_b200_gemm_a4w4_fused", a2, B, A_scale, B_scale, bias, _rows(residual, n), o2, workspace, act, bool(bpreshuffle),
+              kernelName or None)
     return result

@@ -214,7 +214,7 @@ AITER_B200_API int dynamic_per_group_scaled_quant(aiter_tensor_t* out, aiter_ten
  * form in the reference (its Triton gemm_a16w16 takes a bias and an activation).  Operands as for gemm_a16w16_asm,
  * mxfp8_mxfp8_gemm_asm and gemm_a4w4_asm.  bias [N] and residual [M, N]: bf16 / fp16 / fp32 or NULL; out [M, N] bf16 / fp16 /
  * fp32; out may be residual itself (same type and strides), else they must not overlap.  activation: 0 none, 1 relu, 2 silu,
- * 3 gelu (erf), 4 gelu_tanh.  No per-stream workspace is used inside a stream capture. */
+ * 3 gelu (erf), 4 gelu_tanh.  No buffer of the library's is used: calls on any streams and captured graphs may overlap. */
 AITER_B200_API int aiter_b200_gemm_a16w16_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* bias, aiter_tensor_t* residual,
                                                 aiter_tensor_t* out, int activation, int bpreshuffle, const char* kernelName,
                                                 void* stream);
@@ -222,8 +222,12 @@ AITER_B200_API int aiter_b200_gemm_a8w8_mxfp8_fused(aiter_tensor_t* A, aiter_ten
                                                     aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
                                                     int a_preshuffle, const char* kernelName, void* stream);
 AITER_B200_API int aiter_b200_gemm_a4w4_fused(aiter_tensor_t* A, aiter_tensor_t* B, aiter_tensor_t* A_scale, aiter_tensor_t* B_scale,
-                                              aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out, int activation,
-                                              int bpreshuffle, const char* kernelName, void* stream);
+                                              aiter_tensor_t* bias, aiter_tensor_t* residual, aiter_tensor_t* out,
+                                              aiter_tensor_t* workspace, int activation, int bpreshuffle, const char* kernelName,
+                                              void* stream);
+/* Bytes of `workspace` (uint8, 16-byte aligned, written by the call) with which a problem of this size runs fastest: tall MXFP4
+ * problems re-lay their block scales once.  0: none is needed; with NULL the GEMM re-orders them tile by tile. */
+AITER_B200_API long long aiter_b200_gemm_a4w4_fused_workspace(int M, int N, int K);
 
 /* ---- what stands between two GEMMs of a transformer block, one launch each.  No counterpart of this form in the reference
  * (its closest: rmsnorm2d_fwd_with_add / layernorm2d_fwd_with_add, silu_and_mul / gelu_and_mul / gelu_tanh_and_mul).

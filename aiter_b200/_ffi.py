@@ -132,6 +132,15 @@ def _pack_tensor(t):
                           t.get_device() if t.is_cuda else -1)
 
 
+_pack_1d, _pack_2d = _PACKERS[1], _PACKERS[2]
+
+
+def pack_rows(t: torch.Tensor, m: int, n: int, device: int) -> bytes:
+    """Descriptor of a contiguous [m, n] tensor that the caller has just allocated on `device`."""
+    dtype = _DTYPE_IDS.get(t.dtype)
+    return _pack_2d(t.data_ptr(), m * n, 2, m, n, n, 1, aiter_dtype_id(t.dtype) if dtype is None else dtype, device)
+
+
 def _int(value):
     return -1 if value is None else int(value)
 
@@ -177,11 +186,33 @@ def call(name: str, *args):
     stream = None
     for a in args:
         if isinstance(a, torch.Tensor) and a.is_cuda:
-            stream = _raw_stream(a.get_device()) if _raw_stream is not None else torch.cuda.current_stream(a.device).cuda_stream
+            stream = current_stream(a.get_device())
             break
     if fn(*[c(a) for c, a in zip(convert, args)], stream) != 0:
-        msg = _lib.aiter_get_last_error()
-        raise RuntimeError(f"{name} failed: {msg.decode() if msg else 'unknown error'}")
+        _raise(name)
+
+
+def _raise(name: str):
+    msg = _lib.aiter_get_last_error()
+    raise RuntimeError(f"{name} failed: {msg.decode() if msg else 'unknown error'}")
+
+
+def current_stream(device: int):
+    """The current stream of a GPU as the library takes it (device -1: none, the library refuses host tensors)."""
+    if device < 0:
+        return None
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def call_packed(name: str, device: int, *args):
+    """`call` with every argument in the form the library takes: descriptors packed, no None among the numbers."""
+    fn, _ = _FUNCS.get(name) or _bind(name)
+    if AITER_LOG_MORE == 2:
+        import logging
+
+        logging.getLogger("aiter").info("calling %s(%s)", name, ", ".join(f"<{len(a)} bytes>" if isinstance(a, bytes) else repr(a) for a in args))
+    if fn(*args, current_stream(device)) != 0:
+        _raise(name)
 
 
 def get_padded_m(M: int, N: int, K: int, gl: int) -> int:

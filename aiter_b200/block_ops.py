@@ -4,9 +4,10 @@ instead of 16-bit values.  The reference's closest forms: aiter/ops/rmsnorm.py, 
 from __future__ import annotations
 
 import torch
-from torch import Tensor, empty
+from torch import Tensor, empty, empty_like
 
 from . import _ffi, dtypes
+from ._ffi import _pack_tensor as pack, call_packed, pack_rows
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _NORMS = {"rms": 0, "layer": 1}
@@ -66,26 +67,30 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
     m = x2.shape[0]
     r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, residual.shape[-1])
     copies_x = residual is None and gate is None and not post and residual_out is None
+    dev = x.get_device()
     if residual_out is not None:
         if residual_out.shape != x.shape:
             raise ValueError(f"{fn}: residual_out must have x's shape {tuple(x.shape)}, got {tuple(residual_out.shape)}")
         h = residual_out
-        h2 = h if h.dim() == 2 else h.view(-1, n)
+        h2 = pack(h if h.dim() == 2 else h.view(-1, n))
     elif copies_x:
         h, h2 = x, None
     else:
-        h = empty(*x.shape, dtype=x.dtype if residual is None else residual.dtype, device=x.device)
-        h2 = h if h.dim() == 2 else h.view(-1, n)
+        like = x if residual is None else residual
+        h = empty_like(like) if like.is_contiguous() and like.shape == x.shape else empty(*x.shape, dtype=like.dtype, device=x.device)
+        h2 = pack_rows(h, m, n, dev)
     scale, layout = None, 0
     if quant_dtype is not None:
         if otype is not None:
             raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
         y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
+        y2 = pack(y)
     else:
         y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
-    _ffi.call("aiter_b200_gated_residual_norm", y, scale, h2, x2, r2, weight, bias, gate, post_weight, post_bias, residual_scale,
-              weight_offset, eps, _NORMS[norm], post, layout)
+        y2 = pack_rows(y, m, n, dev)
+    call_packed("aiter_b200_gated_residual_norm", dev, y2, pack(scale), h2, pack(x2), pack(r2), pack(weight), pack(bias), pack(gate),
+                pack(post_weight), pack(post_bias), residual_scale, weight_offset, eps, _NORMS[norm], post, layout)
     if x.dim() != 2:
         y = y.view(*x.shape[:-1], y.shape[-1])
     return (y, h) if scale is None else (y, scale, h)
@@ -104,15 +109,18 @@ def act_and_mul(x: Tensor, activation: str = "silu", otype: torch.dtype | None =
         raise ValueError(f"{fn}: the last dimension must be even, got {x.shape[-1]}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     m, n = x2.shape[0], x2.shape[1] // 2
+    dev = x.get_device()
     scale, layout = None, 0
     if quant_dtype is not None:
         if otype is not None:
             raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
         y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
+        y2 = pack(y)
     else:
         y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
-    _ffi.call("aiter_b200_act_and_mul", y, scale, x2, act, layout)
+        y2 = pack_rows(y, m, n, dev)
+    call_packed("aiter_b200_act_and_mul", dev, y2, pack(scale), pack(x2), act, layout)
     if x.dim() != 2:
         y = y.view(*x.shape[:-1], y.shape[-1])
     return y if scale is None else (y, scale)

@@ -249,12 +249,17 @@ static StreamWorkspace& stream_workspace(DeviceState& st, cudaStream_t stream, s
 
 int device_sm_count(int device)
 {
+    static std::atomic<int> known[64]; // (asked for by every launch of the block operators)
+    if(device >= 0 && device < 64 && known[device].load(std::memory_order_relaxed) != 0)
+        return known[device].load(std::memory_order_relaxed);
     int prev = 0;
     B200_CUDA(cudaGetDevice(&prev));
     B200_CUDA(cudaSetDevice(device));
     std::lock_guard<std::mutex> lk(g_mutex);
     int n = device_state(device).sm_count;
     cudaSetDevice(prev);
+    if(device >= 0 && device < 64)
+        known[device].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -787,6 +792,9 @@ static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
     e.act       = prob.activation;
     e.out_mode  = prob.out_mode;
     e.slot_bytes = 2048;
+    // more than L2 holds: neither the residual nor the output should push the operands out of it (16384 x 7168 x 2048, fp32
+    // residual and output: 462 -> 444 us under the power cap; without effect where they fit)
+    e.stream = prob.M * prob.N * ((prob.out_mode == OUT_F32 ? 4 : 2) + (prob.residual == nullptr ? 0 : prob.residual_mode == OUT_F32 ? 4 : 2)) > (256LL << 20);
     return e;
 }
 
@@ -1005,6 +1013,39 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
         cfg.bn   = 256;
         while(cfg.bn > 64 && tiles_p * ((M + cfg.bn - 1) / cfg.bn) < num_sms)
             cfg.bn >>= 1;
+        return;
+    }
+    // MX tiles on CTA pairs: 256 columns leave TMEM no second accumulator beside the scale buffers, so the epilogue is exposed;
+    // 224 (MXFP8, four stages) or 192 have two.  Waves over the SM pairs x time per tile, fitted to 4096 x 7168 x K = 512 .. 8192
+    // (listed in 0.1 us, silu, then with a bf16 residual; the code counts in 0.01 us): MXFP8 256: 63 74 105 163 299, 68 77 112 187 337;
+    // 224: 61 67 86 149 299, 74 86 113 173 332; 192: 52 56 73 148 240, 57 62 89 152 282; MXFP4 256: 62 67 85 114 174,
+    // 65 71 87 116 181; 192: 53 56 65 82 144, 57 61 74 87 145 (224 leaves MXFP4 two stages: 60 67 83 127 232).
+    const long long pair_rows = (M + 2 * kTileP - 1) / (2 * kTileP);
+    if(prob.kind != PK_BF16 && M >= 512 && N >= 192 && pair_rows * ((N + 255) / 256) >= 24)
+    {
+        const bool res      = prob.residual != nullptr;
+        const long long k10 = prob.K * 10 / 1024;
+        auto tile_time      = [&](int bn) -> long long {
+            if(prob.kind == PK_MXFP8)
+                return bn == 256 ? (res ? 500 + 34 * k10 : 430 + 32 * k10) : bn == 224 ? (res ? std::max(760LL, 400 + 36 * k10) : std::max(610LL, 120 + 36 * k10))
+                                                                                       : (res ? std::max(570LL, 230 + 33 * k10) : std::max(520LL, 120 + 32 * k10));
+            return bn == 256 ? (res ? 560 + 16 * k10 : 530 + 16 * k10) : (res ? std::max(570LL, 470 + 12 * k10) : std::max(530LL, 410 + 12 * k10));
+        };
+        const long long pairs = std::max(num_sms / 2, 1);
+        long long best        = 0;
+        for(int bn : {256, 224, 192})
+        {
+            if(bn == 224 && prob.kind != PK_MXFP8)
+                continue;
+            const long long cost = (pair_rows * ((N + bn - 1) / bn) + pairs - 1) / pairs * tile_time(bn);
+            if(best == 0 || cost < best)
+            {
+                best   = cost;
+                cfg.bn = bn;
+            }
+        }
+        cfg.swap = 0;
+        cfg.cg   = 2;
     }
 }
 

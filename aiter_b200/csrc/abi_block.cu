@@ -3,8 +3,10 @@
 #include "abi_checks.h"
 #include "block_ops.cuh"
 #include "launch.h"
+#include "norm_stream.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 using namespace b200;
@@ -138,23 +140,29 @@ bool is_mx(const aiter_tensor_t* out)
     return out->dtype_ == AITER_DTYPE_fp8 || out->dtype_ == AITER_DTYPE_fp4x2 || out->dtype_ == AITER_DTYPE_u8;
 }
 
-template <typename Params>
-void launch(void (*kernel)(Params), dim3 grid, dim3 block, cudaStream_t stream, const Params& prm)
+template <typename... Params>
+void launch_smem(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const Params&... prm)
 {
     // the set-up of the kernel may run while its predecessor in the stream drains: it waits before its first access
     cudaLaunchConfig_t lc{};
     lc.gridDim  = grid;
     lc.blockDim = block;
+    lc.dynamicSmemBytes = smem;
     lc.stream   = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs    = attr;
     lc.numAttrs = programmatic_launch_enabled() ? 1 : 0;
-    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, prm));
+    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, prm...));
     count_launch();
 }
 
+template <typename... Params>
+void launch(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, const Params&... prm)
+{
+    launch_smem(kernel, grid, block, 0, stream, prm...);
+}
 constexpr unsigned kLongRow = 16384; // elements of a row that the register kernels hold at most (512 threads x 32)
 
 template <int VEC, int CNT>
@@ -171,9 +179,114 @@ void launch_norm_rows(const NormParams& prm, dim3 grid, dim3 block, cudaStream_t
         launch(norm_rows_kernel<VEC, CNT, false, false>, grid, block, stream, prm);
 }
 
-void launch_norm(const NormParams& prm, bool aligned, int sms, cudaStream_t stream)
+// ---- many rows: the streaming kernel, for the usual types (types that differ more run the general kernel)
+struct StreamShape
+{
+    unsigned threads, ctas_per_sm;
+    NormStreamLayout lay;
+    size_t smem;
+};
+
+template <int XD, int RD, int PD, int VEC, int CNT>
+void launch_stream(const NormParams& prm, const StreamShape& sh, int sms, cudaStream_t stream)
+{
+    auto kernel = norm_stream_kernel<XD, RD, PD, VEC, CNT>;
+    static std::atomic<unsigned long long> attr_done{0}; // a bit per device
+    int dev = 0;
+    B200_CUDA(cudaGetDevice(&dev));
+    if(dev >= 64 || !((attr_done.load() >> dev) & 1))
+    {
+        B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        if(dev < 64)
+            attr_done.fetch_or(1ull << dev);
+    }
+    const unsigned grid = std::min<unsigned>(prm.M, static_cast<unsigned>(sms) * sh.ctas_per_sm);
+    launch_smem(kernel, dim3(grid), dim3(sh.threads), sh.smem, stream, prm, sh.lay);
+}
+template <int XD, int RD, int PD>
+void launch_stream_shape(const NormParams& prm, bool aligned, unsigned cnt, const StreamShape& sh, int sms, cudaStream_t stream)
+{
+    if(!aligned)
+        cnt == 8 ? launch_stream<XD, RD, PD, 1, 8>(prm, sh, sms, stream) : launch_stream<XD, RD, PD, 1, 16>(prm, sh, sms, stream);
+    else if(cnt == 1)
+        launch_stream<XD, RD, PD, 8, 1>(prm, sh, sms, stream);
+    else if(cnt == 2)
+        launch_stream<XD, RD, PD, 8, 2>(prm, sh, sms, stream);
+    else
+        launch_stream<XD, RD, PD, 8, 4>(prm, sh, sms, stream);
+}
+
+// Returns false where the general kernels have to serve the call.
+bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, cudaStream_t stream)
 {
     const unsigned n = prm.n;
+    const int xd = prm.x.dt, rd = prm.res.ptr != nullptr ? prm.res.dt : (prm.h.ptr != nullptr ? prm.h.dt : xd);
+    if(prm.M <= 2u * static_cast<unsigned>(sms) || n < 64 || (prm.h.ptr != nullptr && prm.h.dt != rd))
+        return false;
+    // one type for all parameters
+    int pd = -1;
+    for(const RowParam* p : {&prm.weight, &prm.bias, &prm.post_weight, &prm.post_bias, &prm.gate})
+    {
+        if(p->ptr == nullptr || (p == &prm.gate && prm.gate_scalar))
+            continue;
+        if(pd >= 0 && pd != p->dt)
+            return false;
+        pd = p->dt;
+    }
+    const int half = xd == OUT_F32 ? (rd == OUT_F32 ? OUT_BF16 : rd) : xd; // the call's 16-bit type
+    if(pd < 0)
+        pd = half;
+    if((xd != OUT_F32 && rd != OUT_F32 && xd != rd) || (xd == OUT_F32 && rd != OUT_F32) || (pd != OUT_F32 && pd != half))
+        return false;
+    StreamShape sh{};
+    unsigned cnt;
+    if(aligned)
+    {
+        if(n > 16384)
+            return false;
+        cnt        = n > 8192 ? 4 : n > 1024 ? 2 : 1;
+        sh.threads = ((n + 8 * cnt - 1) / (8 * cnt) + 31) / 32 * 32;
+    }
+    else
+    {
+        if(n > 8192)
+            return false;
+        cnt        = n > 2048 ? 16 : 8;
+        sh.threads = ((n + cnt - 1) / cnt + 31) / 32 * 32;
+    }
+    const unsigned slack = aligned ? 0u : 16u;
+    sh.lay.x_bytes = (n * bytes_of(xd) + slack + 15u) / 16u * 16u;
+    sh.lay.r_bytes = prm.res.ptr != nullptr ? (n * bytes_of(rd) + slack + 15u) / 16u * 16u : 0u;
+    const unsigned row = sh.lay.x_bytes + sh.lay.r_bytes;
+    // as many CTAs as their threads and registers allow (1024 threads an SM; half of that where a thread holds 32 values), two to
+    // four rows in flight for each
+    sh.ctas_per_sm = std::max(1u, std::min(16u, (cnt == 4 ? 512u : 1024u) / sh.threads));
+    while(sh.ctas_per_sm > 1 && 2u * row * sh.ctas_per_sm > 192u * 1024u)
+        --sh.ctas_per_sm;
+    sh.lay.stages = std::min(4u, 192u * 1024u / (row * sh.ctas_per_sm));
+    if(sh.lay.stages < 2)
+        return false;
+    sh.smem = static_cast<size_t>(sh.lay.stages) * row;
+    wait_report_targets(device, &sh.lay.report.status, &sh.lay.report.host_mirror);
+    const bool p32 = pd == OUT_F32;
+    if(xd == OUT_BF16 && rd == OUT_BF16)
+        p32 ? launch_stream_shape<OUT_BF16, OUT_BF16, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_BF16, OUT_BF16, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
+    else if(xd == OUT_BF16)
+        p32 ? launch_stream_shape<OUT_BF16, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_BF16, OUT_F32, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
+    else if(xd == OUT_F16 && rd == OUT_F16)
+        p32 ? launch_stream_shape<OUT_F16, OUT_F16, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F16, OUT_F16, OUT_F16>(prm, aligned, cnt, sh, sms, stream);
+    else if(xd == OUT_F16)
+        p32 ? launch_stream_shape<OUT_F16, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F16, OUT_F32, OUT_F16>(prm, aligned, cnt, sh, sms, stream);
+    else
+        p32 ? launch_stream_shape<OUT_F32, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F32, OUT_F32, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
+    return true;
+}
+
+void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaStream_t stream)
+{
+    const unsigned n = prm.n;
+    if(try_norm_stream(prm, aligned, device, sms, stream))
+        return;
     if(n > kLongRow)
     {
         if(aligned)
@@ -288,7 +401,7 @@ extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_
         B200_CHECK(aligned || prm.y.dt <= OUT_F32, fn, ": with an MX output every row of every argument must start on a 16-byte boundary");
         const int sms = device_sm_count(x->device_id);
         DeviceGuard guard(x->device_id);
-        launch_norm(prm, aligned, sms, static_cast<cudaStream_t>(stream));
+        launch_norm(prm, aligned, x->device_id, sms, static_cast<cudaStream_t>(stream));
     });
 }
 

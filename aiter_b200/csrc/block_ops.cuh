@@ -63,6 +63,12 @@ __device__ __forceinline__ float dec16(uint32_t bits, int dt)
     return dt == OUT_BF16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
+__device__ __forceinline__ float load_elem_any(const void* base, int dt, size_t at)
+{
+    return dt == OUT_F32 ? static_cast<const float*>(base)[at] : dec16(static_cast<const uint16_t*>(base)[at], dt);
+}
+__host__ __device__ constexpr int bytes_of_mode(int dt) { return dt == OUT_F32 ? 4 : dt == OUT_E2M1 || dt == OUT_MXFP8 ? 1 : 2; }
+
 // ---- raw vectors: VEC = 8 elements as one or two 16-byte loads, VEC = 1 one element
 template <int VEC, bool B32>
 struct Raw

@@ -54,12 +54,34 @@ constexpr uint32_t ST_TIMEOUT_MMA_SF   = 0x103;
 constexpr uint32_t ST_TIMEOUT_SFWARP   = 0x104;
 constexpr uint32_t ST_TIMEOUT_EPILOGUE = 0x105;
 constexpr uint32_t ST_TIMEOUT_DRAIN    = 0x106;
+constexpr uint32_t ST_TIMEOUT_ROWS     = 0x107; // a row copy of the streaming norm
 
 __device__ __forceinline__ uint64_t global_timer_ns()
 {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t)::"memory");
     return t;
+}
+
+// Where a kernel outside the GEMM translation unit leaves the code of a wait that ran out (the host fills it in)
+struct WaitReport
+{
+    unsigned int* status;      // the device status record
+    unsigned int* host_mirror; // pinned host word read before every launch (may be null)
+};
+__device__ __forceinline__ void report_timeout(const WaitReport& r, uint32_t code, uint32_t detail)
+{
+    if(r.status != nullptr && atomicCAS(r.status, 0u, code) == 0u)
+    {
+        r.status[1] = blockIdx.x;
+        r.status[2] = 0;
+        r.status[3] = detail;
+        if(r.host_mirror != nullptr)
+        {
+            *reinterpret_cast<volatile unsigned int*>(r.host_mirror) = code;
+            __threadfence_system();
+        }
+    }
 }
 
 // Wait for an mbarrier phase for at most c_wait_ctl.limit_ns of wall time.  Returns false when the wait

@@ -263,6 +263,21 @@ int device_sm_count(int device)
     return n;
 }
 
+void wait_report_targets(int device, unsigned int** status, unsigned int** host_mirror)
+{
+    int prev = 0;
+    B200_CUDA(cudaGetDevice(&prev));
+    if(prev != device)
+        B200_CUDA(cudaSetDevice(device));
+    std::lock_guard<std::mutex> lk(g_mutex);
+    DeviceState& st = device_state(device);
+    if(prev != device)
+        cudaSetDevice(prev);
+    require_healthy(st, device);
+    *status      = st.status;
+    *host_mirror = st.wait_ctl.host_mirror;
+}
+
 void read_device_status(int device, unsigned int out_words[4])
 {
     int prev = 0;

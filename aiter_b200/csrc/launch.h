@@ -162,6 +162,8 @@ void set_wait_control(int device, unsigned long long limit_ns, int withhold_scal
 unsigned long long launch_count();
 void count_launch(); // kernels launched outside launch.cu report themselves here
 int device_sm_count(int device);
+// Device status record and pinned mirror of a device, for kernels launched outside launch.cu; refuses while a record is pending
+void wait_report_targets(int device, unsigned int** status, unsigned int** host_mirror);
 bool programmatic_launch_enabled(); // launches carry the programmatic-serialization attribute
 
 } // namespace b200

@@ -206,8 +206,19 @@ void launch_stream(const NormParams& prm, const StreamShape& sh, int sms, cudaSt
 template <int XD, int RD, int PD>
 void launch_stream_shape(const NormParams& prm, bool aligned, unsigned cnt, const StreamShape& sh, int sms, cudaStream_t stream)
 {
+    if(cnt == 0)
+    {
+        // short rows: 8 warps a CTA, each 4 groups of 32 / lanes rows
+        const unsigned lanes = prm.n <= 64 ? 8 : prm.n <= 128 ? 16 : 32;
+        const unsigned per   = 8 * 4 * (32 / lanes);
+        const dim3 grid((prm.M + per - 1) / per), block(256);
+        lanes == 8    ? launch(norm_short_kernel<XD, RD, PD, 8>, grid, block, stream, prm)
+        : lanes == 16 ? launch(norm_short_kernel<XD, RD, PD, 16>, grid, block, stream, prm)
+                      : launch(norm_short_kernel<XD, RD, PD, 32>, grid, block, stream, prm);
+        return;
+    }
     if(!aligned)
-        cnt == 8 ? launch_stream<XD, RD, PD, 1, 8>(prm, sh, sms, stream) : launch_stream<XD, RD, PD, 1, 16>(prm, sh, sms, stream);
+        cnt == 4 ? launch_stream<XD, RD, PD, 2, 4>(prm, sh, sms, stream) : launch_stream<XD, RD, PD, 2, 8>(prm, sh, sms, stream);
     else if(cnt == 1)
         launch_stream<XD, RD, PD, 8, 1>(prm, sh, sms, stream);
     else if(cnt == 2)
@@ -221,7 +232,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
 {
     const unsigned n = prm.n;
     const int xd = prm.x.dt, rd = prm.res.ptr != nullptr ? prm.res.dt : (prm.h.ptr != nullptr ? prm.h.dt : xd);
-    if(prm.M <= 2u * static_cast<unsigned>(sms) || n < 64 || (prm.h.ptr != nullptr && prm.h.dt != rd))
+    if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && n < 64) || (prm.h.ptr != nullptr && prm.h.dt != rd))
         return false;
     // one type for all parameters
     int pd = -1;
@@ -242,31 +253,40 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     unsigned cnt;
     if(aligned)
     {
-        if(n > 16384)
+        if(n > kLongRow)
             return false;
-        cnt        = n > 8192 ? 4 : n > 1024 ? 2 : 1;
-        sh.threads = ((n + 8 * cnt - 1) / (8 * cnt) + 31) / 32 * 32;
+        cnt        = n > 8192 ? 4 : n > 512 ? 2 : n > 256 ? 1 : 0; // (0: the short-row kernel)
+        sh.threads = cnt == 0 ? 256 : ((n + 8 * cnt - 1) / (8 * cnt) + 31) / 32 * 32;
     }
     else
     {
         if(n > 8192)
             return false;
-        cnt        = n > 2048 ? 16 : 8;
-        sh.threads = ((n + cnt - 1) / cnt + 31) / 32 * 32;
+        cnt        = n > 2048 ? 8 : 4;
+        sh.threads = ((n + 2 * cnt - 1) / (2 * cnt) + 31) / 32 * 32;
     }
     const unsigned slack = aligned ? 0u : 16u;
     sh.lay.x_bytes = (n * bytes_of(xd) + slack + 15u) / 16u * 16u;
     sh.lay.r_bytes = prm.res.ptr != nullptr ? (n * bytes_of(rd) + slack + 15u) / 16u * 16u : 0u;
     const unsigned row = sh.lay.x_bytes + sh.lay.r_bytes;
-    // as many CTAs as their threads and registers allow (1024 threads an SM; half of that where a thread holds 32 values), two to
-    // four rows in flight for each
-    sh.ctas_per_sm = std::max(1u, std::min(16u, (cnt == 4 ? 512u : 1024u) / sh.threads));
-    while(sh.ctas_per_sm > 1 && 2u * row * sh.ctas_per_sm > 192u * 1024u)
+    // 1024 threads an SM (512 at 32 values a thread), two to four rows in flight for each CTA.  Aligned rows read the parameters
+    // through L1: several vectors of them want 100 KB of the SM's memory left to it (16384 x 8192 with three: 219 us with
+    // 192 KB of rows in flight, 198 with 128; with one: 173 and 191).  Unaligned rows keep them in shared memory.
+    unsigned params = 0;
+    for(const RowParam* p : {&prm.weight, &prm.bias, &prm.post_weight, &prm.post_bias, &prm.gate})
+        params += (p->ptr != nullptr && !(p == &prm.gate && prm.gate_scalar)) ? 1u : 0u;
+    sh.lay.param_pitch    = (n + 3) / 4 * 4;
+    const unsigned fixed  = aligned ? 0u : params * sh.lay.param_pitch * 4u;
+    const unsigned budget = (aligned && params * n * (pd == OUT_F32 ? 4u : 2u) > 20u * 1024u ? 128u : 192u) * 1024u;
+    sh.ctas_per_sm        = std::max(1u, std::min(16u, (cnt == 4 && aligned ? 512u : 1024u) / sh.threads));
+    while(sh.ctas_per_sm > 1 && (2u * row + fixed) * sh.ctas_per_sm > 192u * 1024u)
         --sh.ctas_per_sm;
-    sh.lay.stages = std::min(4u, 192u * 1024u / (row * sh.ctas_per_sm));
-    if(sh.lay.stages < 2)
+    const unsigned share = budget / sh.ctas_per_sm;
+    sh.lay.stages        = std::min(4u, std::max(2u, share > fixed ? (share - fixed) / row : 0u));
+    if((sh.lay.stages * row + fixed) * sh.ctas_per_sm > 200u * 1024u)
         return false;
-    sh.smem = static_cast<size_t>(sh.lay.stages) * row;
+    sh.lay.param_off = sh.lay.stages * row;
+    sh.smem = static_cast<size_t>(sh.lay.stages) * row + fixed;
     wait_report_targets(device, &sh.lay.report.status, &sh.lay.report.host_mirror);
     const bool p32 = pd == OUT_F32;
     if(xd == OUT_BF16 && rd == OUT_BF16)

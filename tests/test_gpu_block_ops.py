@@ -99,6 +99,23 @@ CASES = [
     (2, 20001, "fp16", "fp32", {"post": True, "norm": "layer", "post_bias": True}),
     (4, 2051, "bf16", None, {"gate": "channel"}),
     (9, 16383, "bf16", "bf16", {"norm": "layer"}),
+    # many rows: the streaming kernels, aligned and not, every width class
+    (1200, 64, "bf16", "bf16", {"post": True, "gate": "channel16"}),
+    (999, 40, "fp16", "fp32", {"norm": "layer", "bias": True, "gate": "token"}),
+    (3001, 128, "bf16", "fp32", {"norm": "layer", "bias": True, "post": True, "post_bias": True}),
+    (640, 256, "fp32", "fp32", {"gate": "sample4", "affine": "sample4", "offset": 1.0, "bias": True}),
+    (600, 200, "bf16", None, {"gate": "channel16", "scale": 0.5}),
+    (500, 328, "bf16", "bf16", {"post": True, "gate": "token16"}),
+    (444, 1152, "bf16", "fp32", {"norm": "layer", "affine": "sample4", "offset": 1.0, "bias": True, "gate": "sample4", "post": True}),
+    (400, 1155, "bf16", "fp32", {"norm": "layer", "affine": "sample4", "offset": 1.0, "bias": True, "gate": "sample4", "post": True, "post_bias": True}),
+    (500, 101, "fp16", "fp16", {"post": True, "norm": "layer", "post_bias": True}),
+    (350, 8191, "bf16", "bf16", {"post": True, "norm": "layer"}),
+    (333, 4098, "fp32", "fp32", {}),
+    (300, 16384, "fp16", "fp32", {"post": True, "gate": "token"}),
+    (299, 12296, "bf16", "bf16", {"norm": "layer", "bias": True, "post": True}),
+    (450, 8192, "bf16", "bf16", {"post": True, "gate": "channel16", "scale": 0.5, "post_bias": True}),
+    (310, 9001, "bf16", "bf16", {"post": True}),
+    (400, 512, "bf16", "fp16", {"gate": "channel"}),
 ]
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
@@ -110,23 +127,26 @@ def make(case, seed=0):
     def param(kind):
         if kind == "channel":
             return randn(g, n, dtype=torch.float32, scale=0.5)
-        if kind == "token":
+        if kind == "channel16":  # of x's own type, like the other parameters
+            return randn(g, n, dtype=DT[x], scale=0.5)
+        if kind.startswith("token"):
             return randn(g, m, 1, dtype=torch.bfloat16)
-        return randn(g, int(kind[6:]), n, dtype=torch.float16, scale=0.5)
+        return randn(g, int(kind[6:]), n, dtype=torch.float16 if m < 296 else DT[x], scale=0.5)
 
     args = {"x": randn(g, m, n, dtype=DT[x], scale=2.0) + 0.25, "norm": o.get("norm", "rms"), "eps": 1e-5,
             "residual_scale": o.get("scale", 1.0), "weight_offset": o.get("offset", 0.0)}
     if residual:
         args["residual"] = randn(g, m, n, dtype=DT[residual], scale=3.0)
-    args["weight"] = param(o["affine"]) if "affine" in o else randn(g, n, dtype=torch.bfloat16)
+    few = m < 296  # few rows: parameters of several types; many: of x's, as the streaming kernels want them
+    args["weight"] = param(o["affine"]) if "affine" in o else randn(g, n, dtype=torch.bfloat16 if few else DT[x])
     if o.get("bias"):
-        args["bias"] = param(o["affine"]) if "affine" in o else randn(g, n, dtype=torch.float32)
+        args["bias"] = param(o["affine"]) if "affine" in o else randn(g, n, dtype=torch.float32 if few else DT[x])
     if "gate" in o:
         args["gate"] = param(o["gate"])
     if o.get("post"):
-        args["post_weight"] = randn(g, n, dtype=torch.bfloat16)
+        args["post_weight"] = randn(g, n, dtype=torch.bfloat16 if few else DT[x])
         if o.get("post_bias"):
-            args["post_bias"] = randn(g, n, dtype=torch.bfloat16)
+            args["post_bias"] = randn(g, n, dtype=torch.bfloat16 if few else DT[x])
     return args
 
 
@@ -176,7 +196,7 @@ def test_norm_strides_leading_dimensions_and_in_place(ab):
     check(y3, want[0], want[2], "y unaligned")
 
 
-@pytest.mark.parametrize("m,n", [(1, 32), (33, 320), (300, 1024), (65, 7168), (700, 2176), (2, 20480)])
+@pytest.mark.parametrize("m,n", [(1, 32), (33, 320), (300, 1024), (65, 7168), (700, 2176), (2, 20480), (1001, 32), (777, 128), (545, 224), (301, 416), (333, 8192), (297, 9216)])
 @pytest.mark.parametrize("fp4", [False, True])
 @pytest.mark.parametrize("layout", [False, True, 2])
 def test_norm_mx_output_is_the_quantised_fp32_output(ab, m, n, fp4, layout):

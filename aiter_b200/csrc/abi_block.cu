@@ -179,32 +179,51 @@ void launch_norm_rows(const NormParams& prm, dim3 grid, dim3 block, cudaStream_t
         launch(norm_rows_kernel<VEC, CNT, false, false>, grid, block, stream, prm);
 }
 
-// ---- many rows: the streaming kernel, for the usual types (types that differ more run the general kernel)
+// ---- many rows: the streaming kernels, for the usual types (types that differ more run the general kernels)
 struct StreamShape
 {
-    unsigned threads, ctas_per_sm;
+    unsigned threads;
+    unsigned fixed;  // bytes of shared memory besides the rows
+    unsigned budget; // bytes an SM's CTAs may use for rows in flight
+    bool flat;       // the kernel for rows of any width: a grid that is a multiple of 8
     NormStreamLayout lay;
-    size_t smem;
 };
 
-template <int XD, int RD, int PD, int VEC, int CNT>
-void launch_stream(const NormParams& prm, const StreamShape& sh, int sms, cudaStream_t stream)
+using StreamKernel = void (*)(NormParams, NormStreamLayout);
+template <StreamKernel kernel>
+bool launch_stream(const NormParams& prm, StreamShape sh, int sms, cudaStream_t stream)
 {
-    auto kernel = norm_stream_kernel<XD, RD, PD, VEC, CNT>;
     static std::atomic<unsigned long long> attr_done{0}; // a bit per device
+    static std::atomic<unsigned> regs{0};
     int dev = 0;
     B200_CUDA(cudaGetDevice(&dev));
     if(dev >= 64 || !((attr_done.load() >> dev) & 1))
     {
         B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        cudaFuncAttributes attr{};
+        B200_CUDA(cudaFuncGetAttributes(&attr, kernel));
+        regs = static_cast<unsigned>(attr.numRegs);
         if(dev < 64)
             attr_done.fetch_or(1ull << dev);
     }
-    const unsigned grid = std::min<unsigned>(prm.M, static_cast<unsigned>(sms) * sh.ctas_per_sm);
-    launch_smem(kernel, dim3(grid), dim3(sh.threads), sh.smem, stream, prm, sh.lay);
+    // as many CTAs as the registers allow, two to four rows in flight for each
+    const unsigned row = sh.lay.x_bytes + sh.lay.r_bytes;
+    unsigned ctas      = std::max(1u, std::min({24u, 2048u / sh.threads, 65536u / ((regs + 7) / 8 * 8 * sh.threads)}));
+    while(ctas > 1 && (2u * row + sh.fixed) * ctas > 192u * 1024u)
+        --ctas;
+    const unsigned share = sh.budget / ctas;
+    sh.lay.stages        = std::min(4u, std::max(2u, share > sh.fixed ? (share - sh.fixed) / row : 0u));
+    if((sh.lay.stages * row + sh.fixed) * ctas > 200u * 1024u)
+        return false;
+    sh.lay.param_off = sh.lay.stages * row;
+    unsigned grid    = std::min(prm.M, static_cast<unsigned>(sms) * ctas);
+    if(sh.flat)
+        grid = std::max(8u, grid / 8 * 8);
+    launch_smem(kernel, dim3(grid), dim3(sh.threads), static_cast<size_t>(sh.lay.stages) * row + sh.fixed, stream, prm, sh.lay);
+    return true;
 }
 template <int XD, int RD, int PD>
-void launch_stream_shape(const NormParams& prm, bool aligned, unsigned cnt, const StreamShape& sh, int sms, cudaStream_t stream)
+bool launch_stream_shape(const NormParams& prm, unsigned cnt, const StreamShape& sh, int sms, cudaStream_t stream)
 {
     if(cnt == 0)
     {
@@ -215,16 +234,27 @@ void launch_stream_shape(const NormParams& prm, bool aligned, unsigned cnt, cons
         lanes == 8    ? launch(norm_short_kernel<XD, RD, PD, 8>, grid, block, stream, prm)
         : lanes == 16 ? launch(norm_short_kernel<XD, RD, PD, 16>, grid, block, stream, prm)
                       : launch(norm_short_kernel<XD, RD, PD, 32>, grid, block, stream, prm);
-        return;
+        return true;
     }
-    if(!aligned)
-        cnt == 4 ? launch_stream<XD, RD, PD, 2, 4>(prm, sh, sms, stream) : launch_stream<XD, RD, PD, 2, 8>(prm, sh, sms, stream);
-    else if(cnt == 1)
-        launch_stream<XD, RD, PD, 8, 1>(prm, sh, sms, stream);
-    else if(cnt == 2)
-        launch_stream<XD, RD, PD, 8, 2>(prm, sh, sms, stream);
-    else
-        launch_stream<XD, RD, PD, 8, 4>(prm, sh, sms, stream);
+    if(sh.flat)
+        return cnt == 1 ? launch_stream<norm_stream_flat_kernel<XD, RD, PD, 1>>(prm, sh, sms, stream) : launch_stream<norm_stream_flat_kernel<XD, RD, PD, 2>>(prm, sh, sms, stream);
+    if(cnt == 1)
+        return launch_stream<norm_stream_kernel<XD, RD, PD, 1, false>>(prm, sh, sms, stream);
+    if(cnt == 4)
+        return launch_stream<norm_stream_kernel<XD, RD, PD, 4, false>>(prm, sh, sms, stream);
+    return prm.n == 16 * sh.threads ? launch_stream<norm_stream_kernel<XD, RD, PD, 2, true>>(prm, sh, sms, stream)
+                                    : launch_stream<norm_stream_kernel<XD, RD, PD, 2, false>>(prm, sh, sms, stream);
+}
+
+// Whether element 0 of every row has the same place in its group of eight elements in all of x, residual, h and y, with the groups
+// aligned to their size
+bool same_phase(const NormParams& prm)
+{
+    auto first = [](const RowTensor& v) { return reinterpret_cast<uintptr_t>(v.ptr) / bytes_of(v.dt); };
+    for(const RowTensor* v : {&prm.res, &prm.h, &prm.y})
+        if(v->ptr != nullptr && (((first(*v) ^ first(prm.x)) & 7) != 0 || ((v->ld ^ prm.x.ld) & 7) != 0))
+            return false;
+    return true;
 }
 
 // Returns false where the general kernels have to serve the call.
@@ -235,7 +265,8 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && n < 64) || (prm.h.ptr != nullptr && prm.h.dt != rd))
         return false;
     // one type for all parameters
-    int pd = -1;
+    int pd          = -1;
+    unsigned params = 0;
     for(const RowParam* p : {&prm.weight, &prm.bias, &prm.post_weight, &prm.post_bias, &prm.gate})
     {
         if(p->ptr == nullptr || (p == &prm.gate && prm.gate_scalar))
@@ -243,6 +274,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
         if(pd >= 0 && pd != p->dt)
             return false;
         pd = p->dt;
+        ++params;
     }
     const int half = xd == OUT_F32 ? (rd == OUT_F32 ? OUT_BF16 : rd) : xd; // the call's 16-bit type
     if(pd < 0)
@@ -250,56 +282,47 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     if((xd != OUT_F32 && rd != OUT_F32 && xd != rd) || (xd == OUT_F32 && rd != OUT_F32) || (pd != OUT_F32 && pd != half))
         return false;
     StreamShape sh{};
-    unsigned cnt;
+    unsigned cnt, elems = n;
+    const unsigned param_bytes = pd == OUT_F32 ? 4u : 2u;
     if(aligned)
     {
         if(n > kLongRow)
             return false;
         cnt        = n > 8192 ? 4 : n > 512 ? 2 : n > 256 ? 1 : 0; // (0: the short-row kernel)
         sh.threads = cnt == 0 ? 256 : ((n + 8 * cnt - 1) / (8 * cnt) + 31) / 32 * 32;
+        // The parameters are read through L1: several vectors of them want 100 KB of the SM's memory left to it (16384 x 8192 with
+        // three: 219 us with 192 KB of rows in flight, 198 with 128; with one: 173 and 191).
+        sh.budget = (params * n * param_bytes > 20u * 1024u ? 128u : 192u) * 1024u;
     }
     else
     {
-        if(n > 8192)
+        // groups of eight elements have to be aligned in every tensor at once
+        if(n > 8000 || !same_phase(prm))
             return false;
-        cnt        = n > 2048 ? 8 : 4;
-        sh.threads = ((n + 2 * cnt - 1) / (2 * cnt) + 31) / 32 * 32;
+        elems      = (n + 14) / 8 * 8; // (a row touches at most that many elements in whole groups)
+        cnt        = n > 512 ? 2 : 1;
+        sh.threads = (elems / 8 + cnt - 1) / cnt;
+        sh.threads = (sh.threads + 31) / 32 * 32;
+        sh.flat    = true;
+        sh.budget  = 192u * 1024u;
+        sh.lay.param_pitch = elems * param_bytes;
+        sh.fixed           = params * sh.lay.param_pitch;
     }
-    const unsigned slack = aligned ? 0u : 16u;
-    sh.lay.x_bytes = (n * bytes_of(xd) + slack + 15u) / 16u * 16u;
-    sh.lay.r_bytes = prm.res.ptr != nullptr ? (n * bytes_of(rd) + slack + 15u) / 16u * 16u : 0u;
-    const unsigned row = sh.lay.x_bytes + sh.lay.r_bytes;
-    // 1024 threads an SM (512 at 32 values a thread), two to four rows in flight for each CTA.  Aligned rows read the parameters
-    // through L1: several vectors of them want 100 KB of the SM's memory left to it (16384 x 8192 with three: 219 us with
-    // 192 KB of rows in flight, 198 with 128; with one: 173 and 191).  Unaligned rows keep them in shared memory.
-    unsigned params = 0;
-    for(const RowParam* p : {&prm.weight, &prm.bias, &prm.post_weight, &prm.post_bias, &prm.gate})
-        params += (p->ptr != nullptr && !(p == &prm.gate && prm.gate_scalar)) ? 1u : 0u;
-    sh.lay.param_pitch    = (n + 3) / 4 * 4;
-    const unsigned fixed  = aligned ? 0u : params * sh.lay.param_pitch * 4u;
-    const unsigned budget = (aligned && params * n * (pd == OUT_F32 ? 4u : 2u) > 20u * 1024u ? 128u : 192u) * 1024u;
-    sh.ctas_per_sm        = std::max(1u, std::min(16u, (cnt == 4 && aligned ? 512u : 1024u) / sh.threads));
-    while(sh.ctas_per_sm > 1 && (2u * row + fixed) * sh.ctas_per_sm > 192u * 1024u)
-        --sh.ctas_per_sm;
-    const unsigned share = budget / sh.ctas_per_sm;
-    sh.lay.stages        = std::min(4u, std::max(2u, share > fixed ? (share - fixed) / row : 0u));
-    if((sh.lay.stages * row + fixed) * sh.ctas_per_sm > 200u * 1024u)
-        return false;
-    sh.lay.param_off = sh.lay.stages * row;
-    sh.smem = static_cast<size_t>(sh.lay.stages) * row + fixed;
+    sh.lay.x_bytes = elems * bytes_of(xd);
+    sh.lay.r_bytes = prm.res.ptr != nullptr ? elems * bytes_of(rd) : 0u;
     wait_report_targets(device, &sh.lay.report.status, &sh.lay.report.host_mirror);
-    const bool p32 = pd == OUT_F32;
-    if(xd == OUT_BF16 && rd == OUT_BF16)
-        p32 ? launch_stream_shape<OUT_BF16, OUT_BF16, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_BF16, OUT_BF16, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
-    else if(xd == OUT_BF16)
-        p32 ? launch_stream_shape<OUT_BF16, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_BF16, OUT_F32, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
-    else if(xd == OUT_F16 && rd == OUT_F16)
-        p32 ? launch_stream_shape<OUT_F16, OUT_F16, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F16, OUT_F16, OUT_F16>(prm, aligned, cnt, sh, sms, stream);
-    else if(xd == OUT_F16)
-        p32 ? launch_stream_shape<OUT_F16, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F16, OUT_F32, OUT_F16>(prm, aligned, cnt, sh, sms, stream);
-    else
-        p32 ? launch_stream_shape<OUT_F32, OUT_F32, OUT_F32>(prm, aligned, cnt, sh, sms, stream) : launch_stream_shape<OUT_F32, OUT_F32, OUT_BF16>(prm, aligned, cnt, sh, sms, stream);
-    return true;
+    auto run = [&](auto x, auto r) {
+        constexpr int XD = decltype(x)::value, RD = decltype(r)::value, HD = XD == OUT_F32 ? OUT_BF16 : XD;
+        return pd == OUT_F32 ? launch_stream_shape<XD, RD, OUT_F32>(prm, cnt, sh, sms, stream) : launch_stream_shape<XD, RD, HD>(prm, cnt, sh, sms, stream);
+    };
+    using B = std::integral_constant<int, OUT_BF16>;
+    using H = std::integral_constant<int, OUT_F16>;
+    using F = std::integral_constant<int, OUT_F32>;
+    if(xd == OUT_BF16)
+        return rd == OUT_BF16 ? run(B{}, B{}) : run(B{}, F{});
+    if(xd == OUT_F16)
+        return rd == OUT_F16 ? run(H{}, H{}) : run(H{}, F{});
+    return run(F{}, F{});
 }
 
 void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaStream_t stream)

@@ -180,28 +180,51 @@ __device__ __forceinline__ void st_vec(void* base, int dt, size_t at, const floa
     }
 }
 
+// largest magnitude of three values; a NaN among them survives
+__device__ __forceinline__ float amax3(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// UE8M0 byte of a block with largest magnitude `ab` (bits, sign-less): the exponent of ab / max_pos rounded up.  With
+// max_pos = 1.75 * 2^8 (e4m3) or 1.5 * 2^2 (e2m1) the division only decides whether the significand of ab is above that of
+// max_pos - the two floats around a significand of 1.75 or 1.5 divide to values on their own side of 1 -, so for normal quotients
+// one addition carries into the exponent.  Zero, quotients below the normal range, infinity and NaN take the division itself.
+template <bool FP4>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t ab)
+{
+    if(ab - (16u << 23) < (0x7F800000u - (16u << 23)))
+        return ((ab + (FP4 ? 0x3FFFFFu : 0x1FFFFFu)) >> 23) - (FP4 ? 2u : 8u);
+    const uint32_t qb = __float_as_uint(__fdiv_rn(__uint_as_float(ab), FP4 ? 6.0f : 448.0f));
+    const uint32_t ex = (qb >> 23) & 0xFFu;
+    return ex + (((qb & 0x7FFFFFu) != 0u && ex < 0xFFu) ? 1u : 0u);
+}
+
 // ---- one 32-element block held by four neighbouring lanes, eight values each
-// Returns the UE8M0 byte (the same in the four lanes); q: 8 e4m3 bytes in q[0..1], or 8 e2m1 codes in q[0].  The maximum is
-// taken on the sign-less bit patterns, whose integer order is the order of the values with NaN on top.
+// Returns the UE8M0 byte (the same in the four lanes); q: 8 e4m3 bytes in q[0..1], or 8 e2m1 codes in q[0].
 template <bool FP4>
 __device__ __forceinline__ uint32_t mx_block(const float (&v)[8], uint32_t (&q)[2])
 {
-    uint32_t ab = 0;
-#pragma unroll
-    for(int i = 0; i < 8; ++i)
-        ab = max(ab, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    ab = max(ab, __shfl_xor_sync(0xffffffffu, ab, 1));
-    ab = max(ab, __shfl_xor_sync(0xffffffffu, ab, 2));
-    const uint32_t qb   = __float_as_uint(__fdiv_rn(__uint_as_float(ab), FP4 ? 6.0f : 448.0f));
-    const uint32_t ex   = (qb >> 23) & 0xFFu;
-    const uint32_t byte = ex + (((qb & 0x7FFFFFu) != 0u && ex < 0xFFu) ? 1u : 0u);
+    const float m = amax3(amax3(v[0], v[1], v[2]), amax3(v[3], v[4], v[5]), amax3(v[6], v[7], v[7]));
+    // (the integer order of sign-less bit patterns is the order of the values with NaN on top)
+    uint32_t ab = __float_as_uint(m);
+    ab          = max(ab, __shfl_xor_sync(0xffffffffu, ab, 1));
+    ab          = max(ab, __shfl_xor_sync(0xffffffffu, ab, 2));
+    const uint32_t byte = mx_scale_byte<FP4>(ab);
     const float rscale  = __uint_as_float(byte == 0xFFu ? 0x7F800001u : (byte == 254u ? 0x00400000u : ((254u - byte) << 23)));
+    const float2 r2     = make_float2(rscale, rscale);
+    float2 z[4];
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
+        z[i] = __fmul2_rn(make_float2(v[2 * i], v[2 * i + 1]), r2);
     if(FP4)
     {
         uint32_t packed = 0;
 #pragma unroll
         for(int i = 0; i < 4; ++i)
-            packed |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i] * rscale, v[2 * i + 1] * rscale), __NV_E2M1, cudaRoundNearest)) << (8 * i);
+            packed |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(z[i], __NV_E2M1, cudaRoundNearest)) << (8 * i);
         q[0] = packed;
         q[1] = 0;
     }
@@ -210,8 +233,8 @@ __device__ __forceinline__ uint32_t mx_block(const float (&v)[8], uint32_t (&q)[
 #pragma unroll
         for(int h = 0; h < 2; ++h)
         {
-            const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h] * rscale, v[4 * h + 1] * rscale), __NV_SATFINITE, __NV_E4M3);
-            const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * h + 2] * rscale, v[4 * h + 3] * rscale), __NV_SATFINITE, __NV_E4M3);
+            const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(z[2 * h], __NV_SATFINITE, __NV_E4M3);
+            const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(z[2 * h + 1], __NV_SATFINITE, __NV_E4M3);
             q[h] = static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
         }
     }

@@ -4,20 +4,25 @@
 // an SM always has some 50 KB of loads under way and spends less than about 25 instructions an element.  Hence: a CTA owns a
 // contiguous block of rows and keeps the next ones in flight with bulk copies (one thread, two instructions a row, no
 // registers), while the current row goes from shared memory to registers, through its one or two norms and out; a thread holds
-// 16 to 32 values, over which the fixed work of a row (two sums, addresses) is spread; types are compile-time and the arithmetic
-// is two values an instruction.
+// 16 values, over which the fixed work of a row (its sums, addresses) is spread, and types are compile-time.
 //
-// Rows that start on any address are copied from the 16-byte boundary below to the one above, and read pair by pair.
+// Rows of any width have a kernel of their own below, short rows another.
 #pragma once
 #include "block_ops.cuh"
 
 namespace b200 {
 
+// (Two scalar instructions each: the two-wide forms measured slower here, 16384 x 8192 with both norms and a gate 196 against
+// 178 us - the values come in and go out one by one, and the pairs cost moves.)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return make_float2(fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
+
 struct NormStreamLayout
 {
     unsigned x_bytes, r_bytes; // shared memory of one row, multiples of 16
     unsigned stages;
-    unsigned param_off;        // unaligned rows: where the parameters of the current entry are kept as fp32, pitch param_pitch floats
+    unsigned param_off;        // rows of any width: where the current parameters are kept, param_pitch bytes each
     unsigned param_pitch;
     WaitReport report;
 };
@@ -35,31 +40,11 @@ __device__ __forceinline__ float2 unpack2(uint32_t w)
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
-// VEC consecutive elements of a compile-time type as pairs.  VEC = 8: aligned to the vector.  VEC = 2: aligned to the element
-// only (`even`: to the pair), and the second element exists only if `two`.
-template <int DT, int VEC>
-__device__ __forceinline__ void rd_vec(const uint8_t* p, bool even, bool two, float2 (&v)[VEC / 2])
+// eight consecutive elements of a compile-time type, aligned to the vector, as pairs
+template <int DT>
+__device__ __forceinline__ void rd_vec(const uint8_t* p, float2 (&v)[4])
 {
-    if constexpr(VEC == 2)
-    {
-        if constexpr(DT == OUT_F32)
-        {
-            if(even && two)
-                v[0] = *reinterpret_cast<const float2*>(p);
-            else
-                v[0] = make_float2(reinterpret_cast<const float*>(p)[0], two ? reinterpret_cast<const float*>(p)[1] : 0.f);
-        }
-        else
-        {
-            uint32_t w;
-            if(even && two)
-                w = *reinterpret_cast<const uint32_t*>(p);
-            else
-                w = reinterpret_cast<const uint16_t*>(p)[0] | (two ? static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[1]) << 16 : 0u);
-            v[0] = unpack2<DT>(w);
-        }
-    }
-    else if constexpr(DT == OUT_F32)
+    if constexpr(DT == OUT_F32)
     {
         const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
         v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
@@ -70,36 +55,10 @@ __device__ __forceinline__ void rd_vec(const uint8_t* p, bool even, bool two, fl
         v[0] = unpack2<DT>(a.x), v[1] = unpack2<DT>(a.y), v[2] = unpack2<DT>(a.z), v[3] = unpack2<DT>(a.w);
     }
 }
-template <int DT, int VEC>
-__device__ __forceinline__ void wr_vec(uint8_t* p, bool even, bool two, const float2 (&v)[VEC / 2])
+template <int DT>
+__device__ __forceinline__ void wr_vec(uint8_t* p, const float2 (&v)[4])
 {
-    if constexpr(VEC == 2)
-    {
-        if constexpr(DT == OUT_F32)
-        {
-            if(even && two)
-                *reinterpret_cast<float2*>(p) = v[0];
-            else
-            {
-                reinterpret_cast<float*>(p)[0] = v[0].x;
-                if(two)
-                    reinterpret_cast<float*>(p)[1] = v[0].y;
-            }
-        }
-        else
-        {
-            const uint32_t w = pack_out16x2(v[0].x, v[0].y, DT == OUT_F16);
-            if(even && two)
-                *reinterpret_cast<uint32_t*>(p) = w;
-            else
-            {
-                reinterpret_cast<uint16_t*>(p)[0] = static_cast<uint16_t>(w);
-                if(two)
-                    reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w >> 16);
-            }
-        }
-    }
-    else if constexpr(DT == OUT_F32)
+    if constexpr(DT == OUT_F32)
     {
         reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
         reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
@@ -108,53 +67,46 @@ __device__ __forceinline__ void wr_vec(uint8_t* p, bool even, bool two, const fl
         *reinterpret_cast<uint4*>(p) = make_uint4(pack_out16x2(v[0].x, v[0].y, DT == OUT_F16), pack_out16x2(v[1].x, v[1].y, DT == OUT_F16),
                                                   pack_out16x2(v[2].x, v[2].y, DT == OUT_F16), pack_out16x2(v[3].x, v[3].y, DT == OUT_F16));
 }
-// every pair of a row starts on a boundary of its size
-template <int DT>
-__device__ __forceinline__ bool pairs_aligned(const void* p)
-{
-    return (reinterpret_cast<uintptr_t>(p) & (2 * esize_of(DT) - 1)) == 0;
-}
 
 // h *= offset + p  and  h += p for a parameter vector p of the row
-template <int PD, int VEC, int CNT>
-__device__ __forceinline__ void scale_by(float2 (&h)[CNT][VEC / 2], const uint8_t* p, unsigned col0, unsigned col_step, unsigned n, float offset)
+template <int PD, int CNT, bool FULL = false>
+__device__ __forceinline__ void scale_by(float2 (&h)[CNT][4], const uint8_t* p, unsigned col0, unsigned col_step, unsigned n, float offset)
 {
-    const bool even = pairs_aligned<PD>(p);
-    const float2 o  = make_float2(offset, offset);
+    const float2 o = make_float2(offset, offset);
+    const bool plain = offset == 0.f;
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
         const unsigned col = col0 + j * col_step;
-        if(col < n)
+        if(FULL || col < n)
         {
-            float2 q[VEC / 2];
-            rd_vec<PD, VEC>(p + col * esize_of(PD), even, col + 1 < n, q);
+            float2 q[4];
+            rd_vec<PD>(p + col * esize_of(PD), q);
 #pragma unroll
-            for(int k = 0; k < VEC / 2; ++k)
-                h[j][k] = __fmul2_rn(h[j][k], __fadd2_rn(q[k], o));
+            for(int k = 0; k < 4; ++k)
+                h[j][k] = mul2(h[j][k], plain ? q[k] : add2(q[k], o));
         }
     }
 }
-template <int PD, int VEC, int CNT>
-__device__ __forceinline__ void shift_by(float2 (&h)[CNT][VEC / 2], const uint8_t* p, unsigned col0, unsigned col_step, unsigned n)
+template <int PD, int CNT, bool FULL = false>
+__device__ __forceinline__ void shift_by(float2 (&h)[CNT][4], const uint8_t* p, unsigned col0, unsigned col_step, unsigned n)
 {
-    const bool even = pairs_aligned<PD>(p);
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
         const unsigned col = col0 + j * col_step;
-        if(col < n)
+        if(FULL || col < n)
         {
-            float2 q[VEC / 2];
-            rd_vec<PD, VEC>(p + col * esize_of(PD), even, col + 1 < n, q);
+            float2 q[4];
+            rd_vec<PD>(p + col * esize_of(PD), q);
 #pragma unroll
-            for(int k = 0; k < VEC / 2; ++k)
-                h[j][k] = __fadd2_rn(h[j][k], q[k]);
+            for(int k = 0; k < 4; ++k)
+                h[j][k] = add2(h[j][k], q[k]);
         }
     }
 }
 // the row's vectors as an MX operand
-template <bool FP4, int CNT>
+template <bool FP4, int CNT, bool FULL = false>
 __device__ __forceinline__ void emit_mx(const BlockScales& sf, uint8_t* y, unsigned row, unsigned col0, unsigned col_step, unsigned n, const float2 (&h)[CNT][4])
 {
     uint8_t* const sf_row = sf.ptr + sf_offset(sf, row, 0); // (block 0; the others lie at offsets that do not depend on the row)
@@ -162,7 +114,7 @@ __device__ __forceinline__ void emit_mx(const BlockScales& sf, uint8_t* y, unsig
     for(int j = 0; j < CNT; ++j)
     {
         const unsigned col = col0 + j * col_step;
-        const bool in      = col < n;
+        const bool in      = FULL || col < n;
         const float f[8]   = {h[j][0].x, h[j][0].y, h[j][1].x, h[j][1].y, h[j][2].x, h[j][2].y, h[j][3].x, h[j][3].y};
         uint32_t q[2];
         uint32_t byte = mx_block<FP4>(f, q);
@@ -187,20 +139,19 @@ __device__ __forceinline__ void emit_mx(const BlockScales& sf, uint8_t* y, unsig
     }
 }
 
-// XD, RD: types of x and of the residual and h; PD: of every parameter of more than one value.  A thread holds CNT vectors of VEC
-// elements, vector j at element (j * threads + t) * VEC.
-template <int XD, int RD, int PD, int VEC, int CNT>
-__global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kernel(const __grid_constant__ NormParams prm, const __grid_constant__ NormStreamLayout lay)
+// XD, RD: types of x and of the residual and h; PD: of every parameter of more than one value.  A thread holds CNT vectors of eight
+// elements, vector j at element (j * threads + t) * 8; FULL: exactly the row, no vector lies behind it.
+template <int XD, int RD, int PD, int CNT, bool FULL>
+__global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(const __grid_constant__ NormParams prm, const __grid_constant__ NormStreamLayout lay)
 {
-    constexpr int P = VEC / 2;
+    constexpr int P = 4;
     constexpr int XS = esize_of(XD), RS = esize_of(RD), PS = esize_of(PD);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float red[8][32]; // two sets of slots, for even and odd rows: one barrier a sum is enough
     __shared__ __align__(8) uint64_t full[4];
     const unsigned t = threadIdx.x, T = blockDim.x, n = prm.n;
-    const bool has_res = prm.res.ptr != nullptr, has_h = prm.h.ptr != nullptr, has_w = prm.weight.ptr != nullptr, has_b = prm.bias.ptr != nullptr;
-    const bool post = prm.post != 0, has_pw = prm.post_weight.ptr != nullptr, has_pb = prm.post_bias.ptr != nullptr;
-    const bool gate_vec = prm.gate.ptr != nullptr && !prm.gate_scalar, gate_one = prm.gate.ptr != nullptr && prm.gate_scalar;
+    const bool has_res = prm.res.ptr != nullptr;
+    const bool gate_one = prm.gate.ptr != nullptr && prm.gate_scalar;
     // this CTA's rows: the first `extra` CTAs take one more
     const unsigned per = prm.M / gridDim.x, extra = prm.M % gridDim.x;
     const unsigned row0 = blockIdx.x * per + min(blockIdx.x, extra);
@@ -216,75 +167,47 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
     __syncthreads();
     grid_dependency_wait();
     grid_launch_dependents();
-    const uint8_t* xg = static_cast<const uint8_t*>(prm.x.ptr) + static_cast<size_t>(row0) * prm.x.ld * XS;
-    const uint8_t* rg = static_cast<const uint8_t*>(prm.res.ptr) + static_cast<size_t>(row0) * prm.res.ld * RS;
-    auto load = [&](const uint8_t* xp, const uint8_t* rp, unsigned s) { // a row into stage s, by one thread
+    auto load = [&](unsigned row, unsigned s) { // a row into stage s, by one thread
         const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + s * stage_bytes;
-        const unsigned xo  = VEC == 8 ? 0u : static_cast<unsigned>(reinterpret_cast<uintptr_t>(xp) & 15);
-        const unsigned ro  = VEC == 8 ? 0u : static_cast<unsigned>(reinterpret_cast<uintptr_t>(rp) & 15);
-        const unsigned xb  = (xo + n * XS + 15u) & ~15u;
-        const unsigned rb  = has_res ? (ro + n * RS + 15u) & ~15u : 0u;
-        mbar_arrive_expect_tx(bar, xb + rb);
-        bulk_load(dst, xp - xo, xb, bar);
+        mbar_arrive_expect_tx(bar, stage_bytes);
+        bulk_load(dst, static_cast<const uint8_t*>(prm.x.ptr) + static_cast<size_t>(row) * prm.x.ld * XS, lay.x_bytes, bar);
         if(has_res)
-            bulk_load(dst + lay.x_bytes, rp - ro, rb, bar);
+            bulk_load(dst + lay.x_bytes, static_cast<const uint8_t*>(prm.res.ptr) + static_cast<size_t>(row) * prm.res.ld * RS, lay.r_bytes, bar);
     };
-    const size_t x_step = static_cast<size_t>(prm.x.ld) * XS, r_step = static_cast<size_t>(prm.res.ld) * RS;
     if(t == 0)
         for(unsigned i = 0; i < min(S, rows); ++i)
-            load(xg + i * x_step, rg + i * r_step, i);
-    const unsigned y_size = bytes_of_mode(prm.y.dt);
-    uint8_t* hg = static_cast<uint8_t*>(prm.h.ptr) + static_cast<size_t>(row0) * prm.h.ld * RS;
-    uint8_t* yg = static_cast<uint8_t*>(prm.y.ptr) + static_cast<size_t>(row0) * prm.y.ld * y_size;
-    const size_t h_step = static_cast<size_t>(prm.h.ld) * RS, y_step = static_cast<size_t>(prm.y.ld) * y_size;
-    // The parameters' entries of the current row, until row `change`.  With unaligned rows they are kept in shared memory as fp32
-    // (an entry of an odd number of 16-bit values is as unaligned as the rows, and every row of the CTA reads it again).
-    constexpr int QD = VEC == 2 ? OUT_F32 : PD;
-    const uint8_t *w = nullptr, *b = nullptr, *pw = nullptr, *pb = nullptr, *pg = nullptr;
-    float gate1     = 1.f;
-    unsigned change = 0xFFFFFFFFu;
-    auto entries    = [&](unsigned row) {
-        int k     = 0;
-        auto take = [&](const RowParam& q, const uint8_t*& at) {
-            const uint8_t* src = static_cast<const uint8_t*>(q.ptr) + param_at(q, row) * PS;
-            if(q.ld != 0)
-                change = min(change, (row / q.rows_per + 1) * q.rows_per);
-            at = src;
-            if(VEC == 2 && q.ptr != nullptr)
-            {
-                float* dst = reinterpret_cast<float*>(smem + lay.param_off) + (k++) * lay.param_pitch;
-                for(unsigned e = t; e < n; e += T)
-                    dst[e] = load_elem_any(src, PD, e);
-                at = reinterpret_cast<const uint8_t*>(dst);
-            }
+            load(row0 + i, i);
+    // the parameters' entries of the current row, until row `change`: indexes, since registers are what two CTAs an SM leave
+    // short (addresses are formed where they are used, from the parameter bank)
+    unsigned ew = 0, eb = 0, epw = 0, epb = 0, eg = 0, change = 0;
+    float gate1  = 1.f;
+    auto entries = [&](unsigned row) {
+        change    = 0xFFFFFFFFu;
+        auto take = [&](const RowParam& q) {
+            if(q.ld == 0)
+                return 0u;
+            const unsigned e = row / q.rows_per;
+            change           = min(change, (e + 1) * q.rows_per);
+            return e;
         };
-        change = 0xFFFFFFFFu;
-        if(VEC == 2)
-            __syncthreads(); // nobody reads the previous entries any more
-        take(prm.weight, w);
-        take(prm.bias, b);
-        take(prm.post_weight, pw);
-        take(prm.post_bias, pb);
-        if(gate_vec)
-            take(prm.gate, pg);
-        else if(gate_one)
-        {
-            if(prm.gate.ld != 0)
-                change = min(change, (row / prm.gate.rows_per + 1) * prm.gate.rows_per);
-            gate1 = load_elem_any(prm.gate.ptr, prm.gate.dt, param_at(prm.gate, row));
-        }
-        if(VEC == 2)
-            __syncthreads();
+        ew  = take(prm.weight);
+        eb  = take(prm.bias);
+        epw = take(prm.post_weight);
+        epb = take(prm.post_bias);
+        eg  = take(prm.gate);
+        if(gate_one)
+            gate1 = load_elem_any(prm.gate.ptr, prm.gate.dt, static_cast<size_t>(eg) * prm.gate.ld);
     };
-    entries(row0);
+    auto entry = [&](const RowParam& q, unsigned e) { return static_cast<const uint8_t*>(q.ptr) + static_cast<size_t>(e) * q.ld * PS; };
     unsigned s = 0, phase = 0;
     bool expired = false;
-    const unsigned col0 = t * VEC, col_step = T * VEC;
+    const unsigned col0 = t * 8, col_step = T * 8;
 #pragma unroll 1
     for(unsigned i = 0; i < rows; ++i)
     {
-        if(row0 + i >= change) // (the same for every thread)
-            entries(row0 + i);
+        const unsigned row = row0 + i;
+        if(row >= change) // (the same for every thread)
+            entries(row);
         // (bounded, though a copy of valid memory always completes: on expiry the status record says that the output is incomplete)
         if(!expired && !mbar_try_wait(smem_u32(&full[s]), phase))
         {
@@ -296,20 +219,14 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
         }
         const uint8_t* xs = smem + s * stage_bytes;
         const uint8_t* rs = xs + lay.x_bytes;
-        if(VEC != 8)
-        {
-            xs += reinterpret_cast<uintptr_t>(xg) & 15;
-            rs += reinterpret_cast<uintptr_t>(rg) & 15;
-        }
         float2 h[CNT][P];
         {
-            const bool even = pairs_aligned<XD>(xs);
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
             {
                 const unsigned col = col0 + j * col_step;
-                if(col < n)
-                    rd_vec<XD, VEC>(xs + col * XS, even, col + 1 < n, h[j]);
+                if(FULL || col < n)
+                    rd_vec<XD>(xs + col * XS, h[j]);
                 else
 #pragma unroll
                     for(int k = 0; k < P; ++k)
@@ -326,7 +243,7 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
                 for(int j = 0; j < CNT; ++j)
 #pragma unroll
                     for(int k = 0; k < P; ++k)
-                        a = __fadd2_rn(a, h[j][k]);
+                        a = add2(a, h[j][k]);
                 mean = row_sum(a.x + a.y, red, slot) * prm.inv_n;
                 a    = make_float2(0.f, 0.f);
                 const float2 m = make_float2(-mean, -mean);
@@ -334,14 +251,12 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
                 for(int j = 0; j < CNT; ++j)
                 {
                     const unsigned col = col0 + j * col_step;
-                    if(col < n)
+                    if(FULL || col < n)
 #pragma unroll
                         for(int k = 0; k < P; ++k)
                         {
-                            float2 d = __fadd2_rn(h[j][k], m);
-                            if(VEC == 2 && col + 1 >= n)
-                                d.y = 0.f;
-                            a = __ffma2_rn(d, d, a);
+                            const float2 d = add2(h[j][k], m);
+                            a = fma2(d, d, a);
                         }
                 }
             }
@@ -351,12 +266,12 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
                 for(int j = 0; j < CNT; ++j)
 #pragma unroll
                     for(int k = 0; k < P; ++k)
-                        a = __ffma2_rn(h[j][k], h[j][k], a);
+                        a = fma2(h[j][k], h[j][k], a);
             }
             rstd = rsqrtf(row_sum(a.x + a.y, red, slot + 1) * prm.inv_n + prm.eps);
         };
         float mean = 0.f, rstd = 1.f;
-        if(post)
+        if(prm.post)
         {
             stats(0, mean, rstd);
             const float2 a = make_float2(rstd, rstd);
@@ -367,20 +282,20 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
                 for(int j = 0; j < CNT; ++j)
 #pragma unroll
                     for(int k = 0; k < P; ++k)
-                        h[j][k] = __fadd2_rn(h[j][k], m);
+                        h[j][k] = add2(h[j][k], m);
             }
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
 #pragma unroll
                 for(int k = 0; k < P; ++k)
-                    h[j][k] = __fmul2_rn(h[j][k], a);
-            if(has_pw)
-                scale_by<QD, VEC, CNT>(h, pw, col0, col_step, n, 0.f);
-            if(has_pb)
-                shift_by<QD, VEC, CNT>(h, pb, col0, col_step, n);
+                    h[j][k] = mul2(h[j][k], a);
+            if(prm.post_weight.ptr != nullptr)
+                scale_by<PD, CNT, FULL>(h, entry(prm.post_weight, epw), col0, col_step, n, 0.f);
+            if(prm.post_bias.ptr != nullptr)
+                shift_by<PD, CNT, FULL>(h, entry(prm.post_bias, epb), col0, col_step, n);
         }
-        if(gate_vec)
-            scale_by<QD, VEC, CNT>(h, pg, col0, col_step, n, 0.f);
+        if(prm.gate.ptr != nullptr && !prm.gate_scalar)
+            scale_by<PD, CNT, FULL>(h, entry(prm.gate, eg), col0, col_step, n, 0.f);
         else if(gate_one)
         {
             const float2 a = make_float2(gate1, gate1);
@@ -388,28 +303,27 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
             for(int j = 0; j < CNT; ++j)
 #pragma unroll
                 for(int k = 0; k < P; ++k)
-                    h[j][k] = __fmul2_rn(h[j][k], a);
+                    h[j][k] = mul2(h[j][k], a);
         }
         if(has_res)
         {
-            const float2 a  = make_float2(prm.res_scale, prm.res_scale);
-            const bool even = pairs_aligned<RD>(rs);
+            const float2 a = make_float2(prm.res_scale, prm.res_scale);
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
             {
                 const unsigned col = col0 + j * col_step;
-                if(col < n)
+                if(FULL || col < n)
                 {
                     float2 q[P];
-                    rd_vec<RD, VEC>(rs + col * RS, even, col + 1 < n, q);
+                    rd_vec<RD>(rs + col * RS, q);
 #pragma unroll
                     for(int k = 0; k < P; ++k)
-                        h[j][k] = __ffma2_rn(a, q[k], h[j][k]);
+                        h[j][k] = fma2(a, q[k], h[j][k]);
                 }
             }
         }
         // elements behind the row count for nothing in the sums (a first layer norm or its bias has touched them)
-        if(post)
+        if(!FULL && prm.post)
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
             {
@@ -418,24 +332,22 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
 #pragma unroll
                     for(int k = 0; k < P; ++k)
                         h[j][k] = make_float2(0.f, 0.f);
-                else if(VEC == 2 && col + 1 >= n)
-                    h[j][0].y = 0.f;
             }
-        if(has_h)
+        if(prm.h.ptr != nullptr)
         {
-            const bool even = pairs_aligned<RD>(hg);
+            uint8_t* const hg = static_cast<uint8_t*>(prm.h.ptr) + static_cast<size_t>(row) * prm.h.ld * RS;
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
             {
                 const unsigned col = col0 + j * col_step;
-                if(col < n)
-                    wr_vec<RD, VEC>(hg + col * RS, even, col + 1 < n, h[j]);
+                if(FULL || col < n)
+                    wr_vec<RD>(hg + col * RS, h[j]);
             }
         }
         stats(2, mean, rstd);
         // every thread has read its part of the stage (the sum's barrier): a later row may land there
         if(t == 0 && i + S < rows && !expired)
-            load(xg + S * x_step, rg + S * r_step, s);
+            load(row + S, s);
         if(++s == S)
         {
             s = 0;
@@ -450,28 +362,28 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
                 for(int j = 0; j < CNT; ++j)
 #pragma unroll
                     for(int k = 0; k < P; ++k)
-                        h[j][k] = __fadd2_rn(h[j][k], m);
+                        h[j][k] = add2(h[j][k], m);
             }
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
 #pragma unroll
                 for(int k = 0; k < P; ++k)
-                    h[j][k] = __fmul2_rn(h[j][k], a);
+                    h[j][k] = mul2(h[j][k], a);
         }
-        if(has_w)
-            scale_by<QD, VEC, CNT>(h, w, col0, col_step, n, prm.weight_offset);
-        if(has_b)
-            shift_by<QD, VEC, CNT>(h, b, col0, col_step, n);
+        if(prm.weight.ptr != nullptr)
+            scale_by<PD, CNT, FULL>(h, entry(prm.weight, ew), col0, col_step, n, prm.weight_offset);
+        if(prm.bias.ptr != nullptr)
+            shift_by<PD, CNT, FULL>(h, entry(prm.bias, eb), col0, col_step, n);
         // one test of y's type a row
+        uint8_t* const yg = static_cast<uint8_t*>(prm.y.ptr) + static_cast<size_t>(row) * prm.y.ld * bytes_of_mode(prm.y.dt);
         auto store_all = [&](auto tag) {
             constexpr int YD = decltype(tag)::value;
-            const bool even  = pairs_aligned<YD>(yg);
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
             {
                 const unsigned col = col0 + j * col_step;
-                if(col < n)
-                    wr_vec<YD, VEC>(yg + col * esize_of(YD), even, col + 1 < n, h[j]);
+                if(FULL || col < n)
+                    wr_vec<YD>(yg + col * esize_of(YD), h[j]);
             }
         };
         if(prm.y.dt == OUT_BF16)
@@ -480,24 +392,289 @@ __global__ void __launch_bounds__(512, VEC * CNT <= 16 ? 2 : 1) norm_stream_kern
             store_all(std::integral_constant<int, OUT_F16>{});
         else if(prm.y.dt == OUT_F32)
             store_all(std::integral_constant<int, OUT_F32>{});
-        else if constexpr(VEC == 8)
+        else
         {
-            const unsigned row = row0 + i;
             if(prm.y.dt == OUT_E2M1)
-                emit_mx<true, CNT>(prm.sf, yg, row, col0, col_step, n, h);
+                emit_mx<true, CNT, FULL>(prm.sf, yg, row, col0, col_step, n, h);
             else
-                emit_mx<false, CNT>(prm.sf, yg, row, col0, col_step, n, h);
+                emit_mx<false, CNT, FULL>(prm.sf, yg, row, col0, col_step, n, h);
             if(prm.sf.layout != QSL_PLAIN && (row == prm.M - 1 || (n & 255) != 0))
                 fill_scale_padding(prm.sf, row, prm.M, n >> 5, t, T);
         }
-        xg += x_step;
-        rg += r_step;
-        hg += h_step;
-        yg += y_step;
     }
     if(expired)
     {
         // copies still in flight land before this CTA's shared memory is released (bounded)
+        const uint64_t t0 = global_timer_ns();
+        while(global_timer_ns() - t0 < 200000ull) {}
+    }
+}
+
+// Rows of any width of dense tensors: row r starts at element r * ld, and with equal pitches (modulo 8) and aligned bases the
+// groups of eight elements that are aligned in one tensor are aligned in all.  A thread takes such groups - the first and the last
+// of a row only in part -, so every access of x, residual, h and y stays a 16-byte one.  A row's phase in its groups repeats every
+// eight rows: a CTA takes every eighth row of its block, and keeps the parameters in shared memory at that phase.  (One element a
+// lane at a time: 8192 x 4097 106 to 150 us, at about 100 instructions an element; parameters shifted into place by selects on
+// every row, 8200 x 1155 with three of them, 55 us.)
+template <int XD, int RD, int PD, int CNT>
+__global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_constant__ NormParams prm, const __grid_constant__ NormStreamLayout lay)
+{
+    constexpr int XS = esize_of(XD), RS = esize_of(RD), PS = esize_of(PD);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float red[8][32];
+    __shared__ __align__(8) uint64_t full[4];
+    const unsigned t = threadIdx.x, T = blockDim.x, n = prm.n;
+    const bool has_res  = prm.res.ptr != nullptr;
+    const bool gate_one = prm.gate.ptr != nullptr && prm.gate_scalar;
+    // this CTA's rows: row_of(0), row_of(1), ... of one residue class modulo 8 (the grid is a multiple of 8)
+    const unsigned cls = blockIdx.x & 7, of_class = prm.M > cls ? (prm.M - cls + 7) / 8 : 0;
+    const unsigned team = gridDim.x / 8, mate = blockIdx.x / 8;
+    const unsigned per = of_class / team, extra = of_class % team;
+    const unsigned row0 = cls + 8 * (mate * per + min(mate, extra));
+    const unsigned rows = per + (mate < extra ? 1u : 0u);
+    auto row_of         = [&](unsigned i) { return row0 + 8 * i; };
+    const unsigned S = lay.stages, stage_bytes = lay.x_bytes + lay.r_bytes;
+    if(t == 0)
+    {
+        for(unsigned s = 0; s < S; ++s)
+            mbar_init(smem_u32(&full[s]), 1);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    grid_launch_dependents();
+    // first element of this CTA's rows within their groups of eight (the same in every tensor): the row is elements [e8, end)
+    const unsigned e8 = static_cast<unsigned>((reinterpret_cast<uintptr_t>(prm.x.ptr) / XS + static_cast<size_t>(row0) * prm.x.ld) & 7), end = e8 + n;
+    auto load     = [&](unsigned row, unsigned s) { // whole groups of a row into stage s, by one thread
+        const uint32_t bar = smem_u32(&full[s]), dst = smem_u32(smem) + s * stage_bytes;
+        // the 16-byte pieces that hold something of the row, at their places in its groups
+        const unsigned x0 = (e8 * XS) & ~15u, xb = (((e8 + n) * XS + 15) & ~15u) - x0;
+        const unsigned r0 = (e8 * RS) & ~15u, rb = (((e8 + n) * RS + 15) & ~15u) - r0;
+        mbar_arrive_expect_tx(bar, xb + (has_res ? rb : 0u));
+        bulk_load(dst + x0, static_cast<const uint8_t*>(prm.x.ptr) + (static_cast<size_t>(row) * prm.x.ld - e8) * XS + x0, xb, bar);
+        if(has_res)
+            bulk_load(dst + lay.x_bytes + r0, static_cast<const uint8_t*>(prm.res.ptr) + (static_cast<size_t>(row) * prm.res.ld - e8) * RS + r0, rb, bar);
+    };
+    if(t == 0)
+        for(unsigned i = 0; i < min(S, rows); ++i)
+            load(row_of(i), i);
+    // the parameters of the current entries, element e of each at place e8 + e, until row `change`
+    uint8_t* const params = smem + lay.param_off;
+    float gate1           = 1.f;
+    unsigned change       = 0;
+    auto entries          = [&](unsigned row) {
+        change    = 0xFFFFFFFFu;
+        int k     = 0;
+        auto take = [&](const RowParam& q) {
+            if(q.ptr == nullptr)
+                return;
+            if(q.ld != 0)
+                change = min(change, (row / q.rows_per + 1) * q.rows_per);
+            using E      = std::conditional_t<PD == OUT_F32, uint32_t, uint16_t>;
+            const E* src = static_cast<const E*>(q.ptr) + param_at(q, row);
+            E* dst       = reinterpret_cast<E*>(params + (k++) * lay.param_pitch) + e8;
+            for(unsigned e = t; e < n; e += T)
+                dst[e] = src[e];
+        };
+        __syncthreads(); // nobody reads the previous entries any more
+        take(prm.weight);
+        take(prm.bias);
+        take(prm.post_weight);
+        take(prm.post_bias);
+        if(!gate_one)
+            take(prm.gate);
+        else
+        {
+            if(prm.gate.ld != 0)
+                change = min(change, (row / prm.gate.rows_per + 1) * prm.gate.rows_per);
+            gate1 = load_elem_any(prm.gate.ptr, prm.gate.dt, param_at(prm.gate, row));
+        }
+        __syncthreads();
+    };
+    // where each parameter lies (the order of `take`)
+    int slots      = 0;
+    auto slot      = [&](const RowParam& q) { return q.ptr != nullptr ? slots++ : -1; };
+    const int at_w = slot(prm.weight), at_b = slot(prm.bias), at_pw = slot(prm.post_weight), at_pb = slot(prm.post_bias);
+    const int at_g = gate_one ? -1 : slot(prm.gate);
+    const unsigned col0 = t * 8, col_step = T * 8;
+    auto place = [&](int at) { return params + at * lay.param_pitch; };
+    unsigned s = 0, phase = 0;
+    bool expired = false;
+#pragma unroll 1
+    for(unsigned i = 0; i < rows; ++i)
+    {
+        const unsigned row = row_of(i);
+        if(row >= change) // (the same for every thread)
+            entries(row);
+        if(!expired && !mbar_try_wait(smem_u32(&full[s]), phase))
+        {
+            const uint64_t t0 = global_timer_ns();
+            while(!expired && !mbar_try_wait_parked(smem_u32(&full[s]), phase, kParkNs))
+                expired = global_timer_ns() - t0 > kWaitLimitNs;
+            if(expired)
+                report_timeout(lay.report, ST_TIMEOUT_ROWS, i);
+        }
+        const uint8_t* xs = smem + s * stage_bytes;
+        const uint8_t* rs = xs + lay.x_bytes;
+        auto group   = [&](int j) { return j * T + t; };
+        auto whole   = [&](unsigned v) { return (v != 0 || e8 == 0) && 8 * v + 8 <= end; };
+        auto exists  = [&](unsigned v) { return 8 * v < end; };
+        auto for_row = [&](unsigned v, auto&& f) { // the elements of a group that is only partly the row's
+#pragma unroll
+            for(int k = 0; k < 8; ++k)
+                if(8 * v + k >= e8 && 8 * v + k < end)
+                    f(k);
+        };
+        float2 h[CNT][4];
+        auto clear_outside = [&](unsigned v, float2 (&g)[4]) {
+#pragma unroll
+            for(int k = 0; k < 4; ++k)
+                g[k] = make_float2((8 * v + 2 * k >= e8 && 8 * v + 2 * k < end) ? g[k].x : 0.f, (8 * v + 2 * k + 1 >= e8 && 8 * v + 2 * k + 1 < end) ? g[k].y : 0.f);
+        };
+#pragma unroll
+        for(int j = 0; j < CNT; ++j)
+        {
+            const unsigned v = group(j);
+            if(exists(v))
+            {
+                rd_vec<XD>(xs + v * (8 * XS), h[j]);
+                if(!whole(v))
+                    clear_outside(v, h[j]);
+            }
+            else
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    h[j][k] = make_float2(0.f, 0.f);
+        }
+        auto stats = [&](int slot_, float& mean, float& rstd) {
+            slot_ += 4 * static_cast<int>(i & 1);
+            float2 a = make_float2(0.f, 0.f);
+            mean     = 0.f;
+            if(prm.layer)
+            {
+#pragma unroll
+                for(int j = 0; j < CNT; ++j)
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
+                        a = add2(a, h[j][k]);
+                mean = row_sum(a.x + a.y, red, slot_) * prm.inv_n;
+                a    = make_float2(0.f, 0.f);
+                const float2 m = make_float2(-mean, -mean);
+#pragma unroll
+                for(int j = 0; j < CNT; ++j)
+                {
+                    const unsigned v = group(j);
+                    float2 d[4];
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
+                        d[k] = add2(h[j][k], m);
+                    if(!whole(v))
+                        clear_outside(v, d);
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
+                        a = fma2(d[k], d[k], a);
+                }
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < CNT; ++j)
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
+                        a = fma2(h[j][k], h[j][k], a);
+            }
+            rstd = rsqrtf(row_sum(a.x + a.y, red, slot_ + 1) * prm.inv_n + prm.eps);
+        };
+        auto scale1 = [&](float f) {
+#pragma unroll
+            for(int j = 0; j < CNT; ++j)
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    h[j][k] = mul2(h[j][k], make_float2(f, f));
+        };
+        auto shift1 = [&](float f) {
+#pragma unroll
+            for(int j = 0; j < CNT; ++j)
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    h[j][k] = add2(h[j][k], make_float2(f, f));
+        };
+        float mean = 0.f, rstd = 1.f;
+        if(prm.post)
+        {
+            stats(0, mean, rstd);
+            if(prm.layer)
+                shift1(-mean);
+            scale1(rstd);
+            if(at_pw >= 0)
+                scale_by<PD, CNT>(h, place(at_pw), col0, col_step, end, 0.f);
+            if(at_pb >= 0)
+                shift_by<PD, CNT>(h, place(at_pb), col0, col_step, end);
+        }
+        if(at_g >= 0)
+            scale_by<PD, CNT>(h, place(at_g), col0, col_step, end, 0.f);
+        else if(gate_one)
+            scale1(gate1);
+        if(has_res)
+#pragma unroll
+            for(int j = 0; j < CNT; ++j)
+            {
+                const unsigned v = group(j);
+                if(exists(v))
+                {
+                    float2 q[4];
+                    rd_vec<RD>(rs + v * (8 * RS), q);
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
+                        h[j][k] = fma2(make_float2(prm.res_scale, prm.res_scale), q[k], h[j][k]);
+                }
+            }
+        // values outside the row count for nothing in the sums
+#pragma unroll
+        for(int j = 0; j < CNT; ++j)
+            if(!whole(group(j)))
+                clear_outside(group(j), h[j]);
+        auto store = [&](const RowTensor& y, auto tag) {
+            constexpr int DT = decltype(tag)::value;
+            uint8_t* const p = static_cast<uint8_t*>(y.ptr) + (static_cast<size_t>(row) * y.ld - e8) * esize_of(DT);
+#pragma unroll
+            for(int j = 0; j < CNT; ++j)
+            {
+                const unsigned v = group(j);
+                if(whole(v))
+                    wr_vec<DT>(p + v * (8 * esize_of(DT)), h[j]);
+                else if(exists(v))
+                    for_row(v, [&](int k) { store_out(p, 8 * v + k, (k & 1) ? h[j][k / 2].y : h[j][k / 2].x, DT); });
+            }
+        };
+        if(prm.h.ptr != nullptr)
+            store(prm.h, std::integral_constant<int, RD>{});
+        stats(2, mean, rstd);
+        // every thread has read its part of the stage (the sum's barrier): a later row may land there
+        if(t == 0 && i + S < rows && !expired)
+            load(row_of(i + S), s);
+        if(++s == S)
+        {
+            s = 0;
+            phase ^= 1u;
+        }
+        if(prm.layer)
+            shift1(-mean);
+        scale1(rstd);
+        if(at_w >= 0)
+            scale_by<PD, CNT>(h, place(at_w), col0, col_step, end, prm.weight_offset);
+        if(at_b >= 0)
+            shift_by<PD, CNT>(h, place(at_b), col0, col_step, end);
+        if(prm.y.dt == OUT_BF16)
+            store(prm.y, std::integral_constant<int, OUT_BF16>{});
+        else if(prm.y.dt == OUT_F16)
+            store(prm.y, std::integral_constant<int, OUT_F16>{});
+        else
+            store(prm.y, std::integral_constant<int, OUT_F32>{});
+    }
+    if(expired)
+    {
         const uint64_t t0 = global_timer_ns();
         while(global_timer_ns() - t0 < 200000ull) {}
     }
@@ -568,15 +745,15 @@ __global__ void __launch_bounds__(256) norm_short_kernel(const __grid_constant__
 #pragma unroll
                 for(int k = 0; k < 4; ++k)
                 {
-                    const float2 d = __fadd2_rn(h[0][k], m);
-                    a              = __ffma2_rn(d, d, a);
+                    const float2 d = add2(h[0][k], m);
+                    a              = fma2(d, d, a);
                 }
             rstd = rsqrtf(sum(a.x + a.y) * prm.inv_n + prm.eps);
         };
         auto normalise = [&](float mean, float rstd) {
 #pragma unroll
             for(int k = 0; k < 4; ++k)
-                h[0][k] = __fmul2_rn(__fadd2_rn(h[0][k], make_float2(-mean, -mean)), make_float2(rstd, rstd));
+                h[0][k] = mul2(add2(h[0][k], make_float2(-mean, -mean)), make_float2(rstd, rstd));
         };
         auto entry = [&](const RowParam& q) { return static_cast<const uint8_t*>(q.ptr) + param_at(q, row) * PS; };
         float mean, rstd;
@@ -585,9 +762,9 @@ __global__ void __launch_bounds__(256) norm_short_kernel(const __grid_constant__
             stats(mean, rstd);
             normalise(mean, rstd);
             if(prm.post_weight.ptr != nullptr)
-                scale_by<PD, 8, 1>(h, entry(prm.post_weight), col, 0, n, 0.f);
+                scale_by<PD, 1>(h, entry(prm.post_weight), col, 0, n, 0.f);
             if(prm.post_bias.ptr != nullptr)
-                shift_by<PD, 8, 1>(h, entry(prm.post_bias), col, 0, n);
+                shift_by<PD, 1>(h, entry(prm.post_bias), col, 0, n);
         }
         if(prm.gate.ptr != nullptr)
         {
@@ -596,30 +773,30 @@ __global__ void __launch_bounds__(256) norm_short_kernel(const __grid_constant__
                 const float g = load_elem_any(prm.gate.ptr, prm.gate.dt, param_at(prm.gate, row));
 #pragma unroll
                 for(int k = 0; k < 4; ++k)
-                    h[0][k] = __fmul2_rn(h[0][k], make_float2(g, g));
+                    h[0][k] = mul2(h[0][k], make_float2(g, g));
             }
             else
-                scale_by<PD, 8, 1>(h, entry(prm.gate), col, 0, n, 0.f);
+                scale_by<PD, 1>(h, entry(prm.gate), col, 0, n, 0.f);
         }
         if(has_res && in)
         {
             unpack<8, RD == OUT_F32>(cr, RD, v);
 #pragma unroll
             for(int k = 0; k < 4; ++k)
-                h[0][k] = __ffma2_rn(make_float2(prm.res_scale, prm.res_scale), make_float2(v[2 * k], v[2 * k + 1]), h[0][k]);
+                h[0][k] = fma2(make_float2(prm.res_scale, prm.res_scale), make_float2(v[2 * k], v[2 * k + 1]), h[0][k]);
         }
         if(!in)
 #pragma unroll
             for(int k = 0; k < 4; ++k)
                 h[0][k] = make_float2(0.f, 0.f);
         if(prm.h.ptr != nullptr && in)
-            wr_vec<RD, 8>(static_cast<uint8_t*>(prm.h.ptr) + (static_cast<size_t>(row) * prm.h.ld + col) * RS, true, true, h[0]);
+            wr_vec<RD>(static_cast<uint8_t*>(prm.h.ptr) + (static_cast<size_t>(row) * prm.h.ld + col) * RS, h[0]);
         stats(mean, rstd);
         normalise(mean, rstd);
         if(prm.weight.ptr != nullptr)
-            scale_by<PD, 8, 1>(h, entry(prm.weight), col, 0, n, prm.weight_offset);
+            scale_by<PD, 1>(h, entry(prm.weight), col, 0, n, prm.weight_offset);
         if(prm.bias.ptr != nullptr)
-            shift_by<PD, 8, 1>(h, entry(prm.bias), col, 0, n);
+            shift_by<PD, 1>(h, entry(prm.bias), col, 0, n);
         uint8_t* y = static_cast<uint8_t*>(prm.y.ptr) + static_cast<size_t>(row) * prm.y.ld * bytes_of_mode(prm.y.dt);
         if(prm.y.dt >= OUT_E2M1)
         {
@@ -635,11 +812,11 @@ __global__ void __launch_bounds__(256) norm_short_kernel(const __grid_constant__
         else if(in)
         {
             if(prm.y.dt == OUT_BF16)
-                wr_vec<OUT_BF16, 8>(y + col * 2, true, true, h[0]);
+                wr_vec<OUT_BF16>(y + col * 2, h[0]);
             else if(prm.y.dt == OUT_F16)
-                wr_vec<OUT_F16, 8>(y + col * 2, true, true, h[0]);
+                wr_vec<OUT_F16>(y + col * 2, h[0]);
             else
-                wr_vec<OUT_F32, 8>(y + col * 4, true, true, h[0]);
+                wr_vec<OUT_F32>(y + col * 4, h[0]);
         }
     }
 }

@@ -339,3 +339,26 @@ def test_other_stream_and_captured_graphs(ab):
     want = (*ab.gated_residual_norm(x, r, w), ab.act_and_mul(x))
     for o in outs:
         assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("fp4", [False, True])
+def test_mx_scale_of_every_magnitude(ab, fp4):
+    """Blocks whose largest value runs through every exponent and the significands around the step of the scale, denormals, zero,
+    infinity and NaN among them: bytes and elements as the oracle's division gives them."""
+    tops = []
+    for e in range(-149, 128):
+        for mant in (1.0, 1.5 - 2.0**-23, 1.5, 1.5 + 2.0**-23, 1.75 - 2.0**-23, 1.75, 1.75 + 2.0**-23, 2.0 - 2.0**-23):
+            tops.append(math.ldexp(mant, e))
+    tops += [0.0, float("inf"), float("nan")]
+    top = np.array(tops, dtype=np.float64)
+    top = top[~(np.abs(top) > 3.4028234663852886e38) | np.isinf(top)].astype(np.float32)
+    rows = len(top)
+    # (the factor half is ones: the product is relu of the gate half, x < 0 ? 0 : x, which keeps the sign of a zero)
+    x = np.concatenate([np.tile(top[:, None] * np.float32(1), (1, 32)) * np.linspace(1.0, -0.9, 32, dtype=np.float32)[None, :], np.ones((rows, 32), np.float32)], axis=1)
+    x[:, 0] = top
+    with np.errstate(all="ignore"):
+        want_q, want_s = (ox.quant_mxfp4 if fp4 else ox.quant_mxfp8)(np.where(x[:, :32] < 0, np.float32(0), x[:, :32]))
+    y, s = ab.act_and_mul(torch.from_numpy(x).cuda(), "relu", quant_dtype=ab.dtypes.fp4x2 if fp4 else ab.dtypes.fp8)
+    assert np.array_equal(s.view(torch.uint8).cpu().numpy(), want_s)
+    finite = np.isfinite(top)
+    assert np.array_equal(y.view(torch.uint8).cpu().numpy()[finite], want_q[finite])

@@ -300,9 +300,13 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
         if(n > 8000 || !same_phase(prm))
             return false;
         elems      = (n + 14) / 8 * 8; // (a row touches at most that many elements in whole groups)
-        cnt        = n > 512 ? 2 : 1;
-        sh.threads = (elems / 8 + cnt - 1) / cnt;
-        sh.threads = (sh.threads + 31) / 32 * 32;
+        // two groups a thread, one where whole warps of them would leave more than 15 % of the lanes idle by comparison
+        // (8200 x 1155: 192 lanes for 146 groups 41 us, 160 lanes 35; 16384 x 1001, where both fit, 34 and 38)
+        auto warps = [&](unsigned c) { return ((elems / 8 + c - 1) / c + 31) / 32; };
+        cnt        = n > 512 && 100 * warps(1) > 85 * 2 * warps(2) ? 2 : 1;
+        if(warps(cnt) > 16)
+            cnt = 2;
+        sh.threads = warps(cnt) * 32;
         sh.flat    = true;
         sh.budget  = 192u * 1024u;
         sh.lay.param_pitch = elems * param_bytes;

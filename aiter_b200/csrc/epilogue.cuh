@@ -28,6 +28,7 @@ struct alignas(64) EpilogueParams<1>
     int res_mode;
     int res_vec;
     int res_tma;      // residual tiles come through map_res
+    uint32_t res_step, out_step; // res_ld and the output's pitch as 32-bit numbers (15 rows of either stay below 2^32 elements)
     int act;
     int out_mode;
     int stream;           // residual and output are larger than L2: their lines leave it first
@@ -226,31 +227,106 @@ __device__ __forceinline__ bool fused_tile(FusedWarp& f, const EpilogueParams<1>
 
 // Outputs or residuals whose rows allow no tile copies, and tiles with the weights on the 128-row slot (few rows, a K split over a
 // cluster, or rows that start on odd addresses: there the lanes run along the output's columns and plain accesses coalesce).
-// Sixteen columns of the accumulator at a time, alternating between the two warps of a quarter.  red / red_stride: the other K
-// slices' partial sums of this thread's row.
+// Sixteen columns of the accumulator at a time, alternating between the two warps of a quarter, with the residual of the next
+// sixteen under way (the first before the accumulator is waited for).
+struct FusedPlain
+{
+    uint32_t raw[16]; // residual of the group that comes next
+};
+
+// Sixteen elements `step` apart, of which `valid` exist.  One test of the type and of the tile's edge for all of them: what this
+// epilogue costs is instructions (a test per element: 47 of them a value instead of about 20, and 4096 x 4097 x 1024 with
+// gelu_tanh and a residual 79 us).
+template <typename T>
+__device__ __forceinline__ void load16(uint32_t (&raw)[16], const T* src, uint32_t step, int valid)
+{
+    if(valid >= 16)
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            raw[j] = src[static_cast<size_t>(j * step)];
+    }
+    else
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            raw[j] = j < valid ? static_cast<uint32_t>(src[static_cast<size_t>(j) * step]) : 0u;
+    }
+}
+template <typename T, typename Convert>
+__device__ __forceinline__ void store16(T* dst, const float (&v)[16], uint32_t step, int valid, Convert&& convert)
+{
+    if(valid >= 16)
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            dst[static_cast<size_t>(j * step)] = convert(v[j]);
+    }
+    else
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            if(j < valid)
+                dst[static_cast<size_t>(j) * step] = convert(v[j]);
+    }
+}
+
+template <typename Params>
+__device__ __forceinline__ void fused_plain_load(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, int p, int q_first)
+{
+    if(epi.res == nullptr)
+        return;
+    const bool transposed = prm.transposed_out != 0;
+    const int valid       = p < prm.rows_p ? prm.rows_q - q_first : 0;
+    const uint32_t step   = transposed ? epi.res_step : 1u;
+    const size_t at       = transposed ? static_cast<size_t>(q_first) * epi.res_ld + p : static_cast<size_t>(p) * epi.res_ld + q_first;
+    if(epi.res_mode == OUT_F32)
+        load16(f.raw, static_cast<const uint32_t*>(epi.res) + at, step, valid);
+    else
+        load16(f.raw, static_cast<const uint16_t*>(epi.res) + at, step, valid);
+}
+
+// Before the accumulator is waited for: the first group's residual into registers, the rest of this warp's part of the tile into
+// L2.  The registers of eight warps hold 8 KB of loads, which at the latency of HBM is 1 TB/s, at that of L2 three times as much.
+template <typename Params>
+__device__ __forceinline__ void fused_plain_begin(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, int p_warp0, int col0, int bn, int group, int lane)
+{
+    if(epi.res == nullptr)
+        return;
+    fused_plain_load(f, epi, prm, p_warp0 + lane, col0 + 16 * group);
+    if(prm.transposed_out && p_warp0 < prm.rows_p)
+    {
+        // lane l: row l % 16 of every other group of 16, starting with the second; both ends of its 32 columns
+        const int esize = epi.res_mode == OUT_F32 ? 4 : 2;
+        const int last  = min(p_warp0 + 31, prm.rows_p - 1);
+        for(int c = group + 2 + 2 * (lane >> 4); c < bn / 16; c += 4)
+        {
+            const int q = col0 + c * 16 + (lane & 15);
+            if(q < prm.rows_q)
+            {
+                const uint8_t* row = static_cast<const uint8_t*>(epi.res) + static_cast<size_t>(q) * epi.res_ld * esize;
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(row + static_cast<size_t>(p_warp0) * esize));
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(row + static_cast<size_t>(last) * esize));
+            }
+        }
+    }
+}
+
+// red / red_stride: the other K slices' partial sums of this thread's row.
 template <typename Params, typename Release>
-__device__ __forceinline__ bool fused_plain_tile(const EpilogueParams<1>& epi, const Params& prm, uint32_t tacc, int p, int col0, int bn, int group, int csplit,
+__device__ __forceinline__ bool fused_plain_tile(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, uint32_t tacc, int p, int col0, int bn, int group, int csplit,
                                                  const float* red, size_t red_stride, uint32_t red_bar, volatile uint32_t* abort_f, int uc, Release&& release_acc)
 {
-    const int groups = bn / 16;
+    const int groups  = bn / 16;
     const bool row_in = p < prm.rows_p, transposed = prm.transposed_out != 0;
-    const size_t res_step = transposed ? static_cast<size_t>(epi.res_ld) : 1u;
-    const float bias_p    = (epi.bias != nullptr && transposed && row_in) ? load_elem(epi.bias, epi.bias_mode, p) : 0.f;
+    const float bias_p = (epi.bias != nullptr && transposed && row_in) ? load_elem(epi.bias, epi.bias_mode, p) : 0.f;
     if(group >= groups)
         release_acc();
 #pragma unroll 1
     for(int c = group; c < groups; c += 2)
     {
         const int q_first = col0 + c * 16;
-        const int valid   = row_in ? min(16, prm.rows_q - q_first) : 0;
-        uint32_t raw[16];
-        if(epi.res != nullptr)
-        {
-            const size_t at = transposed ? static_cast<size_t>(q_first) * epi.res_ld + p : static_cast<size_t>(p) * epi.res_ld + q_first;
-#pragma unroll
-            for(int j = 0; j < 16; ++j)
-                raw[j] = j < valid ? load_elem_raw(epi.res, epi.res_mode, at + j * res_step) : 0u;
-        }
+        const int valid   = row_in ? prm.rows_q - q_first : 0;
         float v[16];
         {
             uint32_t r[16];
@@ -287,23 +363,51 @@ __device__ __forceinline__ bool fused_plain_tile(const EpilogueParams<1>& epi, c
         }
         if(epi.bias != nullptr)
         {
+            if(transposed)
+            {
 #pragma unroll
-            for(int j = 0; j < 16; ++j)
-                v[j] += transposed ? bias_p : (j < valid ? load_elem(epi.bias, epi.bias_mode, q_first + j) : 0.f);
+                for(int j = 0; j < 16; ++j)
+                    v[j] += bias_p;
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                    v[j] += j < valid ? load_elem(epi.bias, epi.bias_mode, q_first + j) : 0.f;
+            }
         }
         activate(v, epi.act);
         if(epi.res != nullptr)
         {
+            if(epi.res_mode == OUT_BF16)
+            {
 #pragma unroll
-            for(int j = 0; j < 16; ++j)
-                v[j] += raw_to_f32(raw[j], epi.res_mode);
+                for(int j = 0; j < 16; ++j)
+                    v[j] += __uint_as_float(f.raw[j] << 16);
+            }
+            else if(epi.res_mode == OUT_F16)
+            {
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                    v[j] += raw_to_f32(f.raw[j], OUT_F16);
+            }
+            else
+            {
+#pragma unroll
+                for(int j = 0; j < 16; ++j)
+                    v[j] += __uint_as_float(f.raw[j]);
+            }
+            if(c + 2 < groups)
+                fused_plain_load(f, epi, prm, p, q_first + 32);
         }
-        const size_t at       = transposed ? static_cast<size_t>(q_first) * prm.ldo + p : static_cast<size_t>(p) * prm.ldo + q_first;
-        const size_t out_step = transposed ? static_cast<size_t>(prm.ldo) : 1u;
-#pragma unroll
-        for(int j = 0; j < 16; ++j)
-            if(j < valid)
-                store_out(prm.out, at + j * out_step, v[j], epi.out_mode);
+        const size_t at         = transposed ? static_cast<size_t>(q_first) * prm.ldo + p : static_cast<size_t>(p) * prm.ldo + q_first;
+        const uint32_t out_step = transposed ? epi.out_step : 1u;
+        if(epi.out_mode == OUT_F32)
+            store16(static_cast<float*>(prm.out) + at, v, out_step, valid, [](float x) { return x; });
+        else if(epi.out_mode == OUT_BF16)
+            store16(static_cast<uint16_t*>(prm.out) + at, v, out_step, valid, [](float x) { return cvt_out16(x, false); });
+        else
+            store16(static_cast<uint16_t*>(prm.out) + at, v, out_step, valid, [](float x) { return cvt_out16(x, true); });
     }
     return true;
 }

@@ -856,6 +856,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
         int ebuf             = 0;
         uint32_t wbuf        = 0; // wide stores: which of the two 4 KB buffers comes next (0 when there is only one)
         FusedWarp fused{};
+        FusedPlain plain{};
         if constexpr(EPI != 0)
         {
             fused.slots     = smem_base + L.epi_off + static_cast<uint32_t>(epi_warp) * 2u * epi.slot_bytes;
@@ -959,8 +960,12 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
             const void* const bias_b = prm.bias == nullptr ? nullptr
                                        : static_cast<const uint8_t*>(prm.bias) + static_cast<size_t>(w.b) * static_cast<size_t>(prm.bias_batch_stride) * (prm.bias_is_bf16 ? 2u : 4u);
             if constexpr(EPI != 0)
-                if(prm.tma_store == 3)
+            {
+                if(prm.tma_store != 3)
+                    fused_plain_begin(plain, epi, prm, (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32, row_q0, bn, c_first, lane);
+                else
                     fused_begin(fused, epi, (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32, row_q0, bn, prm.rows_q, lane);
+            }
             ok = bounded_wait(acc_full_bar(a), (uc / prm.n_acc) & 1, abort_f, prm.status, ST_TIMEOUT_EPILOGUE, uc);
             ok = __all_sync(0xffffffffu, ok);
             if(!ok)
@@ -1185,7 +1190,7 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                     else
                     {
                         const float* red = reinterpret_cast<const float*>(smem_gen + L.red_off) + static_cast<size_t>(prow) * bn;
-                        ok = fused_plain_tile(epi, prm, tacc, p, row_q0, bn, c_first, csplit, red, static_cast<size_t>(per) * bn, red_bar, abort_f, uc, release_acc);
+                        ok = fused_plain_tile(plain, epi, prm, tacc, p, row_q0, bn, c_first, csplit, red, static_cast<size_t>(per) * bn, red_bar, abort_f, uc, release_acc);
                     }
                 }
                 else if(prm.out_mode >= OUT_E2M1)

@@ -807,6 +807,9 @@ static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
     e.act       = prob.activation;
     e.out_mode  = prob.out_mode;
     e.slot_bytes = 2048;
+    B200_CHECK(!prob.fused || (prob.residual_ld < (1LL << 28) && prob.ldo < (1LL << 28)), "the rows of the output or the residual lie too far apart");
+    e.res_step = static_cast<uint32_t>(prob.residual_ld);
+    e.out_step = static_cast<uint32_t>(prob.ldo);
     // more than L2 holds: neither the residual nor the output should push the operands out of it (16384 x 7168 x 2048, fp32
     // residual and output: 462 -> 444 us under the power cap; without effect where they fit)
     e.stream = prob.M * prob.N * ((prob.out_mode == OUT_F32 ? 4 : 2) + (prob.residual == nullptr ? 0 : prob.residual_mode == OUT_F32 ? 4 : 2)) > (256LL << 20);
@@ -1001,33 +1004,76 @@ static bool fused_rows_aligned(const GemmProblem& prob)
     return ok(prob.out, prob.ldo, prob.out_mode) && (prob.residual == nullptr || ok(prob.residual, prob.residual_ld, prob.residual_mode));
 }
 
+// bf16 with a fused epilogue, more than 64 rows.  Candidates are compared by a time estimate (units of 10 ns, `it` = K tiles of 64
+// elements) that was fitted to measurements of every tile by name on about 25 shapes (M = 100 .. 16384, N = 512 .. 8192, K = 512 ..
+// 8192): a start-up, and waves over the SMs times the time of a tile.  K is split inside a cluster only, one tile per cluster and
+// all clusters at once: 400 x 512 x 8192 43.8 (no split) -> 20.8 us; two waves of clusters are slower than none (300 x 1024 x 4096
+// in four slices 30.0, two 19.8, one 24.6 us).  Rows on odd addresses: weights on the 128-row slot, so that the lanes run along a
+// row of the output (4096 x 4097 x 1024: pairs 57.7 us, 128 x 256 tiles 64.5, row-major tiles 229).
+static void choose_fused_bf16(const GemmProblem& prob, int num_sms, KernelConfig& cfg)
+{
+    const long long M = prob.M, N = prob.N, it = (prob.K + 63) / 64;
+    auto up      = [](long long a, long long b) { return (a + b - 1) / b; };
+    const long long sms = num_sms, pairs = std::max<long long>(num_sms / 2, 1);
+    long long best = -1;
+    auto offer   = [&](int swap, int cg, int bn, int l2, long long cost) {
+        if(best >= 0 && cost >= best)
+            return;
+        best            = cost;
+        cfg.swap        = swap;
+        cfg.cg          = cg;
+        cfg.bn          = bn;
+        cfg.log2_splitk = l2;
+    };
+    const bool l2_open  = cfg.log2_splitk < 0;
+    const int l2_named  = std::max(cfg.log2_splitk, 0);
+    if(fused_rows_aligned(prob))
+    {
+        offer(0, 2, 256, 0, 500 + up(up(M, 256) * up(N, 256), pairs) * (400 + 30 * it));
+        offer(0, 2, 128, 0, 300 + up(up(M, 256) * up(N, 128), pairs) * (250 + 29 * it));
+        offer(0, 1, 64, 0, 250 + up(up(M, 128) * up(N, 64), sms) * (250 + 31 * it));
+    }
+    else
+    {
+        offer(1, 2, 256, 0, 700 + up(up(N, 256) * up(M, 256), pairs) * std::max<long long>(1380, 200 + 44 * it));
+        offer(1, 2, 128, 0, 600 + up(up(N, 256) * up(M, 128), pairs) * std::max<long long>(700, 200 + 31 * it));
+        offer(1, 1, 128, 0, 300 + up(up(N, 128) * up(M, 128), sms) * (600 + 33 * it));
+        offer(1, 1, 64, 0, 200 + up(up(N, 128) * up(M, 64), sms) * (500 + 30 * it));
+    }
+    const long long t64 = up(N, 128) * up(M, 64), t128 = up(N, 128) * up(M, 128);
+    auto fits = [&](long long ctas, int l2, long long slots) { return ctas <= (l2 >= 2 ? slots - slots / 8 : slots); }; // (clusters of four do not pack to the last SM)
+    for(int l2 = l2_open ? 0 : l2_named; l2 <= (l2_open ? 2 : l2_named) && l2 <= 2; ++l2)
+    {
+        if(M <= 256 && fits(t64 << l2, l2, 2 * sms)) // the few-rows kernel, two CTAs an SM
+            offer(1, 1, 64, l2, 500 + 150 * l2 + (30 * it >> l2) * ((t64 << l2) > sms ? 8 : 5) / 5);
+        if(M > 256 && l2 > 0 && fits(t64 << l2, l2, sms))
+            offer(1, 1, 64, l2, 700 + 300 * l2 + (30 * it >> l2));
+        if(M > 256 && l2 > 0 && fits(t128 << l2, l2, sms))
+            offer(1, 1, 128, l2, 1000 + 500 * l2 + (33 * it >> l2));
+    }
+}
+
 // What the fused epilogue prefers where choose_config would take something else; fields that the caller has set stay.
 static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConfig& cfg)
 {
     if(cfg.swap >= 0 || cfg.bn > 0 || cfg.cg > 0)
         return;
     const long long M = prob.M, N = prob.N;
-    const long long tiles_p = (N + kTileP - 1) / kTileP;
     if(M <= 64)
         return;
-    if(M <= 256 && prob.kind != PK_BF16)
-        return;
-    if(M <= 256)
+    if(prob.kind == PK_BF16)
     {
-        // tiles of 64 rows (128 where those do not fit the machine at once) on the few-rows kernel, K split inside a cluster
-        cfg.swap = 1;
-        cfg.cg   = 1;
-        cfg.bn   = tiles_p * ((M + 63) / 64) <= 2LL * num_sms ? 64 : 128;
+        choose_fused_bf16(prob, num_sms, cfg);
         return;
     }
+    if(M <= 256)
+        return;
     if(!fused_rows_aligned(prob))
     {
-        // rows on odd addresses: the weights on the 128-row slot, so that the lanes run along a row of the output
+        // rows on odd addresses: see above
         cfg.swap = 1;
-        cfg.cg   = 1;
+        cfg.cg   = 2;
         cfg.bn   = 256;
-        while(cfg.bn > 64 && tiles_p * ((M + cfg.bn - 1) / cfg.bn) < num_sms)
-            cfg.bn >>= 1;
         return;
     }
     // MX tiles on CTA pairs: 256 columns leave TMEM no second accumulator beside the scale buffers, so the epilogue is exposed;
@@ -1036,7 +1082,7 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
     // 224: 61 67 86 149 299, 74 86 113 173 332; 192: 52 56 73 148 240, 57 62 89 152 282; MXFP4 256: 62 67 85 114 174,
     // 65 71 87 116 181; 192: 53 56 65 82 144, 57 61 74 87 145 (224 leaves MXFP4 two stages: 60 67 83 127 232).
     const long long pair_rows = (M + 2 * kTileP - 1) / (2 * kTileP);
-    if(prob.kind != PK_BF16 && M >= 512 && N >= 192 && pair_rows * ((N + 255) / 256) >= 24)
+    if(M >= 512 && N >= 192 && pair_rows * ((N + 255) / 256) >= 24)
     {
         const bool res      = prob.residual != nullptr;
         const long long k10 = prob.K * 10 / 1024;

@@ -120,7 +120,7 @@ def test_against_64_bits(ab, kind, shape):
 
 @pytest.mark.parametrize("name", ["tc5_128x64_n_s0", "tc5_128x128_n_s0", "tc5_128x192_n_s3", "tc5_128x256_n_s0", "tc5_128x96_n_s0", "tc5_128x32_n_s0", "tc5_256x128_n_s0",
                                   "tc5_256x192_n_s0", "tc5_256x256_n_s0", "tc5_128x16_t_s0_k2", "tc5_128x64_t_s0_k1", "tc5_128x128_t_s0_k2", "tc5_128x128_t_s8_k3", "tc5_128x256_t_s0",
-                                  "tc5_128x128_n_s0_k4"])
+                                  "tc5_128x128_n_s0_k4", "tc5_256x256_t_s0", "tc5_256x128_t_s0", "tc5_256x192_t_s0"])
 def test_named_tiles(ab, name):
     m, n, k = (14, 1160, 1024) if "x16_t" in name else (240, 1160, 1024) if "_t_" in name else (700, 1160, 1024)
     p = Problem(ab, "bf16", m, n, k)

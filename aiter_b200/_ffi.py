@@ -126,13 +126,18 @@ def _pack_tensor(t):
         return None
     shape = t.shape
     ndim = len(shape)
-    assert ndim <= 8, f"aiter_tensor_t supports at most 8 dims, got {ndim}"
     dtype = _DTYPE_IDS.get(t.dtype)
-    return _PACKERS[ndim](t.data_ptr(), t.numel(), ndim, *shape, *t.stride(), aiter_dtype_id(t.dtype) if dtype is None else dtype,
-                          t.get_device() if t.is_cuda else -1)
+    if dtype is None:
+        dtype = aiter_dtype_id(t.dtype)  # raises, naming the type
+    if ndim == 2:
+        rows, cols = shape
+        row_stride, col_stride = t.stride()
+        return _pack_2d(t.data_ptr(), rows * cols, 2, rows, cols, row_stride, col_stride, dtype, t.get_device())
+    assert ndim <= 8, f"aiter_tensor_t supports at most 8 dims, got {ndim}"
+    return _PACKERS[ndim](t.data_ptr(), t.numel(), ndim, *shape, *t.stride(), dtype, t.get_device())
 
 
-_pack_1d, _pack_2d = _PACKERS[1], _PACKERS[2]
+_pack_2d = _PACKERS[2]
 
 
 def pack_rows(t: torch.Tensor, m: int, n: int, device: int) -> bytes:

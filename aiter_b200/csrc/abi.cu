@@ -78,6 +78,7 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
     require_tensor(out, fn, "out", 2);
     B200_CHECK(out->shape[0] == M && out->shape[1] == N, fn, ": out must be [", M, ", ", N, "] (got [", out->shape[0], ", ", out->shape[1], "])");
     require_rows_contiguous(out, fn, "out");
+    B200_CHECK(M <= 1 || out->strides[0] >= N, fn, ": the rows of out overlap one another");
     p.out_mode = plain_out_mode(out->dtype_);
     B200_CHECK(p.out_mode >= 0, fn, ": out must be bf16, fp16 or fp32 (got ", dtype_name(out->dtype_), ")");
     B200_CHECK(f.activation >= ACT_NONE && f.activation < ACT_COUNT, fn, ": activation must be 0 (none), 1 (relu), 2 (silu), 3 (gelu) or 4 (gelu_tanh), got ", f.activation);

@@ -68,12 +68,13 @@ int bytes_of(int dt) { return dt == OUT_F32 ? 4 : dt == OUT_E2M1 || dt == OUT_MX
 // every vector of eight elements of every row starts on a 16-byte boundary
 bool rows_aligned(const void* p, long long ld, int dt) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * bytes_of(dt)) % 16 == 0; }
 
-// A row of [M, n] values, contiguous along n
-RowTensor row_tensor(const aiter_tensor_t* t, const char* fn, const char* name, long long M, long long n)
+// A row of [M, n] values, contiguous along n (`written`: the rows do not overlap one another)
+RowTensor row_tensor(const aiter_tensor_t* t, const char* fn, const char* name, long long M, long long n, bool written = false)
 {
     require_tensor(t, fn, name, 2);
     B200_CHECK(t->shape[0] == M && t->shape[1] == n, fn, ": ", name, " must be [", M, ", ", n, "] (got [", t->shape[0], ", ", t->shape[1], "])");
     require_rows_contiguous(t, fn, name);
+    B200_CHECK(!written || M <= 1 || t->strides[0] >= n, fn, ": the rows of ", name, " overlap one another");
     return RowTensor{t->ptr, t->strides[0], float_type(t, fn, name)};
 }
 
@@ -117,6 +118,7 @@ void mx_output(const aiter_tensor_t* out, const aiter_tensor_t* scales, int layo
     B200_CHECK(layout >= 0 && layout <= 2, fn, ": shuffle_scale must be 0 (plain), 1 (e8m0_shuffle) or 2 ((m/32,k/4,32,4))");
     B200_CHECK(out->shape[0] == M && out->shape[1] == (fp4 ? n / 2 : n), fn, ": out must be [M, ", (fp4 ? "n/2" : "n"), "]");
     require_rows_contiguous(out, fn, "out");
+    B200_CHECK(M <= 1 || out->strides[0] >= out->shape[1], fn, ": the rows of out overlap one another");
     B200_CHECK((reinterpret_cast<uintptr_t>(out->ptr) & 7) == 0 && out->strides[0] % 8 == 0, fn, ": out rows must start on 8-byte boundaries");
     require_tensor(scales, fn, "scales", 2);
     B200_CHECK(scales->dtype_ == AITER_DTYPE_fp8_e8m0 || scales->dtype_ == AITER_DTYPE_u8, fn, ": scales must be e8m0 / uint8 (got ", dtype_name(scales->dtype_), ")");
@@ -403,7 +405,7 @@ extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_
         if(residual != nullptr)
             prm.res = row_tensor(residual, fn, "residual", M, n);
         if(residual_out != nullptr)
-            prm.h = row_tensor(residual_out, fn, "residual_out", M, n);
+            prm.h = row_tensor(residual_out, fn, "residual_out", M, n, true);
         prm.weight      = row_param(weight, fn, "weight", M, n);
         prm.bias        = row_param(bias, fn, "bias", M, n);
         prm.gate        = row_param(gate, fn, "gate", M, n, &prm.gate_scalar);
@@ -414,7 +416,7 @@ extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_
         else
         {
             B200_CHECK(scales == nullptr, fn, ": scales go with an MX output only");
-            prm.y = row_tensor(out, fn, "out", M, n);
+            prm.y = row_tensor(out, fn, "out", M, n, true);
         }
         for(const aiter_tensor_t* t : {out, scales, residual_out, residual, weight, bias, gate, post_weight, post_bias})
             require_same_device(x, t, fn, "an argument");
@@ -470,7 +472,7 @@ extern "C" int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* scale
         else
         {
             B200_CHECK(scales == nullptr, fn, ": scales go with an MX output only");
-            y = row_tensor(out, fn, "out", M, n);
+            y = row_tensor(out, fn, "out", M, n, true);
         }
         require_same_device(input, out, fn, "out");
         require_same_device(input, scales, fn, "scales");

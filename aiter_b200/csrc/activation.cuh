@@ -26,15 +26,14 @@ __device__ __forceinline__ float ex2_approx(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Two values at a time: sm_100 has two-wide fp32 multiply-adds (one issue slot for two), and in an epilogue issue slots are what
-// an activation costs.
+// Two values at a time.  Only gelu's polynomial uses the two-wide fp32 instructions of sm_100: for the short chains of silu and
+// gelu_tanh the moves into register pairs cost more than the issue slots they save (16384 x 12288 silu 192 against 181 us), for
+// gelu they save a little (217 -> 214 us; in the GEMM's epilogue 39 -> 35 us on 4096 x 4096 x 1024).
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }
-__device__ __forceinline__ float2 act_silu(float2 x)
-{
-    return __fmul2_rn(x, rcp2(__fadd2_rn(ex2_2(__fmul2_rn(x, splat(-1.4426950408889634f))), splat(1.f))));
-}
+__device__ __forceinline__ float act_silu1(float x) { return x * rcp_approx(1.f + ex2_approx(-1.4426950408889634f * x)); }
+__device__ __forceinline__ float2 act_silu(float2 x) { return make_float2(act_silu1(x.x), act_silu1(x.y)); }
 // x Phi(x) = max(x, 0) - |x| Phi(-|x|), which cancels nowhere.  Phi(-a) = e^(-a^2 / 2) P(t), t = 1 / (1 + 0.305 a): the form of
 // Hastings' approximation of the error function (Abramowitz and Stegun 7.1.26) with eight terms, fitted here by weighted least
 // squares to a relative error of 1e-7 over 0 <= a <= 14.5, behind which the product is below the smallest float.
@@ -54,11 +53,12 @@ __device__ __forceinline__ float2 act_gelu(float2 x)
     const float2 q = __fmul2_rn(__fmul2_rn(a, t), __fmul2_rn(p, e));
     return make_float2(x.x > 15.f ? x.x : fmaxf(x.x, 0.f) - q.x, x.y > 15.f ? x.y : fmaxf(x.y, 0.f) - q.y);
 }
-__device__ __forceinline__ float2 act_gelu_tanh(float2 x)
+__device__ __forceinline__ float act_gelu_tanh1(float x)
 {
-    const float2 u = __fmul2_rn(x, __ffma2_rn(__fmul2_rn(x, x), splat(-0.10294324f), splat(-2.3022082f))); // -2 u log2 e
-    return __fmul2_rn(x, rcp2(__fadd2_rn(ex2_2(u), splat(1.f))));
+    const float u = x * fmaf(x * x, -0.10294324f, -2.3022082f); // -2 u log2 e
+    return x * rcp_approx(1.f + ex2_approx(u));
 }
+__device__ __forceinline__ float2 act_gelu_tanh(float2 x) { return make_float2(act_gelu_tanh1(x.x), act_gelu_tanh1(x.y)); }
 
 // One test of `act` for N values, N even or 1 (a test per value would sit in every epilogue's innermost loop).
 template <int N>

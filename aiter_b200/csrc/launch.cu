@@ -803,7 +803,8 @@ static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
     e.res       = prob.residual;
     e.res_ld    = prob.residual_ld;
     e.res_mode  = prob.residual_mode;
-    e.res_vec   = (reinterpret_cast<uintptr_t>(prob.residual) & 15) == 0 && (prob.residual_ld * (prob.residual_mode == OUT_F32 ? 4 : 2)) % 16 == 0;
+    // (rows that do not overlap: a residual that is one broadcast row goes the plain way)
+    e.res_vec   = (reinterpret_cast<uintptr_t>(prob.residual) & 15) == 0 && (prob.residual_ld * (prob.residual_mode == OUT_F32 ? 4 : 2)) % 16 == 0 && prob.residual_ld >= prob.N;
     e.act       = prob.activation;
     e.out_mode  = prob.out_mode;
     e.slot_bytes = 2048;
@@ -1000,7 +1001,7 @@ constexpr long long kWidenPrepassMinM = 512;
 // Output and residual whose rows allow tile copies
 static bool fused_rows_aligned(const GemmProblem& prob)
 {
-    auto ok = [](const void* p, long long ld, int mode) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (mode == OUT_F32 ? 4 : 2)) % 16 == 0; };
+    auto ok = [&](const void* p, long long ld, int mode) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * (mode == OUT_F32 ? 4 : 2)) % 16 == 0 && ld >= prob.N; };
     return ok(prob.out, prob.ldo, prob.out_mode) && (prob.residual == nullptr || ok(prob.residual, prob.residual_ld, prob.residual_mode));
 }
 

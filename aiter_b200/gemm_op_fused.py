@@ -7,12 +7,14 @@ from torch import Tensor, empty
 
 from . import _ffi, dtypes
 from ._ffi import _pack_tensor as pack, call_packed, pack_rows
-from .block_ops import activation_id
+from .block_ops import ACTIVATIONS, activation_id
 
 
 def _prepare(fn: str, A: Tensor, k: int, n: int, activation, residual: Tensor | None, otype, out: Tensor | None):
     """Checks, the allocation of the output -> (rows, activation id, packed A, packed residual, packed out, result)"""
-    act = activation_id(activation, fn)
+    act = ACTIVATIONS.get(activation, 0)
+    if act == 0:
+        act = activation_id(activation, fn)
     flat = A.dim() == 2
     a2 = A if flat else A.reshape(-1, k)
     m = a2.shape[0]

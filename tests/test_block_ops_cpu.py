@@ -87,6 +87,8 @@ def test_norm_refusals(ab):
         ({"out": f((M, N), ptr=BASE + (3 << 20) + 64)}, "out overlaps residual"),
         ({"residual_out": f((M, N), ptr=BASE + (3 << 20) - 16)}, "residual_out overlaps residual"),
         ({"residual_out": f((M, N), torch.float16, ptr=BASE + (3 << 20))}, "residual_out overlaps residual"),
+        ({"residual_out": f((M, N), strides=(0, 1), ptr=far)}, "rows of residual_out overlap"),
+        ({"out": f((M, N), strides=(N - 8, 1))}, "rows of out overlap"),
     ]
     for over, match in cases:
         refuse(ab, name, norm_args(ab, **over), match)
@@ -111,6 +113,60 @@ def test_act_refusals(ab):
         ([f((M, N), torch.float8_e4m3fn), f((M, N // 32), torch.uint8, ptr=far + (1 << 20)), f((M, 2 * N), strides=(2 * N + 4, 1), ptr=far), 2, 0], "16-byte boundaries"),
     ]:
         refuse(ab, name, args, match)
+
+
+def test_fused_gemm_refusals(ab):
+    K, far = 128, BASE + (9 << 20)
+    f = lambda *a, **k: fake(ab, *a, **k)  # noqa: E731
+    A, B, out, bias, res = (f((M, K), ptr=BASE), f((N, K), ptr=BASE + (1 << 20)), f((M, N), ptr=BASE + (2 << 20)), f((N,), ptr=BASE + (3 << 20)), f((M, N), ptr=BASE + (4 << 20)))
+    base = dict(A=A, B=B, bias=bias, residual=res, out=out, activation=2, bpreshuffle=0, name=None)
+    for over, match in [
+        (dict(activation=5), "activation must be 0"),
+        (dict(activation=-1), "activation must be 0"),
+        (dict(out=f((M, N + 1), ptr=far)), "out must be [M, N]"),
+        (dict(out=f((M, N), torch.int32, ptr=far)), "unsupported output dtype"),
+        (dict(out=f((M, N), strides=(N // 2, 1), ptr=far)), "rows of out overlap"),
+        (dict(bias=f((N + 1,), ptr=far)), "bias must be [256]"),
+        (dict(bias=f((1, N), ptr=far)), "bias must be 1-D"),
+        (dict(bias=f((N,), strides=(2,), ptr=far)), "contiguous along its last dimension"),
+        (dict(bias=f((N,), torch.int8, ptr=far)), "bias must be bf16, fp16 or fp32"),
+        (dict(residual=f((M + 1, N), ptr=far)), "residual must be [4, 256]"),
+        (dict(residual=f((M, N), strides=(1, M), ptr=far)), "contiguous along its last dimension"),
+        (dict(residual=f((M, N), ptr=BASE + (2 << 20) + 2 * N)), "out overlaps residual"),
+        (dict(residual=f((M, N), torch.float16, ptr=BASE + (2 << 20))), "out overlaps residual"),
+        (dict(residual=f((M, N), ptr=far, device=2)), "lives on device 2"),
+        (dict(B=f((N, K + 8), ptr=far)), "disagree on K"),
+        (dict(B=f((N, K), ptr=far, device=1)), "lives on device 1"),
+        (dict(A=f((M, K), torch.float16, ptr=far)), "only bf16 inputs"),
+        (dict(A=f((M, K), ptr=far, device=-1)), "must live on a GPU"),
+        (dict(bpreshuffle=1, B=f((N, K), strides=(K + 8, 1), ptr=far)), "shuffled weight must be contiguous"),
+    ]:
+        args = {**base, **over}
+        refuse(ab, "aiter_b200_gemm_a16w16_fused", list(args.values()), match)
+    q, s32 = torch.float8_e4m3fn, f((32, K // 32), torch.uint8, ptr=BASE + (5 << 20))
+    sb = f((N, K // 32), torch.uint8, ptr=BASE + (6 << 20))
+    for args, match in [
+        ([f((M, K), q), f((N, K), q, ptr=far), s32, sb, f((N, 1), ptr=far), None, out, 0, 0, None], "bias must be 1-D"),
+        ([f((M, K), q), f((N, K), q, ptr=far), s32, f((N, K // 32), torch.uint8, ptr=far, device=1), None, None, out, 0, 0, None], "lives on device 1"),
+        ([f((M, K), q), f((N, K), q, ptr=far), s32, sb, None, None, out, 7, 0, None], "activation must be 0"),
+        ([f((M, 96), q), f((N, 96), q, ptr=far), s32, sb, None, None, out, 0, 0, None], "K must be divisible by 128"),
+    ]:
+        refuse(ab, "aiter_b200_gemm_a8w8_mxfp8_fused", args, match)
+    a4, b4 = f((M, K // 2), torch.uint8), f((N, K // 2), torch.uint8, ptr=far)
+    s4 = f((256, 8), torch.uint8, ptr=BASE + (7 << 20))
+    for ws, match in [(f((16,), torch.float32, ptr=far + (1 << 20)), "workspace must be a uint8"), (f((4, 4), torch.uint8, ptr=far + (1 << 20)), "workspace must be 1-D"),
+                      (f((16,), torch.uint8, ptr=far + 8), "workspace must be 16-byte aligned"), (f((16,), torch.uint8, ptr=far, device=3), "lives on device 3")]:
+        refuse(ab, "aiter_b200_gemm_a4w4_fused", [a4, b4, s4, s4, None, None, out, ws, 0, 1, None], match)
+    # workspace is asked for where the scales are re-laid: tall problems with a long K
+    assert ab._ffi.fused_workspace_bytes(64, 4096, 4096) == 0 and ab._ffi.fused_workspace_bytes(4096, 4096, 4096) == (128 + 128) * 32 * 128
+    with pytest.raises(ValueError, match="unknown activation"):
+        ab.gemm_a16w16_fused(torch.zeros(4, 64), torch.zeros(8, 64), activation="swish")
+    with pytest.raises(ValueError, match="residual must be"):
+        ab.gemm_a16w16_fused(torch.zeros(4, 64), torch.zeros(8, 64), residual=torch.zeros(4, 9))
+    with pytest.raises(ValueError, match="out must be"):
+        ab.gemm_a16w16_fused(torch.zeros(4, 64), torch.zeros(8, 64), out=torch.zeros(5, 8))
+    with pytest.raises(RuntimeError, match="must live on a GPU"):
+        ab.gemm_a16w16_fused(torch.zeros(4, 64).bfloat16(), torch.zeros(8, 64).bfloat16())
 
 
 def test_python_refusals(ab):

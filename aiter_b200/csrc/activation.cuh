@@ -60,17 +60,20 @@ __device__ __forceinline__ float act_gelu_tanh1(float x)
 }
 __device__ __forceinline__ float2 act_gelu_tanh(float2 x) { return make_float2(act_gelu_tanh1(x.x), act_gelu_tanh1(x.y)); }
 
-// One test of `act` for N values, N even or 1 (a test per value would sit in every epilogue's innermost loop).
-template <int N>
+// One test of `act` for N values, N even or 1 (a test per value would sit in every epilogue's innermost loop).  CLASS: 0 for any
+// activation, else only the code of one, 1 standing for none and relu.  (The persistent GEMMs are compiled per class: with all of
+// them in one kernel its warps evict one another's instructions.)
+template <int CLASS = 0, int N>
 __device__ __forceinline__ void activate(float (&v)[N], int act)
 {
-    if(act == ACT_RELU)
+    constexpr bool any = CLASS == 0;
+    if((any || CLASS == 1) && act == ACT_RELU)
     {
 #pragma unroll
         for(int i = 0; i < N; ++i)
             v[i] = act_relu(v[i]);
     }
-    else if(act == ACT_SILU)
+    else if(CLASS == ACT_SILU || (any && act == ACT_SILU))
     {
 #pragma unroll
         for(int i = 0; i < N; i += 2)
@@ -81,7 +84,7 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
                 v[(i + 1) % N] = y.y;
         }
     }
-    else if(act == ACT_GELU)
+    else if(CLASS == ACT_GELU || (any && act == ACT_GELU))
     {
 #pragma unroll
         for(int i = 0; i < N; i += 2)
@@ -92,7 +95,7 @@ __device__ __forceinline__ void activate(float (&v)[N], int act)
                 v[(i + 1) % N] = y.y;
         }
     }
-    else if(act == ACT_GELU_TANH)
+    else if(CLASS == ACT_GELU_TANH || (any && act == ACT_GELU_TANH))
     {
 #pragma unroll
         for(int i = 0; i < N; i += 2)

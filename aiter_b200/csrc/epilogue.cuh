@@ -6,19 +6,24 @@
 // slots in shared memory: the residual's tile of a step is loaded into a slot by TMA, read by the lanes (one row each,
 // swizzled), the finished rows are written back into the same slot and leave as a TMA tile store.  The loads of a warp's first
 // two steps and its bias values are requested before the accumulator is waited for.  (Prefetching the remaining residual tiles
-// into L2 as well measured no faster: 16384 x 7168 x 2048 with an fp32 residual 448 us with, 444 us without.)
+// into L2 as well measured no faster: 16384 x 7168 x 2048 with an fp32 residual 448 us with, 444 us without.  Plain 32-byte
+// stores from registers instead of slots and tile stores: 4096 x 7168 x 2048 MXFP8 with silu 64 us against 61 us, with a residual 73
+// against 63.  Steps of 16 columns, which halve the code: 79 us.)
+//
+// The kernels are compiled per activation: all of them in one kernel overflow the instruction caches that the epilogue, scale,
+// load and MMA warps share (4096 x 7168 x 2048 MXFP8: no activation 61 -> 56 us, silu 71 -> 61, gelu 89 -> 75; MXFP4 61 -> 52, 68 -> 57,
+// 76 -> 67).
 #pragma once
 #include "activation.cuh"
 #include "gemm_common.cuh"
+#include <type_traits>
 
 namespace b200 {
 
-template <int EPI>
-struct EpilogueParams
+struct NoEpilogue
 {
 };
-template <>
-struct alignas(64) EpilogueParams<1>
+struct alignas(64) FusedParams
 {
     CUtensorMap map_res;
     const void* bias; // [N]
@@ -34,6 +39,10 @@ struct alignas(64) EpilogueParams<1>
     int stream;           // residual and output are larger than L2: their lines leave it first
     uint32_t slot_bytes;  // 32 rows x 32 columns of the wider of residual and output: 2048 or 4096
 };
+
+// EPI of the kernels: 0 the plain epilogue, else the activation class (persistent kernel) or 1 (the others)
+template <int EPI>
+using EpilogueParams = std::conditional_t<EPI == 0, NoEpilogue, FusedParams>;
 
 constexpr int kFusedStep      = 32;
 constexpr int kFusedWarps     = 8;
@@ -77,7 +86,7 @@ struct FusedWarp
     int group;              // 0 or 1: the steps it takes
 };
 
-__device__ __forceinline__ void fused_load(const FusedWarp& f, const EpilogueParams<1>& epi, uint32_t seq, int row0, int col0)
+__device__ __forceinline__ void fused_load(const FusedWarp& f, const FusedParams& epi, uint32_t seq, int row0, int col0)
 {
     const uint32_t esize = epi.res_mode == OUT_F32 ? 4u : 2u;
     const uint32_t bar   = f.rbars + 8u * (seq & 1);
@@ -89,7 +98,7 @@ __device__ __forceinline__ void fused_load(const FusedWarp& f, const EpiloguePar
 }
 
 // Before the accumulator of a tile is waited for.  row0, col0: first row of the warp's 32, first column of the tile.
-__device__ __forceinline__ void fused_begin(const FusedWarp& f, const EpilogueParams<1>& epi, int row0, int col0, int bn, int rows_q, int lane)
+__device__ __forceinline__ void fused_begin(const FusedWarp& f, const FusedParams& epi, int row0, int col0, int bn, int rows_q, int lane)
 {
     const int steps = bn / kFusedStep;
     if(epi.bias != nullptr)
@@ -111,8 +120,8 @@ __device__ __forceinline__ void fused_begin(const FusedWarp& f, const EpiloguePa
 }
 
 // One warp's share of a tile.  Returns false when a wait ran out.
-template <typename Params, typename Release>
-__device__ __forceinline__ bool fused_tile(FusedWarp& f, const EpilogueParams<1>& epi, const Params& prm, const CUtensorMap* map_out, uint32_t tacc, int row0, int col0,
+template <int EPI, typename Params, typename Release>
+__device__ __forceinline__ bool fused_tile(FusedWarp& f, const FusedParams& epi, const Params& prm, const CUtensorMap* map_out, uint32_t tacc, int row0, int col0,
                                            int bn, volatile uint32_t* abort_f, int lane, int uc, Release&& release_acc)
 {
     constexpr int STEP = kFusedStep;
@@ -159,7 +168,7 @@ __device__ __forceinline__ bool fused_tile(FusedWarp& f, const EpilogueParams<1>
                 v[4 * j + 3] += t.w;
             }
         }
-        activate(v, epi.act);
+        activate<EPI>(v, epi.act);
         __syncwarp();
         uint8_t* slot = f.slots_gen + (f.seq & 1) * epi.slot_bytes;
         // a lane's row: 128 bytes of fp32, or 64 of a 16-bit type, in 16-byte pieces swizzled against bank conflicts
@@ -272,7 +281,7 @@ __device__ __forceinline__ void store16(T* dst, const float (&v)[16], uint32_t s
 }
 
 template <typename Params>
-__device__ __forceinline__ void fused_plain_load(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, int p, int q_first)
+__device__ __forceinline__ void fused_plain_load(FusedPlain& f, const FusedParams& epi, const Params& prm, int p, int q_first)
 {
     if(epi.res == nullptr)
         return;
@@ -289,7 +298,7 @@ __device__ __forceinline__ void fused_plain_load(FusedPlain& f, const EpiloguePa
 // Before the accumulator is waited for: the first group's residual into registers, the rest of this warp's part of the tile into
 // L2.  The registers of eight warps hold 8 KB of loads, which at the latency of HBM is 1 TB/s, at that of L2 three times as much.
 template <typename Params>
-__device__ __forceinline__ void fused_plain_begin(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, int p_warp0, int col0, int bn, int group, int lane)
+__device__ __forceinline__ void fused_plain_begin(FusedPlain& f, const FusedParams& epi, const Params& prm, int p_warp0, int col0, int bn, int group, int lane)
 {
     if(epi.res == nullptr)
         return;
@@ -313,8 +322,8 @@ __device__ __forceinline__ void fused_plain_begin(FusedPlain& f, const EpilogueP
 }
 
 // red / red_stride: the other K slices' partial sums of this thread's row.
-template <typename Params, typename Release>
-__device__ __forceinline__ bool fused_plain_tile(FusedPlain& f, const EpilogueParams<1>& epi, const Params& prm, uint32_t tacc, int p, int col0, int bn, int group, int csplit,
+template <int EPI, typename Params, typename Release>
+__device__ __forceinline__ bool fused_plain_tile(FusedPlain& f, const FusedParams& epi, const Params& prm, uint32_t tacc, int p, int col0, int bn, int group, int csplit,
                                                  const float* red, size_t red_stride, uint32_t red_bar, volatile uint32_t* abort_f, int uc, Release&& release_acc)
 {
     const int groups  = bn / 16;
@@ -376,7 +385,7 @@ __device__ __forceinline__ bool fused_plain_tile(FusedPlain& f, const EpiloguePa
                     v[j] += j < valid ? load_elem(epi.bias, epi.bias_mode, q_first + j) : 0.f;
             }
         }
-        activate(v, epi.act);
+        activate<EPI>(v, epi.act);
         if(epi.res != nullptr)
         {
             if(epi.res_mode == OUT_BF16)

@@ -70,7 +70,7 @@ struct DecodeFused
     float bias;
     uint32_t res[16];  // raw residual values of the next 16 rows
 };
-__device__ __forceinline__ void decode_load_residual(DecodeFused& f, const EpilogueParams<1>& epi, int row0, int rows)
+__device__ __forceinline__ void decode_load_residual(DecodeFused& f, const FusedParams& epi, int row0, int rows)
 {
     if(epi.res == nullptr)
         return;
@@ -78,9 +78,9 @@ __device__ __forceinline__ void decode_load_residual(DecodeFused& f, const Epilo
     for(int j = 0; j < 16; ++j)
         f.res[j] = (f.mine && row0 + j < rows) ? load_elem_raw(epi.res, epi.res_mode, static_cast<size_t>(row0 + j) * epi.res_ld + f.p) : 0u;
 }
-__device__ __forceinline__ void decode_load_residual(const DecodeFused&, const EpilogueParams<0>&, int, int) {}
+__device__ __forceinline__ void decode_load_residual(const DecodeFused&, const NoEpilogue&, int, int) {}
 
-__device__ __forceinline__ void decode_fused_epilogue(DecodeFused& f, const EpilogueParams<1>& epi, const DecodeParams& prm, const CUtensorMap* map_out, uint8_t* smem_gen,
+__device__ __forceinline__ void decode_fused_epilogue(DecodeFused& f, const FusedParams& epi, const DecodeParams& prm, const CUtensorMap* map_out, uint8_t* smem_gen,
                                                       uint32_t smem_base, uint32_t red_bar, uint32_t tlane, int p_local, int p_warp0, int row_q0, uint32_t zrank,
                                                       uint32_t per, volatile uint32_t* abort_f, int w, int lane)
 {

@@ -1186,11 +1186,11 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                 {
                     const int p_warp0 = (w.tp * CG + static_cast<int>(crank)) * kTileP + quarter * 32;
                     if(prm.tma_store == 3)
-                        ok = fused_tile(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, abort_f, lane, uc, release_acc);
+                        ok = fused_tile<EPI>(fused, epi, prm, &map_out, tacc, p_warp0, row_q0, bn, abort_f, lane, uc, release_acc);
                     else
                     {
                         const float* red = reinterpret_cast<const float*>(smem_gen + L.red_off) + static_cast<size_t>(prow) * bn;
-                        ok = fused_plain_tile(plain, epi, prm, tacc, p, row_q0, bn, c_first, csplit, red, static_cast<size_t>(per) * bn, red_bar, abort_f, uc, release_acc);
+                        ok = fused_plain_tile<EPI>(plain, epi, prm, tacc, p, row_q0, bn, c_first, csplit, red, static_cast<size_t>(per) * bn, red_bar, abort_f, uc, release_acc);
                     }
                 }
                 else if(prm.out_mode >= OUT_E2M1)

@@ -795,9 +795,9 @@ static void launch_decode_instance(int ctas, int tiles_q, int csplit, size_t sme
 }
 
 // What both kernels need of a fused epilogue; the residual's tensor map is filled in by the persistent launch.
-static EpilogueParams<1> epilogue_params(const GemmProblem& prob)
+static FusedParams epilogue_params(const GemmProblem& prob)
 {
-    EpilogueParams<1> e{};
+    FusedParams e{};
     e.bias      = prob.fused_bias;
     e.bias_mode = prob.fused_bias_mode;
     e.res       = prob.residual;
@@ -962,7 +962,7 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
     const size_t smem = L.total + 1024;
     if(prob.fused)
     {
-        const EpilogueParams<1> epi = epilogue_params(prob);
+        const FusedParams epi = epilogue_params(prob);
         if(kkind == KIND_BF16)
             launch_decode_instance<KIND_BF16, SFW_NONE, 1>(ctas, tiles_q, csplit, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
         else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
@@ -1079,19 +1079,23 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
     }
     // MX tiles on CTA pairs: 256 columns leave TMEM no second accumulator beside the scale buffers, so the epilogue is exposed;
     // 224 (MXFP8, four stages) or 192 have two.  Waves over the SM pairs x time per tile, fitted to 4096 x 7168 x K = 512 .. 8192
-    // (listed in 0.1 us, silu, then with a bf16 residual; the code counts in 0.01 us): MXFP8 256: 63 74 105 163 299, 68 77 112 187 337;
-    // 224: 61 67 86 149 299, 74 86 113 173 332; 192: 52 56 73 148 240, 57 62 89 152 282; MXFP4 256: 62 67 85 114 174,
-    // 65 71 87 116 181; 192: 53 56 65 82 144, 57 61 74 87 145 (224 leaves MXFP4 two stages: 60 67 83 127 232).
+    // (listed in 0.1 us, without activation, with silu, with a bf16 residual; the code counts in 0.01 us): MXFP8 256: 48 60 87 167 289,
+    // 65 76 104 170 300, 64 77 103 191 325; 224: 45 49 79 150 273, 63 67 87 165 312, 64 69 91 160 304; 192: 42 44 69 129 251,
+    // 56 59 74 151 292, 56 59 77 147 287; MXFP4 256: 47 50 67 98 156, 65 67 83 115 174, 64 66 82 114 177; 192: 44 46 58 77 133,
+    // 58 59 64 83 139, 58 58 64 84 146 (224 leaves MXFP4 two stages: 60 67 83 127 232 with silu).
     const long long pair_rows = (M + 2 * kTileP - 1) / (2 * kTileP);
     if(M >= 512 && N >= 192 && pair_rows * ((N + 255) / 256) >= 24)
     {
         const bool res      = prob.residual != nullptr;
+        const bool bare     = !res && prob.activation <= ACT_RELU;
         const long long k10 = prob.K * 10 / 1024;
+        auto line           = [&](long long least, long long start, long long slope) { return std::max(least, start + slope * k10); };
         auto tile_time      = [&](int bn) -> long long {
             if(prob.kind == PK_MXFP8)
-                return bn == 256 ? (res ? 500 + 34 * k10 : 430 + 32 * k10) : bn == 224 ? (res ? std::max(760LL, 400 + 36 * k10) : std::max(610LL, 120 + 36 * k10))
-                                                                                       : (res ? std::max(570LL, 230 + 33 * k10) : std::max(520LL, 120 + 32 * k10));
-            return bn == 256 ? (res ? 560 + 16 * k10 : 530 + 16 * k10) : (res ? std::max(570LL, 470 + 12 * k10) : std::max(530LL, 410 + 12 * k10));
+                return bn == 256   ? (bare ? line(0, 250, 33) : res ? line(0, 460, 34) : line(0, 430, 32))
+                       : bn == 224 ? (bare ? line(450, 90, 34) : res ? line(640, 200, 35) : line(610, 120, 36))
+                                   : (bare ? line(420, 60, 31) : res ? line(560, 150, 33) : line(520, 120, 32));
+            return bn == 256 ? (bare ? line(0, 370, 15) : line(0, 530, 16)) : bare ? line(440, 340, 12) : res ? line(560, 420, 12) : line(540, 410, 12);
         };
         const long long pairs = std::max(num_sms / 2, 1);
         long long best        = 0;
@@ -1353,7 +1357,7 @@ static void launch_gemm_locked(const GemmProblem& prob)
     const bool tma_store = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % 8 == 0) && (cfg.swap || cfg.bn >= 32) &&
                            (prob.out_mode == OUT_BF16 || prob.out_mode == OUT_F16) && prob.batch == 1;
     // fused epilogue through its slots: row-major output and residual whose pitches and bases allow tensor maps
-    EpilogueParams<1> epi = epilogue_params(prob);
+    FusedParams epi = epilogue_params(prob);
     const bool slots      = prob.fused && !cfg.swap && cfg.bn % kFusedStep == 0 && prob.batch == 1 && (reinterpret_cast<uintptr_t>(prob.out) & 15) == 0 &&
                        (prob.ldo * (prob.out_mode == OUT_F32 ? 4 : 2)) % 16 == 0 && (prob.residual == nullptr || epi.res_vec);
     int epi_units = tma_store && !prob.fused ? 1 : 0; // staging areas of 16 KB
@@ -1581,14 +1585,24 @@ static void launch_gemm_locked(const GemmProblem& prob)
     const int ctas         = clusters * cg * csplit;
     if(prob.fused)
     {
+        auto go = [&](auto kind, auto scales) {
+            constexpr int KIND = decltype(kind)::value, SFW = decltype(scales)::value;
+            switch(prob.activation)
+            {
+            case ACT_SILU: return launch_persistent_cg<KIND, SFW, ACT_SILU>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            case ACT_GELU: return launch_persistent_cg<KIND, SFW, ACT_GELU>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            case ACT_GELU_TANH: return launch_persistent_cg<KIND, SFW, ACT_GELU_TANH>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            default: return launch_persistent_cg<KIND, SFW, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            }
+        };
         if(kkind == KIND_BF16)
-            launch_persistent_cg<KIND_BF16, SFW_NONE, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            go(std::integral_constant<int, KIND_BF16>{}, std::integral_constant<int, SFW_NONE>{});
         else if(kkind == KIND_MXF8 && sfw == SFW_G1250)
-            launch_persistent_cg<KIND_MXF8, SFW_G1250, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            go(std::integral_constant<int, KIND_MXF8>{}, std::integral_constant<int, SFW_G1250>{});
         else if(kkind == KIND_MXF4 && sfw == SFW_E8M0_SHUFFLE)
-            launch_persistent_cg<KIND_MXF4, SFW_E8M0_SHUFFLE, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            go(std::integral_constant<int, KIND_MXF4>{}, std::integral_constant<int, SFW_E8M0_SHUFFLE>{});
         else if(kkind == KIND_MXF4 && sfw == SFW_G1250)
-            launch_persistent_cg<KIND_MXF4, SFW_G1250, 1>(cg, ctas, smem, prob.stream, mp, mq, msp, msq, mo, prm, epi);
+            go(std::integral_constant<int, KIND_MXF4>{}, std::integral_constant<int, SFW_G1250>{});
         else
             fail("no fused kernel instance for kind ", kkind, " with scale layout ", sfw);
     }

@@ -81,6 +81,8 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
     B200_CHECK(M <= 1 || out->strides[0] >= N, fn, ": the rows of out overlap one another");
     p.out_mode = plain_out_mode(out->dtype_);
     B200_CHECK(p.out_mode >= 0, fn, ": out must be bf16, fp16 or fp32 (got ", dtype_name(out->dtype_), ")");
+    const int ob = p.out_mode == OUT_F32 ? 4 : 2;
+    require_rows(out, ob, fn, "out");
     B200_CHECK(f.activation >= ACT_NONE && f.activation < ACT_COUNT, fn, ": activation must be 0 (none), 1 (relu), 2 (silu), 3 (gelu) or 4 (gelu_tanh), got ", f.activation);
     require_same_device(first, out, fn, "out");
     p.out        = out->ptr;
@@ -106,6 +108,10 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
         p.fused_bias      = f.bias->ptr;
         p.fused_bias_mode = plain_out_mode(f.bias->dtype_);
         B200_CHECK(p.fused_bias_mode >= 0, fn, ": bias must be bf16, fp16 or fp32 (got ", dtype_name(f.bias->dtype_), ")");
+        const int bb = p.fused_bias_mode == OUT_F32 ? 4 : 2;
+        require_rows(f.bias, bb, fn, "bias");
+        B200_CHECK(M == 0 || !overlap(Span{reinterpret_cast<uintptr_t>(f.bias->ptr), 0, N * bb, 1}, Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}), fn,
+                   ": out overlaps bias");
     }
     if(f.residual != nullptr)
     {
@@ -119,7 +125,8 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
         p.residual_mode = plain_out_mode(r->dtype_);
         B200_CHECK(p.residual_mode >= 0, fn, ": residual must be bf16, fp16 or fp32 (got ", dtype_name(r->dtype_), ")");
         // every value is read by the thread that writes it: the very same matrix may be updated in place, nothing else may overlap
-        const int rb = p.residual_mode == OUT_F32 ? 4 : 2, ob = p.out_mode == OUT_F32 ? 4 : 2;
+        const int rb = p.residual_mode == OUT_F32 ? 4 : 2;
+        require_rows(r, rb, fn, "residual");
         const bool same = r->ptr == out->ptr && p.residual_ld == p.ldo && p.residual_mode == p.out_mode;
         B200_CHECK(M == 0 || same ||
                        !overlap(Span{reinterpret_cast<uintptr_t>(r->ptr), p.residual_ld * rb, N * rb, M}, Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}),

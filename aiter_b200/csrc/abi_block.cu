@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <atomic>
 #include <string>
+#include <type_traits>
 
 using namespace b200;
 
@@ -75,7 +76,9 @@ RowTensor row_tensor(const aiter_tensor_t* t, const char* fn, const char* name, 
     B200_CHECK(t->shape[0] == M && t->shape[1] == n, fn, ": ", name, " must be [", M, ", ", n, "] (got [", t->shape[0], ", ", t->shape[1], "])");
     require_rows_contiguous(t, fn, name);
     B200_CHECK(!written || M <= 1 || t->strides[0] >= n, fn, ": the rows of ", name, " overlap one another");
-    return RowTensor{t->ptr, t->strides[0], float_type(t, fn, name)};
+    const int dt = float_type(t, fn, name);
+    require_rows(t, bytes_of(dt), fn, name);
+    return RowTensor{t->ptr, t->strides[0], dt};
 }
 
 // [n] for every row, or [groups, n]: M must be a multiple of groups, row r uses entry r / (M / groups).  `scalar`: [groups, 1] is
@@ -374,14 +377,24 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
         launch_norm_rows<8, 4>(prm, grid, block, stream);
 }
 
-template <int VEC, bool X32>
-void launch_act_mul(const ActMulParams& prm, cudaStream_t stream)
+template <bool X32, int ACT>
+void launch_act_mul(ActMulParams& prm, int out_dt, bool aligned, cudaStream_t stream)
 {
-    constexpr int U                = VEC == 1 ? 8 : 2;
-    const unsigned long long total = static_cast<unsigned long long>(prm.M) * prm.row_vecs;
-    const unsigned long long ctas  = (total + 256 * U - 1) / (256 * U);
-    B200_CHECK(ctas < (1ull << 31), "act_and_mul: too many elements");
-    launch(act_mul_kernel<VEC, X32, U>, dim3(static_cast<unsigned>(ctas)), dim3(256), stream, prm);
+    const char* big = "act_and_mul: too many elements";
+    if(out_dt > OUT_F32)
+    {
+        const unsigned long long tiles = static_cast<unsigned long long>((prm.M + 31ull) / 32) * ((prm.n / 32 + 7) / 8);
+        B200_CHECK(tiles < (1ull << 31), big);
+        const dim3 grid(static_cast<unsigned>(tiles)), block(256);
+        out_dt == OUT_E2M1 ? launch(act_mul_mx_kernel<X32, true, ACT>, grid, block, stream, prm) : launch(act_mul_mx_kernel<X32, false, ACT>, grid, block, stream, prm);
+        return;
+    }
+    prm.row_vecs                   = aligned ? prm.n / 8 : (prm.n + 14) / 8;
+    const unsigned per             = !aligned && X32 ? 256 : 512; // vectors of a CTA
+    const unsigned long long ctas  = (static_cast<unsigned long long>(prm.M) * prm.row_vecs + per - 1) / per;
+    B200_CHECK(ctas < (1ull << 31), big);
+    const dim3 grid(static_cast<unsigned>(ctas)), block(256);
+    aligned ? launch(act_mul_kernel<X32, ACT>, grid, block, stream, prm) : launch(act_mul_shift_kernel<X32, ACT>, grid, block, stream, prm);
 }
 
 } // namespace
@@ -493,22 +506,17 @@ extern "C" int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* scale
         const bool x32       = in.dt == OUT_F32;
         B200_CHECK(in_vec || y.dt <= OUT_F32, fn, ": with an MX output the input's rows must start on 16-byte boundaries");
         DeviceGuard guard(input->device_id);
-        if(y.dt > OUT_F32)
+        const bool aligned = in_vec && (y.dt > OUT_F32 || rows_aligned(y.ptr, y.ld, y.dt));
+        auto go = [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            x32 ? launch_act_mul<true, ACT>(prm, y.dt, aligned, s) : launch_act_mul<false, ACT>(prm, y.dt, aligned, s);
+        };
+        switch(activation)
         {
-            const unsigned long long tiles = static_cast<unsigned long long>((M + 31) / 32) * ((n / 32 + 7) / 8);
-            B200_CHECK(tiles < (1ull << 31), fn, ": too many elements");
-            const dim3 grid(static_cast<unsigned>(tiles)), block(256);
-            if(y.dt == OUT_E2M1)
-                x32 ? launch(act_mul_mx_kernel<true, true>, grid, block, s, prm) : launch(act_mul_mx_kernel<false, true>, grid, block, s, prm);
-            else
-                x32 ? launch(act_mul_mx_kernel<true, false>, grid, block, s, prm) : launch(act_mul_mx_kernel<false, false>, grid, block, s, prm);
-            return;
+        case ACT_RELU: return go(std::integral_constant<int, ACT_RELU>{});
+        case ACT_SILU: return go(std::integral_constant<int, ACT_SILU>{});
+        case ACT_GELU: return go(std::integral_constant<int, ACT_GELU>{});
+        default: return go(std::integral_constant<int, ACT_GELU_TANH>{});
         }
-        const bool vec = in_vec && rows_aligned(y.ptr, y.ld, y.dt);
-        prm.row_vecs   = static_cast<unsigned>(vec ? n / 8 : n);
-        if(vec)
-            x32 ? launch_act_mul<8, true>(prm, s) : launch_act_mul<8, false>(prm, s);
-        else
-            x32 ? launch_act_mul<1, true>(prm, s) : launch_act_mul<1, false>(prm, s);
     });
 }

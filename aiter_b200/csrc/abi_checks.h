@@ -40,6 +40,13 @@ inline void require_rows_contiguous(const aiter_tensor_t* t, const char* fn, con
                " must be contiguous along its last dimension");
 }
 
+// rows of `size`-byte elements: they start on an element's boundary and follow one another upwards
+inline void require_rows(const aiter_tensor_t* t, int size, const char* fn, const char* name)
+{
+    B200_CHECK(reinterpret_cast<uintptr_t>(t->ptr) % static_cast<unsigned>(size) == 0, fn, ": ", name, " does not start on an element's boundary");
+    B200_CHECK(t->ndim < 2 || t->shape[0] <= 1 || t->strides[0] >= 0, fn, ": ", name, " has a negative stride");
+}
+
 inline void require_dense(const aiter_tensor_t* t, const char* fn, const char* name)
 {
     int64_t expect = 1;

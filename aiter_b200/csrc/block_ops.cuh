@@ -620,19 +620,22 @@ struct ActMulParams
     long long out_ld;
     int in_dt, out_dt, act;
     unsigned M, n;
-    unsigned row_vecs; // vectors per row (plain outputs)
+    unsigned row_vecs; // vectors of eight per row, the partial ones included (plain outputs)
     BlockScales sf;
 };
 
-// Plain outputs: a thread takes U vectors, 256 vectors apart, of the flat list of all rows' vectors; HBM-bound.
-template <int VEC, bool X32, int U>
+// Plain outputs: a thread takes U vectors of eight, 256 vectors apart, of the flat list of all rows' vectors; HBM-bound
+// (16384 x 12288: silu and gelu_tanh 175 us, 6.9 TB/s; gelu 202, whose arithmetic shows).  Compiled per activation: with all of them in
+// one kernel 190 and 207 us.
+template <bool X32, int ACT>
 __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ ActMulParams prm)
 {
+    constexpr int U = 2;
     grid_dependency_wait();
     grid_launch_dependents();
     const unsigned long long total = static_cast<unsigned long long>(prm.M) * prm.row_vecs;
     const unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * (256 * U) + threadIdx.x;
-    Raw<VEC, X32> a[U], b[U];
+    Raw<8, X32> a[U], b[U];
     size_t out_at[U];
 #pragma unroll
     for(int u = 0; u < U; ++u)
@@ -641,10 +644,10 @@ __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ Ac
         if(i < total)
         {
             const unsigned row = total <= 0xFFFFFFFFull ? static_cast<unsigned>(i) / prm.row_vecs : static_cast<unsigned>(i / prm.row_vecs);
-            const unsigned col = static_cast<unsigned>(i - static_cast<unsigned long long>(row) * prm.row_vecs) * VEC;
+            const unsigned col = static_cast<unsigned>(i - static_cast<unsigned long long>(row) * prm.row_vecs) * 8;
             const size_t at    = static_cast<size_t>(row) * prm.in_ld + col;
-            ld_raw<VEC, X32>(a[u], prm.in, at);
-            ld_raw<VEC, X32>(b[u], prm.in, at + prm.n);
+            ld_raw<8, X32>(a[u], prm.in, at);
+            ld_raw<8, X32>(b[u], prm.in, at + prm.n);
             out_at[u] = static_cast<size_t>(row) * prm.out_ld + col;
         }
     }
@@ -653,21 +656,125 @@ __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ Ac
     {
         if(first + static_cast<unsigned long long>(u) * 256 < total)
         {
-            float g[VEC], v[VEC];
-            unpack<VEC, X32>(a[u], prm.in_dt, g);
-            unpack<VEC, X32>(b[u], prm.in_dt, v);
-            activate(g, prm.act);
+            float g[8], v[8];
+            unpack<8, X32>(a[u], prm.in_dt, g);
+            unpack<8, X32>(b[u], prm.in_dt, v);
+            activate<ACT>(g, prm.act);
 #pragma unroll
-            for(int i = 0; i < VEC; ++i)
+            for(int i = 0; i < 8; ++i)
                 v[i] *= g[i];
-            st_vec<VEC>(prm.out, prm.out_dt, out_at[u], v);
+            st_vec<8>(prm.out, prm.out_dt, out_at[u], v);
+        }
+    }
+}
+
+// Elements `lo` .. `hi` - 1 of the eight that begin at `p`, on any element's address: the 16-byte pieces that hold one of them, moved
+// into place.  (No other piece is read: a piece with one byte of the tensor lies in its memory.)
+template <bool B32>
+__device__ __forceinline__ void ld_shifted(Raw<8, B32>& r, const uint8_t* p, int lo, int hi)
+{
+    constexpr int E = B32 ? 4 : 8, PIECES = B32 ? 3 : 2;
+    const int s          = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / (16 / E); // element 0's place in its piece
+    const uint8_t* piece = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+    uint32_t w[4 * PIECES];
+#pragma unroll
+    for(int i = 0; i < PIECES; ++i)
+    {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if(i * E - s < hi && (i + 1) * E - s > lo)
+            v = *reinterpret_cast<const uint4*>(piece + 16 * i); // (through L1: the next thread reads one of the pieces too)
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+    if(B32)
+    {
+        // by two words, by one
+#pragma unroll
+        for(int i = 0; i < 9; ++i)
+            w[i] = (s & 2) ? w[(i + 2) % (4 * PIECES)] : w[i];
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+            r.w[i] = (s & 1) ? w[i + 1] : w[i];
+    }
+    else
+    {
+        // by two words, by one, by half a word
+#pragma unroll
+        for(int i = 0; i < 6; ++i)
+            w[i] = (s & 4) ? w[i + 2] : w[i];
+#pragma unroll
+        for(int i = 0; i < 5; ++i)
+            w[i] = (s & 2) ? w[i + 1] : w[i];
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            r.w[B32 ? 0 : i] = __funnelshift_r(w[i], w[i + 1], (s & 1) * 16);
+    }
+}
+
+// Rows that start on any element's address: a thread's eight outputs begin on a 16-byte boundary of the output's row (its first and
+// last groups are partial), their operands are shifted into place (8192 x 1001 14.5 us, one element at a time 26).
+template <bool X32, int ACT>
+__global__ void __launch_bounds__(256) act_mul_shift_kernel(const __grid_constant__ ActMulParams prm)
+{
+    constexpr int U = X32 ? 1 : 2;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const unsigned long long total = static_cast<unsigned long long>(prm.M) * prm.row_vecs;
+    const unsigned long long first = static_cast<unsigned long long>(blockIdx.x) * (256 * U) + threadIdx.x;
+    const int in_size = X32 ? 4 : 2, out_size = prm.out_dt == OUT_F32 ? 4 : 2;
+    Raw<8, X32> a[U], b[U];
+    int lo[U], hi[U];
+    long long out_at[U];
+#pragma unroll
+    for(int u = 0; u < U; ++u)
+    {
+        const unsigned long long i = first + static_cast<unsigned long long>(u) * 256;
+        lo[u] = hi[u] = 0;
+        if(i < total)
+        {
+            const unsigned row   = total <= 0xFFFFFFFFull ? static_cast<unsigned>(i) / prm.row_vecs : static_cast<unsigned>(i / prm.row_vecs);
+            const unsigned group = static_cast<unsigned>(i - static_cast<unsigned long long>(row) * prm.row_vecs);
+            const long long dst  = static_cast<long long>(row) * prm.out_ld;
+            const int before     = static_cast<int>((reinterpret_cast<uintptr_t>(prm.out) + dst * out_size) & 15) / out_size; // elements of the first group in front of the row
+            const long long col  = static_cast<long long>(group) * 8 - before;
+            lo[u]                = group == 0 ? before : 0;
+            hi[u]                = static_cast<int>(min(8ll, static_cast<long long>(prm.n) - col));
+            out_at[u]            = dst + col;
+            if(lo[u] < hi[u])
+            {
+                const uint8_t* src = static_cast<const uint8_t*>(prm.in) + (static_cast<long long>(row) * prm.in_ld + col) * in_size;
+                ld_shifted<X32>(a[u], src, lo[u], hi[u]);
+                ld_shifted<X32>(b[u], src + static_cast<size_t>(prm.n) * in_size, lo[u], hi[u]);
+            }
+        }
+    }
+#pragma unroll
+    for(int u = 0; u < U; ++u)
+    {
+        if(lo[u] < hi[u])
+        {
+            float g[8], v[8];
+            unpack<8, X32>(a[u], prm.in_dt, g);
+            unpack<8, X32>(b[u], prm.in_dt, v);
+            activate<ACT>(g, prm.act);
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                v[i] *= g[i];
+            if(hi[u] - lo[u] == 8)
+                st_vec<8>(static_cast<uint8_t*>(prm.out) + out_at[u] * out_size, prm.out_dt, 0, v);
+            else
+            {
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    if(i >= lo[u] && i < hi[u])
+                        store_out(static_cast<uint8_t*>(prm.out) + (out_at[u] + i) * out_size, 0, v[i], prm.out_dt);
+            }
         }
     }
 }
 
 // MX outputs: a CTA of eight warps takes 32 rows x 8 blocks (256 columns), four rows a warp, so that the tile's 256 scale
 // bytes, one chunk of either GEMM layout, are collected in shared memory and leave in whole words.
-template <bool X32, bool FP4>
+template <bool X32, bool FP4, int ACT>
 __global__ void __launch_bounds__(256) act_mul_mx_kernel(const __grid_constant__ ActMulParams prm)
 {
     __shared__ __align__(16) uint8_t sf_tile[256];
@@ -700,7 +807,7 @@ __global__ void __launch_bounds__(256) act_mul_mx_kernel(const __grid_constant__
         {
             unpack<8, X32>(a[u], prm.in_dt, g);
             unpack<8, X32>(b[u], prm.in_dt, v);
-            activate(g, prm.act);
+            activate<ACT>(g, prm.act);
         }
 #pragma unroll
         for(int i = 0; i < 8; ++i)

@@ -9,6 +9,8 @@ There is no fallback: if the library is missing the import of this module fails.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 
@@ -140,12 +142,6 @@ def _pack_tensor(t):
 _pack_2d = _PACKERS[2]
 
 
-def pack_rows(t: torch.Tensor, m: int, n: int, device: int) -> bytes:
-    """Descriptor of a contiguous [m, n] tensor that the caller has just allocated on `device`."""
-    dtype = _DTYPE_IDS.get(t.dtype)
-    return _pack_2d(t.data_ptr(), m * n, 2, m, n, n, 1, aiter_dtype_id(t.dtype) if dtype is None else dtype, device)
-
-
 def _int(value):
     return -1 if value is None else int(value)
 
@@ -209,15 +205,32 @@ def current_stream(device: int):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def call_packed(name: str, device: int, *args):
-    """`call` with every argument in the form the library takes: descriptors packed, no None among the numbers."""
-    fn, _ = _FUNCS.get(name) or _bind(name)
+def _load_host():
+    """The extension that allocates, fills descriptors and calls for the operators whose host time shows (see csrc/host.cpp)."""
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "_aiter_b200_host.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python aiter_b200/build.py`")
+    loader = importlib.machinery.ExtensionFileLoader("_aiter_b200_host", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_aiter_b200_host", loader))
+    loader.exec_module(module)
+    names = ("gated_residual_norm", "act_and_mul", "gemm_a16w16_fused", "gemm_a8w8_mxfp8_fused", "gemm_a4w4_fused", "gemm_a4w4_fused_workspace")
+    module.bind(*(ctypes.cast(getattr(_lib, f"aiter_b200_{n}"), ctypes.c_void_p).value for n in names), dict(_DTYPE_IDS), aiter_dtype_id)
+    return module
+
+
+host = _load_host()
+
+
+def call_host(name: str, function, *args):
+    """A function of the extension: the entry point `name` on the stream that ends `args`; what it returns."""
     if AITER_LOG_MORE == 2:
         import logging
 
-        logging.getLogger("aiter").info("calling %s(%s)", name, ", ".join(f"<{len(a)} bytes>" if isinstance(a, bytes) else repr(a) for a in args))
-    if fn(*args, current_stream(device)) != 0:
+        logging.getLogger("aiter").info("calling %s(%s)", name, ", ".join(_describe(a) for a in args))
+    result = function(*args)
+    if result is None:
         _raise(name)
+    return result
 
 
 def get_padded_m(M: int, N: int, K: int, gl: int) -> int:
@@ -252,10 +265,6 @@ def debug_wait_control(device: int = 0, limit_ns: int = 1_000_000_000, withhold_
     if rc != 0:
         msg = _lib.aiter_get_last_error()
         raise RuntimeError(f"aiter_b200_debug_wait_control failed: {msg.decode() if msg else ''}")
-
-
-def fused_workspace_bytes(M: int, N: int, K: int) -> int:
-    return int(_lib.aiter_b200_gemm_a4w4_fused_workspace(int(M), int(N), int(K)))
 
 
 def kernel_list() -> str:

@@ -4,10 +4,10 @@ instead of 16-bit values.  The reference's closest forms: aiter/ops/rmsnorm.py, 
 from __future__ import annotations
 
 import torch
-from torch import Tensor, empty, empty_like
+from torch import Tensor, empty
 
-from . import _ffi, dtypes
-from ._ffi import _pack_tensor as pack, call_packed, pack_rows
+from . import dtypes
+from ._ffi import call_host, current_stream, host
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 _NORMS = {"rms": 0, "layer": 1}
@@ -62,37 +62,29 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
     if norm not in _NORMS:
         raise ValueError(f"{fn}: unknown norm {norm!r}, expected 'rms' or 'layer'")
     post = (post_weight is not None or post_bias is not None) if post_norm is None else bool(post_norm)
-    n = x.shape[-1]
-    x2 = x if x.dim() == 2 else x.reshape(-1, n)
-    m = x2.shape[0]
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
     r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, residual.shape[-1])
-    copies_x = residual is None and gate is None and not post and residual_out is None
-    dev = x.get_device()
-    if residual_out is not None:
-        if residual_out.shape != x.shape:
-            raise ValueError(f"{fn}: residual_out must have x's shape {tuple(x.shape)}, got {tuple(residual_out.shape)}")
-        h = residual_out
-        h2 = pack(h if h.dim() == 2 else h.view(-1, n))
-    elif copies_x:
-        h, h2 = x, None
-    else:
-        like = x if residual is None else residual
-        h = empty_like(like) if like.is_contiguous() and like.shape == x.shape else empty(*x.shape, dtype=like.dtype, device=x.device)
-        h2 = pack_rows(h, m, n, dev)
-    scale, layout = None, 0
+    o2 = residual_out
+    if o2 is not None:
+        if o2.shape != x.shape:
+            raise ValueError(f"{fn}: residual_out must have x's shape {tuple(x.shape)}, got {tuple(o2.shape)}")
+        o2 = o2 if flat else o2.view(-1, x.shape[-1])
+    y, scale, layout = None, None, 0
     if quant_dtype is not None:
         if otype is not None:
             raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
-        y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
+        y, scale = _mx_out(fn, *x2.shape, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
-        y2 = pack(y)
-    else:
-        y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
-        y2 = pack_rows(y, m, n, dev)
-    call_packed("aiter_b200_gated_residual_norm", dev, y2, pack(scale), h2, pack(x2), pack(r2), pack(weight), pack(bias), pack(gate),
-                pack(post_weight), pack(post_bias), residual_scale, weight_offset, eps, _NORMS[norm], post, layout)
-    if x.dim() != 2:
+    y, h = call_host("aiter_b200_gated_residual_norm", host.norm, x2, r2, weight, bias, gate, post_weight, post_bias, o2, y, scale, otype,
+                     residual_scale, weight_offset, eps, _NORMS[norm], post, layout, current_stream(x.get_device()))
+    if not flat:
         y = y.view(*x.shape[:-1], y.shape[-1])
+        h = h if h is None else h.view(x.shape)
+    if residual_out is not None:
+        h = residual_out
+    elif h is None:
+        h = x
     return (y, h) if scale is None else (y, scale, h)
 
 
@@ -107,21 +99,16 @@ def act_and_mul(x: Tensor, activation: str = "silu", otype: torch.dtype | None =
         raise ValueError(f"{fn}: an activation is required")
     if x.shape[-1] % 2 != 0:
         raise ValueError(f"{fn}: the last dimension must be even, got {x.shape[-1]}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    m, n = x2.shape[0], x2.shape[1] // 2
-    dev = x.get_device()
-    scale, layout = None, 0
+    flat = x.dim() == 2
+    x2 = x if flat else x.reshape(-1, x.shape[-1])
+    y, scale, layout = None, None, 0
     if quant_dtype is not None:
         if otype is not None:
             raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
-        y, scale = _mx_out(fn, m, n, quant_dtype, shuffle, x.device)
+        y, scale = _mx_out(fn, x2.shape[0], x2.shape[1] // 2, quant_dtype, shuffle, x.device)
         layout = int(shuffle)
-        y2 = pack(y)
-    else:
-        y = empty(m, n, dtype=x.dtype if otype is None else otype, device=x.device)
-        y2 = pack_rows(y, m, n, dev)
-    call_packed("aiter_b200_act_and_mul", dev, y2, pack(scale), pack(x2), act, layout)
-    if x.dim() != 2:
+    y = call_host("aiter_b200_act_and_mul", host.act, x2, y, scale, otype, act, layout, current_stream(x.get_device()))
+    if not flat:
         y = y.view(*x.shape[:-1], y.shape[-1])
     return y if scale is None else (y, scale)
 
@@ -142,4 +129,4 @@ def gelu_tanh_and_mul(out: Tensor, input: Tensor) -> None:
 def _act_and_mul_into(out: Tensor, input: Tensor, activation: str) -> None:
     x2 = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
     o2 = out if out.dim() == 2 else out.view(-1, out.shape[-1])
-    _ffi.call("aiter_b200_act_and_mul", o2, None, x2, ACTIVATIONS[activation], 0)
+    call_host("aiter_b200_act_and_mul", host.act, x2, o2, None, None, ACTIVATIONS[activation], 0, current_stream(input.get_device()))

@@ -158,7 +158,8 @@ def test_fused_gemm_refusals(ab):
                       (f((16,), torch.uint8, ptr=far + 8), "workspace must be 16-byte aligned"), (f((16,), torch.uint8, ptr=far, device=3), "lives on device 3")]:
         refuse(ab, "aiter_b200_gemm_a4w4_fused", [a4, b4, s4, s4, None, None, out, ws, 0, 1, None], match)
     # workspace is asked for where the scales are re-laid: tall problems with a long K
-    assert ab._ffi.fused_workspace_bytes(64, 4096, 4096) == 0 and ab._ffi.fused_workspace_bytes(4096, 4096, 4096) == (128 + 128) * 32 * 128
+    workspace = ab._ffi._lib.aiter_b200_gemm_a4w4_fused_workspace
+    assert workspace(64, 4096, 4096) == 0 and workspace(4096, 4096, 4096) == (128 + 128) * 32 * 128
     with pytest.raises(ValueError, match="unknown activation"):
         ab.gemm_a16w16_fused(torch.zeros(4, 64), torch.zeros(8, 64), activation="swish")
     with pytest.raises(ValueError, match="residual must be"):

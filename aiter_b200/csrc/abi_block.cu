@@ -168,20 +168,20 @@ void launch(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t strea
 {
     launch_smem(kernel, grid, block, 0, stream, prm...);
 }
-constexpr unsigned kLongRow = 16384; // elements of a row that the register kernels hold at most (512 threads x 32)
+constexpr unsigned kLongRow = 16384; // elements of a row that the register kernels hold at most (512 threads x 4 groups of eight)
 
-template <int VEC, int CNT>
+template <int CNT, bool SHIFT>
 void launch_norm_rows(const NormParams& prm, dim3 grid, dim3 block, cudaStream_t stream)
 {
     const bool x32 = prm.x.dt == OUT_F32, r32 = prm.res.ptr != nullptr && prm.res.dt == OUT_F32;
     if(x32 && r32)
-        launch(norm_rows_kernel<VEC, CNT, true, true>, grid, block, stream, prm);
+        launch(norm_rows_kernel<CNT, true, true, SHIFT>, grid, block, stream, prm);
     else if(x32)
-        launch(norm_rows_kernel<VEC, CNT, true, false>, grid, block, stream, prm);
+        launch(norm_rows_kernel<CNT, true, false, SHIFT>, grid, block, stream, prm);
     else if(r32)
-        launch(norm_rows_kernel<VEC, CNT, false, true>, grid, block, stream, prm);
+        launch(norm_rows_kernel<CNT, false, true, SHIFT>, grid, block, stream, prm);
     else
-        launch(norm_rows_kernel<VEC, CNT, false, false>, grid, block, stream, prm);
+        launch(norm_rows_kernel<CNT, false, false, SHIFT>, grid, block, stream, prm);
 }
 
 // ---- many rows: the streaming kernels, for the usual types (types that differ more run the general kernels)
@@ -339,7 +339,8 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
     const unsigned n = prm.n;
     if(try_norm_stream(prm, aligned, device, sms, stream))
         return;
-    if(n > kLongRow)
+    const unsigned vecs = aligned ? (n + 7) / 8 : (n + 14) / 8; // groups of eight that a row touches at most
+    if(vecs > kLongRow / 8)
     {
         if(aligned)
             launch(norm_long_kernel<8>, dim3(prm.M), dim3(512), stream, prm);
@@ -347,34 +348,17 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
             launch(norm_long_kernel<1>, dim3(prm.M), dim3(512), stream, prm);
         return;
     }
-    const unsigned per = aligned ? 8 : 1; // elements of a vector
-    const unsigned vecs = (n + per - 1) / per;
-    auto shape = [&](unsigned cnt) {
-        const unsigned t = ((vecs + cnt - 1) / cnt + 31) / 32 * 32;
-        const unsigned r = t == 32 ? 4 : 1; // a warp a row: four rows a CTA
-        return std::make_pair(dim3((prm.M + r - 1) / r), dim3(t, r));
-    };
-    if(!aligned)
-    {
-        // one element at a time: 8 or 32 a thread
-        const unsigned cnt = vecs > 2048 ? 32 : 8;
-        auto [grid, block] = shape(cnt);
-        if(cnt == 8)
-            launch_norm_rows<1, 8>(prm, grid, block, stream);
-        else
-            launch_norm_rows<1, 32>(prm, grid, block, stream);
-        return;
-    }
-    // one vector a thread where there are few rows (the shortest chain), up to four where the machine is full
+    // one group a thread where there are few rows (the shortest chain), up to four where the machine is full
     const bool few     = prm.M <= 2u * static_cast<unsigned>(sms);
     const unsigned cnt = vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1;
-    auto [grid, block] = shape(cnt);
+    const unsigned t   = ((vecs + cnt - 1) / cnt + 31) / 32 * 32, r = t == 32 ? 4 : 1; // (a warp a row: four rows a CTA)
+    const dim3 grid((prm.M + r - 1) / r), block(t, r);
     if(cnt == 1)
-        launch_norm_rows<8, 1>(prm, grid, block, stream);
+        aligned ? launch_norm_rows<1, false>(prm, grid, block, stream) : launch_norm_rows<1, true>(prm, grid, block, stream);
     else if(cnt == 2)
-        launch_norm_rows<8, 2>(prm, grid, block, stream);
+        aligned ? launch_norm_rows<2, false>(prm, grid, block, stream) : launch_norm_rows<2, true>(prm, grid, block, stream);
     else
-        launch_norm_rows<8, 4>(prm, grid, block, stream);
+        aligned ? launch_norm_rows<4, false>(prm, grid, block, stream) : launch_norm_rows<4, true>(prm, grid, block, stream);
 }
 
 template <bool X32, int ACT>

@@ -180,6 +180,77 @@ __device__ __forceinline__ void st_vec(void* base, int dt, size_t at, const floa
     }
 }
 
+// Elements `lo` .. `hi` - 1 of the eight that begin at `p`, on any element's address: the 16-byte pieces that hold one of them, moved
+// into place.  (No other piece is read: a piece with one byte of the tensor lies in its memory.)
+template <bool B32>
+__device__ __forceinline__ void ld_shifted(Raw<8, B32>& r, const uint8_t* p, int lo, int hi)
+{
+    constexpr int E = B32 ? 4 : 8, PIECES = B32 ? 3 : 2;
+    const int s          = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / (16 / E); // element 0's place in its piece
+    const uint8_t* piece = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
+    uint32_t w[4 * PIECES];
+#pragma unroll
+    for(int i = 0; i < PIECES; ++i)
+    {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if(i * E - s < hi && (i + 1) * E - s > lo)
+            v = *reinterpret_cast<const uint4*>(piece + 16 * i); // (through L1: the next thread reads one of the pieces too)
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+    if(B32)
+    {
+        // by two words, by one
+#pragma unroll
+        for(int i = 0; i < 9; ++i)
+            w[i] = (s & 2) ? w[(i + 2) % (4 * PIECES)] : w[i];
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+            r.w[i] = (s & 1) ? w[i + 1] : w[i];
+    }
+    else
+    {
+        // by two words, by one, by half a word
+#pragma unroll
+        for(int i = 0; i < 6; ++i)
+            w[i] = (s & 4) ? w[i + 2] : w[i];
+#pragma unroll
+        for(int i = 0; i < 5; ++i)
+            w[i] = (s & 2) ? w[i + 1] : w[i];
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            r.w[B32 ? 0 : i] = __funnelshift_r(w[i], w[i + 1], (s & 1) * 16);
+    }
+}
+
+// the same of a parameter, whose type is looked at here
+__device__ __forceinline__ void ld_param_shifted(const void* base, int dt, long long at, int lo, int hi, float (&v)[8])
+{
+    if(dt == OUT_F32)
+    {
+        Raw<8, true> r;
+        ld_shifted<true>(r, static_cast<const uint8_t*>(base) + at * 4, lo, hi);
+        unpack<8, true>(r, dt, v);
+    }
+    else
+    {
+        Raw<8, false> r;
+        ld_shifted<false>(r, static_cast<const uint8_t*>(base) + at * 2, lo, hi);
+        unpack<8, false>(r, dt, v);
+    }
+}
+// elements `lo` .. `hi` - 1 of the eight that begin at element `at`
+__device__ __forceinline__ void st_shifted(void* base, int dt, long long at, int lo, int hi, const float (&v)[8])
+{
+    uint8_t* p = static_cast<uint8_t*>(base) + at * (dt == OUT_F32 ? 4 : 2);
+    if(hi - lo == 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0)
+        st_vec<8>(p, dt, 0, v);
+    else
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+            if(i >= lo && i < hi)
+                store_out(p, i, v[i], dt);
+}
+
 // largest magnitude of three values; a NaN among them survives
 __device__ __forceinline__ float amax3(float a, float b, float c)
 {
@@ -328,22 +399,23 @@ __device__ __forceinline__ void emit(const NormParams& prm, unsigned row, unsign
 
 __device__ __forceinline__ size_t param_at(const RowParam& p, unsigned row) { return p.ld == 0 ? 0 : static_cast<size_t>(row / p.rows_per) * p.ld; }
 
-// h of VEC columns from x's (already normed if there is a first norm) and the residual's values
-template <int VEC>
-__device__ __forceinline__ void residual_sum(const NormParams& prm, unsigned col, size_t at_pw, size_t at_pb, size_t at_g, float gate1, float mean, float rstd,
+// h of VEC columns from x's (already normed if there is a first norm) and the residual's values.  get(parameter, at, v): the
+// parameter's values of these columns, its entry beginning at element `at`.
+template <int VEC, typename Get>
+__device__ __forceinline__ void residual_sum(const NormParams& prm, Get&& get, size_t at_pw, size_t at_pb, size_t at_g, float gate1, float mean, float rstd,
                                              bool has_res, const float (&res)[VEC], float (&h)[VEC])
 {
     if(prm.post)
     {
         float w[VEC];
         if(prm.post_weight.ptr != nullptr)
-            ld_param<VEC>(prm.post_weight.ptr, prm.post_weight.dt, at_pw + col, w);
+            get(prm.post_weight, at_pw, w);
 #pragma unroll
         for(int i = 0; i < VEC; ++i)
             h[i] = (h[i] - mean) * rstd * (prm.post_weight.ptr != nullptr ? w[i] : 1.f);
         if(prm.post_bias.ptr != nullptr)
         {
-            ld_param<VEC>(prm.post_bias.ptr, prm.post_bias.dt, at_pb + col, w);
+            get(prm.post_bias, at_pb, w);
 #pragma unroll
             for(int i = 0; i < VEC; ++i)
                 h[i] += w[i];
@@ -360,7 +432,7 @@ __device__ __forceinline__ void residual_sum(const NormParams& prm, unsigned col
         else
         {
             float g[VEC];
-            ld_param<VEC>(prm.gate.ptr, prm.gate.dt, at_g + col, g);
+            get(prm.gate, at_g, g);
 #pragma unroll
             for(int i = 0; i < VEC; ++i)
                 h[i] *= g[i];
@@ -373,8 +445,8 @@ __device__ __forceinline__ void residual_sum(const NormParams& prm, unsigned col
             h[i] = fmaf(prm.res_scale, res[i], h[i]);
     }
 }
-template <int VEC>
-__device__ __forceinline__ void affine(const NormParams& prm, unsigned col, size_t at_w, size_t at_b, float mean, float rstd, float (&y)[VEC])
+template <int VEC, typename Get>
+__device__ __forceinline__ void affine(const NormParams& prm, Get&& get, size_t at_w, size_t at_b, float mean, float rstd, float (&y)[VEC])
 {
 #pragma unroll
     for(int i = 0; i < VEC; ++i)
@@ -382,25 +454,27 @@ __device__ __forceinline__ void affine(const NormParams& prm, unsigned col, size
     float p[VEC];
     if(prm.weight.ptr != nullptr)
     {
-        ld_param<VEC>(prm.weight.ptr, prm.weight.dt, at_w + col, p);
+        get(prm.weight, at_w, p);
 #pragma unroll
         for(int i = 0; i < VEC; ++i)
             y[i] *= prm.weight_offset + p[i];
     }
     if(prm.bias.ptr != nullptr)
     {
-        ld_param<VEC>(prm.bias.ptr, prm.bias.dt, at_b + col, p);
+        get(prm.bias, at_b, p);
 #pragma unroll
         for(int i = 0; i < VEC; ++i)
             y[i] += p[i];
     }
 }
 
-// The row stays in registers: every thread holds CNT vectors of VEC elements, vector j at element (j * threads + t) * VEC.
-// blockDim = (threads of a row, rows); more than one row per CTA only with one warp a row.  Bound by HBM for many rows
-// (x, residual in, h, y out), by the chain load - sum - load - store for one.
-template <int VEC, int CNT, bool X32, bool R32>
-__global__ void __launch_bounds__(VEC * CNT == 8 ? 1024 : 512) norm_rows_kernel(const __grid_constant__ NormParams prm)
+// The row stays in registers: every thread holds CNT groups of eight elements, group j * threads + t.  blockDim = (threads of a row,
+// rows); more than one row per CTA only with one warp a row.  Bound by HBM for many rows (x, residual in, h, y out), by the chain load -
+// sum - load - store for one.  SHIFT: rows and parameters start on any element's address; the groups then begin on y's 16-byte
+// boundaries, the first and the last hold only some of the row, and the operands are shifted into place (one element at a time instead:
+// @OLD@).
+template <int CNT, bool X32, bool R32, bool SHIFT>
+__global__ void __launch_bounds__(CNT == 1 ? 1024 : 512) norm_rows_kernel(const __grid_constant__ NormParams prm)
 {
     __shared__ float red[4][32];
     const unsigned t = threadIdx.x, T = blockDim.x;
@@ -409,30 +483,57 @@ __global__ void __launch_bounds__(VEC * CNT == 8 ? 1024 : 512) norm_rows_kernel(
     grid_launch_dependents();
     if(row >= prm.M)
         return; // (whole warps: several rows per CTA only with a warp a row)
-    const unsigned n = prm.n;
-    Raw<VEC, X32> rx[CNT];
-    Raw<VEC, R32> rr[CNT];
+    const int n = static_cast<int>(prm.n);
+    const long long x_at = static_cast<long long>(row) * prm.x.ld, r_at = static_cast<long long>(row) * prm.res.ld;
+    const long long h_at = static_cast<long long>(row) * prm.h.ld, y_at = static_cast<long long>(row) * prm.y.ld;
+    // elements in front of the row in its first group
+    const int before = SHIFT ? static_cast<int>((reinterpret_cast<uintptr_t>(prm.y.ptr) / (prm.y.dt == OUT_F32 ? 4 : 2) + y_at) & 7) : 0;
+    auto first = [&](int j) { return static_cast<int>(j * T + t) * 8 - before; };        // column of a group's first element
+    auto lo    = [&](int j) { return SHIFT ? max(0, -first(j)) : 0; };                   // the elements of the group that are the row's
+    auto hi    = [&](int j) { return SHIFT ? min(8, n - first(j)) : 8; };
+    auto some  = [&](int j) { return first(j) < n; };
+    auto inside = [&](int j, int i) { return !SHIFT || (i >= lo(j) && i < hi(j)); };
+    Raw<8, X32> rx[CNT];
+    Raw<8, R32> rr[CNT];
     const bool has_res = prm.res.ptr != nullptr;
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
-        const unsigned col = (j * T + t) * VEC;
-        if(col < n)
+        if(some(j))
         {
-            ld_raw<VEC, X32>(rx[j], prm.x.ptr, static_cast<size_t>(row) * prm.x.ld + col);
-            if(has_res)
-                ld_raw<VEC, R32>(rr[j], prm.res.ptr, static_cast<size_t>(row) * prm.res.ld + col);
+            if(SHIFT)
+            {
+                ld_shifted<X32>(rx[j], static_cast<const uint8_t*>(prm.x.ptr) + (x_at + first(j)) * (X32 ? 4 : 2), lo(j), hi(j));
+                if(has_res)
+                    ld_shifted<R32>(rr[j], static_cast<const uint8_t*>(prm.res.ptr) + (r_at + first(j)) * (R32 ? 4 : 2), lo(j), hi(j));
+            }
+            else
+            {
+                ld_raw<8, X32>(rx[j], prm.x.ptr, x_at + first(j));
+                if(has_res)
+                    ld_raw<8, R32>(rr[j], prm.res.ptr, r_at + first(j));
+            }
         }
     }
-    float h[CNT][VEC];
+    float h[CNT][8];
+    // values outside the row count for nothing in the sums
+    auto clear_outside = [&](int j) {
+        if(SHIFT && hi(j) - lo(j) != 8)
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                h[j][i] = inside(j, i) ? h[j][i] : 0.f;
+    };
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
-        if((j * T + t) * VEC < n)
-            unpack<VEC, X32>(rx[j], prm.x.dt, h[j]);
+        if(some(j))
+        {
+            unpack<8, X32>(rx[j], prm.x.dt, h[j]);
+            clear_outside(j);
+        }
         else
 #pragma unroll
-            for(int i = 0; i < VEC; ++i)
+            for(int i = 0; i < 8; ++i)
                 h[j][i] = 0.f;
     }
     auto stats = [&](int slot, float& mean, float& rstd) {
@@ -443,20 +544,23 @@ __global__ void __launch_bounds__(VEC * CNT == 8 ? 1024 : 512) norm_rows_kernel(
 #pragma unroll
             for(int j = 0; j < CNT; ++j)
 #pragma unroll
-                for(int i = 0; i < VEC; ++i)
+                for(int i = 0; i < 8; ++i)
                     s += h[j][i];
             mean = row_sum(s, red, slot) * prm.inv_n;
         }
         float s = 0.f;
 #pragma unroll
         for(int j = 0; j < CNT; ++j)
-            if((j * T + t) * VEC < n)
+            if(some(j))
+            {
+                const bool whole = !SHIFT || hi(j) - lo(j) == 8;
 #pragma unroll
-                for(int i = 0; i < VEC; ++i)
+                for(int i = 0; i < 8; ++i)
                 {
-                    const float d = h[j][i] - mean;
+                    const float d = whole || inside(j, i) ? h[j][i] - mean : 0.f;
                     s             = fmaf(d, d, s);
                 }
+            }
         rstd = rsqrtf(row_sum(s, red, slot + 1) * prm.inv_n + prm.eps);
     };
     float mean = 0.f, rstd = 1.f;
@@ -470,18 +574,31 @@ __global__ void __launch_bounds__(VEC * CNT == 8 ? 1024 : 512) norm_rows_kernel(
         ld_param<1>(prm.gate.ptr, prm.gate.dt, at_g, g);
         gate1 = g[0];
     }
+    auto getter = [&](int j) {
+        return [&, j](const RowParam& q, size_t at, float (&v)[8]) {
+            if(SHIFT)
+                ld_param_shifted(q.ptr, q.dt, static_cast<long long>(at) + first(j), lo(j), hi(j), v);
+            else
+                ld_param<8>(q.ptr, q.dt, at + first(j), v);
+        };
+    };
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
-        const unsigned col = (j * T + t) * VEC;
-        if(col < n)
+        if(some(j))
         {
-            float r[VEC];
+            float r[8];
             if(has_res)
-                unpack<VEC, R32>(rr[j], prm.res.dt, r);
-            residual_sum<VEC>(prm, col, at_pw, at_pb, at_g, gate1, mean, rstd, has_res, r, h[j]);
+                unpack<8, R32>(rr[j], prm.res.dt, r);
+            residual_sum<8>(prm, getter(j), at_pw, at_pb, at_g, gate1, mean, rstd, has_res, r, h[j]);
+            clear_outside(j);
             if(prm.h.ptr != nullptr)
-                st_vec<VEC>(prm.h.ptr, prm.h.dt, static_cast<size_t>(row) * prm.h.ld + col, h[j]);
+            {
+                if(SHIFT)
+                    st_shifted(prm.h.ptr, prm.h.dt, h_at + first(j), lo(j), hi(j), h[j]);
+                else
+                    st_vec<8>(prm.h.ptr, prm.h.dt, h_at + first(j), h[j]);
+            }
         }
     }
     stats(2, mean, rstd);
@@ -489,14 +606,18 @@ __global__ void __launch_bounds__(VEC * CNT == 8 ? 1024 : 512) norm_rows_kernel(
 #pragma unroll
     for(int j = 0; j < CNT; ++j)
     {
-        const unsigned col = (j * T + t) * VEC;
-        const bool in      = col < n;
-        if(in)
-            affine<VEC>(prm, col, at_w, at_b, mean, rstd, h[j]);
-        emit<VEC>(prm, row, col, in, h[j]);
+        if(some(j))
+            affine<8>(prm, getter(j), at_w, at_b, mean, rstd, h[j]);
+        if(SHIFT)
+        {
+            if(some(j))
+                st_shifted(prm.y.ptr, prm.y.dt, y_at + first(j), lo(j), hi(j), h[j]);
+        }
+        else
+            emit<8>(prm, row, first(j), some(j), h[j]);
     }
-    if(prm.y.dt >= OUT_E2M1)
-        fill_scale_padding(prm.sf, row, prm.M, n >> 5, t, T);
+    if(!SHIFT && prm.y.dt >= OUT_E2M1)
+        fill_scale_padding(prm.sf, row, prm.M, prm.n >> 5, t, T);
 }
 
 // Rows that do not fit the registers: a CTA goes over its row once per sum and once for the outputs, recomputing h each
@@ -552,7 +673,8 @@ __global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ 
                 unpack<VEC, false>(rr, prm.res.dt, r);
             }
         }
-        residual_sum<VEC>(prm, col, at_pw, at_pb, at_g, gate1, pmean, prstd, has_res, r, v);
+        auto get = [&](const RowParam& q, size_t at, float (&v)[VEC]) { ld_param<VEC>(q.ptr, q.dt, at + col, v); };
+        residual_sum<VEC>(prm, get, at_pw, at_pb, at_g, gate1, pmean, prstd, has_res, r, v);
     };
     auto stats = [&](int slot, auto&& load, float& mean, float& rstd) {
         float m = 0.f;
@@ -603,7 +725,8 @@ __global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ 
             load_h(col, v);
             if(prm.h.ptr != nullptr)
                 st_vec<VEC>(prm.h.ptr, prm.h.dt, static_cast<size_t>(row) * prm.h.ld + col, v);
-            affine<VEC>(prm, col, at_w, at_b, mean, rstd, v);
+            auto get = [&](const RowParam& q, size_t at, float (&v)[VEC]) { ld_param<VEC>(q.ptr, q.dt, at + col, v); };
+            affine<VEC>(prm, get, at_w, at_b, mean, rstd, v);
         }
         emit<VEC>(prm, row, col, in, v);
     }
@@ -665,48 +788,6 @@ __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ Ac
                 v[i] *= g[i];
             st_vec<8>(prm.out, prm.out_dt, out_at[u], v);
         }
-    }
-}
-
-// Elements `lo` .. `hi` - 1 of the eight that begin at `p`, on any element's address: the 16-byte pieces that hold one of them, moved
-// into place.  (No other piece is read: a piece with one byte of the tensor lies in its memory.)
-template <bool B32>
-__device__ __forceinline__ void ld_shifted(Raw<8, B32>& r, const uint8_t* p, int lo, int hi)
-{
-    constexpr int E = B32 ? 4 : 8, PIECES = B32 ? 3 : 2;
-    const int s          = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / (16 / E); // element 0's place in its piece
-    const uint8_t* piece = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(p) & ~static_cast<uintptr_t>(15));
-    uint32_t w[4 * PIECES];
-#pragma unroll
-    for(int i = 0; i < PIECES; ++i)
-    {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if(i * E - s < hi && (i + 1) * E - s > lo)
-            v = *reinterpret_cast<const uint4*>(piece + 16 * i); // (through L1: the next thread reads one of the pieces too)
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    }
-    if(B32)
-    {
-        // by two words, by one
-#pragma unroll
-        for(int i = 0; i < 9; ++i)
-            w[i] = (s & 2) ? w[(i + 2) % (4 * PIECES)] : w[i];
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            r.w[i] = (s & 1) ? w[i + 1] : w[i];
-    }
-    else
-    {
-        // by two words, by one, by half a word
-#pragma unroll
-        for(int i = 0; i < 6; ++i)
-            w[i] = (s & 4) ? w[i + 2] : w[i];
-#pragma unroll
-        for(int i = 0; i < 5; ++i)
-            w[i] = (s & 2) ? w[i + 1] : w[i];
-#pragma unroll
-        for(int i = 0; i < 4; ++i)
-            r.w[B32 ? 0 : i] = __funnelshift_r(w[i], w[i + 1], (s & 1) * 16);
     }
 }
 

@@ -99,6 +99,15 @@ CASES = [
     (2, 20001, "fp16", "fp32", {"post": True, "norm": "layer", "post_bias": True}),
     (4, 2051, "bf16", None, {"gate": "channel"}),
     (9, 16383, "bf16", "bf16", {"norm": "layer"}),
+    # rows on any element's address, types that differ
+    (29, 9371, "bf16", "fp32", {"post": True, "gate": "token"}),
+    (6, 3075, "bf16", "fp32", {"affine": "sample3", "bias": True}),
+    (400, 5287, "fp32", "bf16", {"gate": "token", "affine": "sample2", "bias": True, "norm": "layer"}),
+    (600, 1571, "fp32", "fp16", {"norm": "layer", "gate": "channel16", "scale": 1.25, "post": True, "post_bias": True}),
+    (350, 8203, "bf16", "fp16", {"norm": "layer", "post": True}),
+    (2, 16377, "fp32", "bf16", {"gate": "channel"}),
+    (5, 7, "fp16", "bf16", {"norm": "layer", "bias": True}),
+    (3, 8190, "bf16", "bf16", {"post": True, "post_bias": True}),
     # many rows: the streaming kernels, aligned and not, every width class
     (1200, 64, "bf16", "bf16", {"post": True, "gate": "channel16"}),
     (999, 40, "fp16", "fp32", {"norm": "layer", "bias": True, "gate": "token"}),

@@ -350,15 +350,18 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
     }
     // one group a thread where there are few rows (the shortest chain), up to four where the machine is full
     const bool few     = prm.M <= 2u * static_cast<unsigned>(sms);
-    const unsigned cnt = vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1;
+    // (SHIFT holds more registers a group: two at most, so that an SM keeps 32 warps; with four 4096 x 9001 141 us, with two 109)
+    const unsigned cnt = aligned ? (vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1) : vecs > 1024 || (!few && vecs >= 256) ? 2 : 1;
     const unsigned t   = ((vecs + cnt - 1) / cnt + 31) / 32 * 32, r = t == 32 ? 4 : 1; // (a warp a row: four rows a CTA)
     const dim3 grid((prm.M + r - 1) / r), block(t, r);
-    if(cnt == 1)
-        aligned ? launch_norm_rows<1, false>(prm, grid, block, stream) : launch_norm_rows<1, true>(prm, grid, block, stream);
+    if(!aligned)
+        cnt == 1 ? launch_norm_rows<1, true>(prm, grid, block, stream) : launch_norm_rows<2, true>(prm, grid, block, stream);
+    else if(cnt == 1)
+        launch_norm_rows<1, false>(prm, grid, block, stream);
     else if(cnt == 2)
-        aligned ? launch_norm_rows<2, false>(prm, grid, block, stream) : launch_norm_rows<2, true>(prm, grid, block, stream);
+        launch_norm_rows<2, false>(prm, grid, block, stream);
     else
-        aligned ? launch_norm_rows<4, false>(prm, grid, block, stream) : launch_norm_rows<4, true>(prm, grid, block, stream);
+        launch_norm_rows<4, false>(prm, grid, block, stream);
 }
 
 template <bool X32, int ACT>

@@ -267,7 +267,9 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
 {
     const unsigned n = prm.n;
     const int xd = prm.x.dt, rd = prm.res.ptr != nullptr ? prm.res.dt : (prm.h.ptr != nullptr ? prm.h.dt : xd);
-    if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && n < 64) || (prm.h.ptr != nullptr && prm.h.dt != rd))
+    // (rows on any address: up to about four million elements the general kernel's shifted groups are ahead - 1000 x 1155 6.3 us against
+    // 10, 400 x 3001 8.4 and 13.5, 8200 x 1155 40 and 38, 8192 x 4097 76 and 50 -, and so they are for short rows, 16384 x 203 17 and 22)
+    if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && (n < 256 || static_cast<unsigned long long>(prm.M) * n < (4u << 20))) || (prm.h.ptr != nullptr && prm.h.dt != rd))
         return false;
     // one type for all parameters
     int pd          = -1;
@@ -352,7 +354,10 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
     const bool few     = prm.M <= 2u * static_cast<unsigned>(sms);
     // (SHIFT holds more registers a group: two at most, so that an SM keeps 32 warps; with four 4096 x 9001 141 us, with two 109)
     const unsigned cnt = aligned ? (vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1) : vecs > 1024 || (!few && vecs >= 256) ? 2 : 1;
-    const unsigned t   = ((vecs + cnt - 1) / cnt + 31) / 32 * 32, r = t == 32 ? 4 : 1; // (a warp a row: four rows a CTA)
+    unsigned t         = ((vecs + cnt - 1) / cnt + 31) / 32 * 32;
+    if(!aligned && vecs <= 16)
+        t = vecs <= 8 ? 8 : 16;
+    const unsigned r = t <= 32 ? 128 / t : 1; // (short rows: as many as make four warps a CTA)
     const dim3 grid((prm.M + r - 1) / r), block(t, r);
     if(!aligned)
         cnt == 1 ? launch_norm_rows<1, true>(prm, grid, block, stream) : launch_norm_rows<2, true>(prm, grid, block, stream);

@@ -365,19 +365,20 @@ __device__ __forceinline__ void fill_scale_padding(const BlockScales& sf, unsign
                 sf.ptr[sf_offset(sf, r, kb)] = fill;
 }
 
-__device__ __forceinline__ float warp_sum(float v)
+__device__ __forceinline__ float warp_sum(float v, unsigned lanes = 32)
 {
 #pragma unroll
-    for(int d = 16; d > 0; d >>= 1)
-        v += __shfl_xor_sync(0xffffffffu, v, d);
+    for(unsigned d = 16; d > 0; d >>= 1)
+        if(d < lanes)
+            v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-// Sum over the threads of a row: one warp, or the whole CTA (`slot`: consecutive sums use different slots, so that one
+// Sum over the threads of a row: 8, 16 or 32 lanes, or the whole CTA (`slot`: consecutive sums use different slots, so that one
 // barrier a sum is enough).  The order of the additions is fixed.
 __device__ __forceinline__ float row_sum(float v, float (*red)[32], int slot)
 {
-    v = warp_sum(v);
-    if(blockDim.x == 32)
+    v = warp_sum(v, blockDim.x);
+    if(blockDim.x <= 32)
         return v;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if(lane == 0)
@@ -497,7 +498,7 @@ __device__ __forceinline__ void affine(const NormParams& prm, Get&& get, size_t 
 }
 
 // The row stays in registers: every thread holds CNT groups of eight elements, group j * threads + t.  blockDim = (threads of a row,
-// rows); more than one row per CTA only with one warp a row.  Bound by HBM for many rows (x, residual in, h, y out), by the chain load -
+// rows); more than one row per CTA only with at most a warp a row.  Bound by HBM for many rows (x, residual in, h, y out), by the chain load -
 // sum - load - store for one.  SHIFT: rows and parameters start on any element's address; the groups then begin on y's 16-byte
 // boundaries, the first and the last hold only some of the row, and the operands are shifted into place (one element at a time instead:
 // 6 x 3075 30 us against 3.8, 1142 x 5287 fp32 with a bf16 residual 146 against 25, 4096 x 9001 952 against 109).
@@ -506,11 +507,12 @@ __global__ void __launch_bounds__(CNT == 1 || SHIFT ? 1024 : 512) norm_rows_kern
 {
     __shared__ float red[4][32];
     const unsigned t = threadIdx.x, T = blockDim.x;
-    const unsigned row = blockIdx.x * blockDim.y + threadIdx.y;
+    const unsigned mine = blockIdx.x * blockDim.y + threadIdx.y, row = min(mine, prm.M - 1);
+    const bool live     = mine < prm.M;
     grid_dependency_wait();
     grid_launch_dependents();
-    if(row >= prm.M)
-        return; // (whole warps: several rows per CTA only with a warp a row)
+    if(!live && T >= 32)
+        return; // (whole warps; where rows share a warp, all of its lanes take part in the sums)
     const int n = static_cast<int>(prm.n);
     const long long x_at = static_cast<long long>(row) * prm.x.ld, r_at = static_cast<long long>(row) * prm.res.ld;
     const long long h_at = static_cast<long long>(row) * prm.h.ld, y_at = static_cast<long long>(row) * prm.y.ld;
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(CNT == 1 || SHIFT ? 1024 : 512) norm_rows_kern
     auto first = [&](int j) { return static_cast<int>(j * T + t) * 8 - before; };        // column of a group's first element
     auto lo    = [&](int j) { return SHIFT ? max(0, -first(j)) : 0; };                   // the elements of the group that are the row's
     auto hi    = [&](int j) { return SHIFT ? min(8, n - first(j)) : 8; };
-    auto some  = [&](int j) { return first(j) < n; };
+    auto some  = [&](int j) { return live && first(j) < n; };
     auto inside = [&](int j, int i) { return !SHIFT || (i >= lo(j) && i < hi(j)); };
     Raw<8, X32> rx[CNT];
     Raw<8, R32> rr[CNT];

@@ -17,7 +17,7 @@ import struct
 import torch
 
 from .dtypes import _torch_to_aiter_dtype as _DTYPE_IDS
-from .dtypes import aiter_dtype_id
+from .dtypes import aiter_dtype_id, fp4x2, fp8, fp8_e8m0
 
 # AITER_B200_LIBRARY points at another build of the library (comparing two builds on one machine)
 LIB_PATH = os.environ.get("AITER_B200_LIBRARY") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "libaiter_b200.so")
@@ -214,7 +214,7 @@ def _load_host():
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_aiter_b200_host", loader))
     loader.exec_module(module)
     names = ("gated_residual_norm", "act_and_mul", "gemm_a16w16_fused", "gemm_a8w8_mxfp8_fused", "gemm_a4w4_fused", "gemm_a4w4_fused_workspace")
-    module.bind(*(ctypes.cast(getattr(_lib, f"aiter_b200_{n}"), ctypes.c_void_p).value for n in names), dict(_DTYPE_IDS), aiter_dtype_id)
+    module.bind(*(ctypes.cast(getattr(_lib, f"aiter_b200_{n}"), ctypes.c_void_p).value for n in names), dict(_DTYPE_IDS), aiter_dtype_id, fp4x2, fp8, fp8_e8m0)
     return module
 
 

@@ -4,7 +4,7 @@ instead of 16-bit values.  The reference's closest forms: aiter/ops/rmsnorm.py, 
 from __future__ import annotations
 
 import torch
-from torch import Tensor, empty
+from torch import Tensor
 
 from . import dtypes
 from ._ffi import call_host, current_stream, host
@@ -20,22 +20,16 @@ def activation_id(activation: str | None, fn: str) -> int:
         raise ValueError(f"{fn}: unknown activation {activation!r}, expected one of {', '.join(ACTIVATIONS)}") from None
 
 
-def _mx_out(fn: str, m: int, n: int, quant_dtype, shuffle, device):
-    """Data and scale tensors of an MX output, shaped as per_1x32_mx_quant_hip shapes them."""
+def _mx_bits(fn: str, n: int, quant_dtype, otype) -> int:
+    if otype is not None:
+        raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
     if n % 32 != 0:
         raise ValueError(f"{fn}: an MX output needs a multiple of 32 columns, got {n}")
     if quant_dtype == dtypes.fp4x2:
-        y = empty(m, n // 2, dtype=dtypes.fp4x2, device=device)
-    elif quant_dtype == dtypes.fp8:
-        y = empty(m, n, dtype=dtypes.fp8, device=device)
-    else:
-        raise ValueError(f"{fn}: unsupported quant_dtype {quant_dtype}, expected one of (dtypes.fp4x2, dtypes.fp8)")
-    kb = n // 32
-    if shuffle == 2:
-        m = (m + 31) // 32 * 32
-    elif shuffle:
-        m, kb = (m + 255) // 256 * 256, (kb + 7) // 8 * 8
-    return y, empty(m, kb, dtype=dtypes.fp8_e8m0, device=device)
+        return 4
+    if quant_dtype == dtypes.fp8:
+        return 8
+    raise ValueError(f"{fn}: unsupported quant_dtype {quant_dtype}, expected one of (dtypes.fp4x2, dtypes.fp8)")
 
 
 def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -70,13 +64,8 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
         if o2.shape != x.shape:
             raise ValueError(f"{fn}: residual_out must have x's shape {tuple(x.shape)}, got {tuple(o2.shape)}")
         o2 = o2 if flat else o2.view(-1, x.shape[-1])
-    y, scale, layout = None, None, 0
-    if quant_dtype is not None:
-        if otype is not None:
-            raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
-        y, scale = _mx_out(fn, *x2.shape, quant_dtype, shuffle, x.device)
-        layout = int(shuffle)
-    y, h = call_host("aiter_b200_gated_residual_norm", host.norm, x2, r2, weight, bias, gate, post_weight, post_bias, o2, y, scale, otype,
+    bits, layout = (0, 0) if quant_dtype is None else (_mx_bits(fn, x2.shape[1], quant_dtype, otype), int(shuffle))
+    y, scale, h = call_host("aiter_b200_gated_residual_norm", host.norm, x2, r2, weight, bias, gate, post_weight, post_bias, o2, bits, otype,
                      residual_scale, weight_offset, eps, _NORMS[norm], post, layout, current_stream(x.get_device()))
     if not flat:
         y = y.view(*x.shape[:-1], y.shape[-1])
@@ -101,13 +90,8 @@ def act_and_mul(x: Tensor, activation: str = "silu", otype: torch.dtype | None =
         raise ValueError(f"{fn}: the last dimension must be even, got {x.shape[-1]}")
     flat = x.dim() == 2
     x2 = x if flat else x.reshape(-1, x.shape[-1])
-    y, scale, layout = None, None, 0
-    if quant_dtype is not None:
-        if otype is not None:
-            raise ValueError(f"{fn}: otype and quant_dtype exclude one another")
-        y, scale = _mx_out(fn, x2.shape[0], x2.shape[1] // 2, quant_dtype, shuffle, x.device)
-        layout = int(shuffle)
-    y = call_host("aiter_b200_act_and_mul", host.act, x2, y, scale, otype, act, layout, current_stream(x.get_device()))
+    bits, layout = (0, 0) if quant_dtype is None else (_mx_bits(fn, x2.shape[1] // 2, quant_dtype, otype), int(shuffle))
+    y, scale = call_host("aiter_b200_act_and_mul", host.act, x2, None, bits, otype, act, layout, current_stream(x.get_device()))
     if not flat:
         y = y.view(*x.shape[:-1], y.shape[-1])
     return y if scale is None else (y, scale)
@@ -129,4 +113,4 @@ def gelu_tanh_and_mul(out: Tensor, input: Tensor) -> None:
 def _act_and_mul_into(out: Tensor, input: Tensor, activation: str) -> None:
     x2 = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
     o2 = out if out.dim() == 2 else out.view(-1, out.shape[-1])
-    call_host("aiter_b200_act_and_mul", host.act, x2, o2, None, None, ACTIVATIONS[activation], 0, current_stream(input.get_device()))
+    call_host("aiter_b200_act_and_mul", host.act, x2, o2, 0, None, ACTIVATIONS[activation], 0, current_stream(input.get_device()))

@@ -33,6 +33,7 @@ struct Bound
     Gemm4Fn gemm4;
     WorkspaceFn workspace;
     int dtypes[64]; // library's id of an ATen scalar type, -1: none
+    at::ScalarType fp4x2, fp8, e8m0; // of MX operands and their scales
 } bound = {};
 PyObject* unsupported = nullptr; // raises, naming the type
 
@@ -68,7 +69,11 @@ struct Arg
         d.device_id = t.is_cuda() ? static_cast<int>(t.get_device()) : -1;
         ptr         = &d;
     }
-    explicit Arg(const at::Tensor& t) { set(t); }
+    explicit Arg(const at::Tensor& t)
+    {
+        if(t.defined())
+            set(t);
+    }
     explicit Arg(PyObject* o)
     {
         if(o == Py_None)
@@ -94,6 +99,18 @@ at::Tensor rows_like(const at::Tensor& t, int64_t m, int64_t n, PyObject* dtype)
     }
     return at::empty({m, n}, options);
 }
+// Data and scale tensors of an MX output [m, n], shaped as per_1x32_mx_quant_hip shapes them for the layout
+void mx_out(const at::Tensor& x, int64_t m, int64_t n, long bits, long layout, at::Tensor& y, at::Tensor& scale)
+{
+    int64_t rows = m, blocks = n / 32;
+    if(layout == 1)
+        rows = (m + 255) / 256 * 256, blocks = (blocks + 7) / 8 * 8;
+    else if(layout == 2)
+        rows = (m + 31) / 32 * 32;
+    y     = at::empty({m, bits == 4 ? n / 2 : n}, x.options().dtype(bits == 4 ? bound.fp4x2 : bound.fp8));
+    scale = at::empty({rows, blocks}, x.options().dtype(bound.e8m0));
+}
+PyObject* wrap(at::Tensor& t) { return t.defined() ? THPVariable_Wrap(std::move(t)) : Py_NewRef(Py_None); }
 long integer(PyObject* o)
 {
     const long v = PyLong_AsLong(o);
@@ -121,56 +138,62 @@ void count(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "exp
 
 // Every function below returns its tensors, or None when the library refused the call (its message is read by the caller).
 
-// norm(x, residual, weight, bias, gate, post_weight, post_bias, residual_out, y, scale, otype, residual_scale, weight_offset, eps, layer,
-//      post, layout, stream) -> (y, h); y and scale are given for an MX output; h is None where it would be a copy of x
+// norm(x, residual, weight, bias, gate, post_weight, post_bias, residual_out, bits, otype, residual_scale, weight_offset, eps, layer,
+//      post, layout, stream) -> (y, scale, h); bits: 0, or 4 or 8 for an MX output; scale is None without it, h where it would be a copy of x
 PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    count(n, 18);
+    count(n, 17);
     const at::Tensor& x = tensor(a[0]);
     TORCH_CHECK(x.dim() == 2, "gated_residual_norm: x must have two dimensions");
-    const bool post = integer(a[15]) != 0;
-    at::Tensor h, y;
+    const long bits = integer(a[8]), layout = integer(a[15]);
+    const bool post = integer(a[14]) != 0;
+    at::Tensor h, y, sf;
     if(a[7] != Py_None)
         h = tensor(a[7]);
     else if(a[1] != Py_None || a[4] != Py_None || post)
         h = rows_like(a[1] != Py_None ? tensor(a[1]) : x, x.size(0), x.size(1), Py_None);
-    y = a[8] != Py_None ? tensor(a[8]) : rows_like(x, x.size(0), x.size(1), a[10]);
-    Arg dx(x), dr(a[1]), dw(a[2]), db(a[3]), dg(a[4]), dpw(a[5]), dpb(a[6]), ds(a[9]), dy(y), dh(Py_None);
-    if(h.defined())
-        dh.set(h);
-    const float scale = number(a[11]), offset = number(a[12]), eps = number(a[13]);
-    const int layer = static_cast<int>(integer(a[14])), layout = static_cast<int>(integer(a[16]));
-    void* const stream = address(a[17]);
+    if(bits != 0)
+        mx_out(x, x.size(0), x.size(1), bits, layout, y, sf);
+    else
+        y = rows_like(x, x.size(0), x.size(1), a[9]);
+    Arg dx(x), dr(a[1]), dw(a[2]), db(a[3]), dg(a[4]), dpw(a[5]), dpb(a[6]), dy(y), ds(sf), dh(h);
+    const float scale = number(a[10]), offset = number(a[11]), eps = number(a[12]);
+    const int layer    = static_cast<int>(integer(a[13]));
+    void* const stream = address(a[16]);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = bound.norm(dy.ptr, ds.ptr, dh.ptr, dx.ptr, dr.ptr, dw.ptr, db.ptr, dg.ptr, dpw.ptr, dpb.ptr, scale, offset, eps, layer, post, layout, stream);
+    rc = bound.norm(dy.ptr, ds.ptr, dh.ptr, dx.ptr, dr.ptr, dw.ptr, db.ptr, dg.ptr, dpw.ptr, dpb.ptr, scale, offset, eps, layer, post, static_cast<int>(layout), stream);
     Py_END_ALLOW_THREADS
     if(rc != 0)
         Py_RETURN_NONE;
-    PyObject* hy = h.defined() ? THPVariable_Wrap(std::move(h)) : Py_NewRef(Py_None);
-    return Py_BuildValue("NN", THPVariable_Wrap(std::move(y)), hy);
+    return Py_BuildValue("NNN", wrap(y), wrap(sf), wrap(h));
     END_HANDLE_TH_ERRORS
 }
 
-// act(x, y, scale, otype, activation, layout, stream) -> y; y is given for an MX output and for the out-forms
+// act(x, y, bits, otype, activation, layout, stream) -> (y, scale); y is given for the out-forms
 PyObject* act(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     count(n, 7);
     const at::Tensor& x = tensor(a[0]);
     TORCH_CHECK(x.dim() == 2, "act_and_mul: x must have two dimensions");
-    at::Tensor y = a[1] != Py_None ? tensor(a[1]) : rows_like(x, x.size(0), x.size(1) / 2, a[3]);
-    Arg dx(x), dy(y), ds(a[2]);
-    const int activation = static_cast<int>(integer(a[4])), layout = static_cast<int>(integer(a[5]));
+    const long bits = integer(a[2]), layout = integer(a[5]);
+    at::Tensor y, sf;
+    if(bits != 0)
+        mx_out(x, x.size(0), x.size(1) / 2, bits, layout, y, sf);
+    else
+        y = a[1] != Py_None ? tensor(a[1]) : rows_like(x, x.size(0), x.size(1) / 2, a[3]);
+    Arg dx(x), dy(y), ds(sf);
+    const int activation = static_cast<int>(integer(a[4]));
     void* const stream = address(a[6]);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = bound.act(dy.ptr, ds.ptr, dx.ptr, activation, layout, stream);
+    rc = bound.act(dy.ptr, ds.ptr, dx.ptr, activation, static_cast<int>(layout), stream);
     Py_END_ALLOW_THREADS
     if(rc != 0)
         Py_RETURN_NONE;
-    return THPVariable_Wrap(std::move(y));
+    return Py_BuildValue("NN", wrap(y), wrap(sf));
     END_HANDLE_TH_ERRORS
 }
 
@@ -214,11 +237,12 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
-// bind(norm, act, gemm16, gemm8, gemm4, workspace: addresses in the library, dtypes: {torch.dtype: id}, unsupported: callable)
+// bind(norm, act, gemm16, gemm8, gemm4, workspace: addresses in the library, dtypes: {torch.dtype: id}, unsupported: callable, fp4x2, fp8,
+//      e8m0: torch.dtype)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    count(n, 8);
+    count(n, 11);
     bound.norm      = reinterpret_cast<NormFn>(address(a[0]));
     bound.act       = reinterpret_cast<ActFn>(address(a[1]));
     bound.gemm16    = reinterpret_cast<Gemm16Fn>(address(a[2]));
@@ -238,6 +262,11 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
             bound.dtypes[type] = static_cast<int>(integer(value));
     }
     Py_XSETREF(unsupported, Py_NewRef(a[7]));
+    for(int i = 8; i < 11; ++i)
+    {
+        TORCH_CHECK_TYPE(THPDtype_Check(a[i]), "expected a torch.dtype");
+        (i == 8 ? bound.fp4x2 : i == 9 ? bound.fp8 : bound.e8m0) = reinterpret_cast<THPDtype*>(a[i])->scalar_type;
+    }
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }

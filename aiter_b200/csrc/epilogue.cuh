@@ -280,6 +280,38 @@ __device__ __forceinline__ void store16(T* dst, const float (&v)[16], uint32_t s
     }
 }
 
+// v += sixteen raw values of one type
+__device__ __forceinline__ void add_raw16(float (&v)[16], const uint32_t (&raw)[16], int mode)
+{
+    if(mode == OUT_BF16)
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            v[j] += __uint_as_float(raw[j] << 16);
+    }
+    else if(mode == OUT_F16)
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            v[j] += raw_to_f32(raw[j], OUT_F16);
+    }
+    else
+    {
+#pragma unroll
+        for(int j = 0; j < 16; ++j)
+            v[j] += __uint_as_float(raw[j]);
+    }
+}
+__device__ __forceinline__ void store_rows16(void* out, int mode, size_t at, const float (&v)[16], uint32_t step, int valid)
+{
+    if(mode == OUT_F32)
+        store16(static_cast<float*>(out) + at, v, step, valid, [](float x) { return x; });
+    else if(mode == OUT_BF16)
+        store16(static_cast<uint16_t*>(out) + at, v, step, valid, [](float x) { return cvt_out16(x, false); });
+    else
+        store16(static_cast<uint16_t*>(out) + at, v, step, valid, [](float x) { return cvt_out16(x, true); });
+}
+
 template <typename Params>
 __device__ __forceinline__ void fused_plain_load(FusedPlain& f, const FusedParams& epi, const Params& prm, int p, int q_first)
 {
@@ -388,35 +420,13 @@ __device__ __forceinline__ bool fused_plain_tile(FusedPlain& f, const FusedParam
         activate<EPI>(v, epi.act);
         if(epi.res != nullptr)
         {
-            if(epi.res_mode == OUT_BF16)
-            {
-#pragma unroll
-                for(int j = 0; j < 16; ++j)
-                    v[j] += __uint_as_float(f.raw[j] << 16);
-            }
-            else if(epi.res_mode == OUT_F16)
-            {
-#pragma unroll
-                for(int j = 0; j < 16; ++j)
-                    v[j] += raw_to_f32(f.raw[j], OUT_F16);
-            }
-            else
-            {
-#pragma unroll
-                for(int j = 0; j < 16; ++j)
-                    v[j] += __uint_as_float(f.raw[j]);
-            }
+            add_raw16(v, f.raw, epi.res_mode);
             if(c + 2 < groups)
                 fused_plain_load(f, epi, prm, p, q_first + 32);
         }
         const size_t at         = transposed ? static_cast<size_t>(q_first) * prm.ldo + p : static_cast<size_t>(p) * prm.ldo + q_first;
         const uint32_t out_step = transposed ? epi.out_step : 1u;
-        if(epi.out_mode == OUT_F32)
-            store16(static_cast<float*>(prm.out) + at, v, out_step, valid, [](float x) { return x; });
-        else if(epi.out_mode == OUT_BF16)
-            store16(static_cast<uint16_t*>(prm.out) + at, v, out_step, valid, [](float x) { return cvt_out16(x, false); });
-        else
-            store16(static_cast<uint16_t*>(prm.out) + at, v, out_step, valid, [](float x) { return cvt_out16(x, true); });
+        store_rows16(prm.out, epi.out_mode, at, v, out_step, valid);
     }
     return true;
 }

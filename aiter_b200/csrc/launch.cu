@@ -938,18 +938,8 @@ static bool try_launch_decode(const GemmProblem& prob, const KernelConfig& cfg, 
         cols <<= 1;
     prm.tmem_cols = cols;
     CUtensorMap mo = mp;
-    const bool out32 = (prob.out_mode == OUT_F32); // (fused epilogue only)
-    prm.tma_store  = ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % (out32 ? 4 : 8) == 0) ? 1 : 0;
-    if(prm.tma_store && prob.fused)
-    {
-        // 16 rows of a warp's 32 columns per store
-        const int esize             = out32 ? 4 : 2;
-        const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * esize, static_cast<cuuint64_t>(prob.M)};
-        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(prob.ldo) * esize};
-        const cuuint32_t box[2]     = {static_cast<cuuint32_t>(32 * esize), 16u};
-        mo = encode_map(prob.out, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE, "output");
-    }
-    else if(prm.tma_store)
+    prm.tma_store  = !prob.fused && ((reinterpret_cast<uintptr_t>(prob.out) & 15) == 0) && (prob.ldo % 8 == 0) ? 1 : 0;
+    if(prm.tma_store)
     {
         // bf16 [M][N] seen as bytes; a warp's box is its 32 output columns by the tile's bn rows
         const cuuint64_t dims[2]    = {static_cast<cuuint64_t>(prob.N) * 2, static_cast<cuuint64_t>(prob.M)};

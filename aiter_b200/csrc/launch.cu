@@ -1050,6 +1050,25 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
     if(cfg.swap >= 0 || cfg.bn > 0 || cfg.cg > 0)
         return;
     const long long M = prob.M, N = prob.N;
+    // Tiles of 32 rows with the weights on the 128-row slot where they leave room for a K split over clusters: what a call with few
+    // tiles takes is its epilogue, which goes over a tile's rows 16 at a time, and one slice's K loop (us, tiles of 32 / what the
+    // rules below take, bf16, MXFP8, MXFP4: 76 x 464 x 512 6.4 / 8.8, 6.3 / 8.7, 6.0 / 8.0; 128 x 2048 x 2048 10.2 / 11.7, 9.9 / 11.1,
+    // 9.4 / 9.7; 128 x 1024 x 8192 15.4 / 20.3, 13.2 / 15.6, 12.0 / 13.0; not without that room: 76 x 4096 x 4096 22.2 / 18.5).
+    if(M > 32 && M <= 600 && cfg.log2_splitk < 0)
+    {
+        const long long tiles = ((M + 31) / 32) * ((N + kTileP - 1) / kTileP);
+        const int room        = tiles * 4 <= num_sms ? 2 : tiles * 2 <= num_sms ? 1 : tiles <= num_sms ? 0 : -1;
+        const bool bf16       = prob.kind == PK_BF16;
+        if(room == 2 || (room == 1 && prob.K <= 4096) || (room == 0 && bf16 && prob.K <= 2048))
+        {
+            cfg.swap = 1;
+            cfg.cg   = 1;
+            cfg.bn   = 32;
+            for(cfg.log2_splitk = room; cfg.log2_splitk > 0 && (prob.K >> cfg.log2_splitk) < (bf16 ? 256 : 512);)
+                --cfg.log2_splitk;
+            return;
+        }
+    }
     if(M <= 64)
         return;
     if(prob.kind == PK_BF16)

@@ -72,7 +72,7 @@ struct FusedArgs
     const aiter_tensor_t* workspace = nullptr; // dense bytes
 };
 
-static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_tensor_t* out, const FusedArgs& f, const char* fn)
+static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_tensor_t* B, const aiter_tensor_t* out, const FusedArgs& f, const char* fn)
 {
     const long long M = p.M, N = p.N;
     require_tensor(out, fn, "out", 2);
@@ -89,6 +89,14 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
     p.ldo        = M == 1 ? (N + 7) / 8 * 8 : out->strides[0]; // (one row: any pitch, and one that allows a tensor map)
     p.fused      = true;
     p.activation = f.activation;
+    // the operands are read until the last tile has been written
+    for(const aiter_tensor_t* t : {first, B})
+    {
+        const int size = t->dtype_ == AITER_DTYPE_bf16 || t->dtype_ == AITER_DTYPE_fp16 ? 2 : 1;
+        B200_CHECK(M == 0 || !overlap(Span{reinterpret_cast<uintptr_t>(t->ptr), t->strides[0] * size, t->shape[1] * size, t->shape[0]},
+                                      Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}),
+                   fn, ": out overlaps an operand");
+    }
     if(f.workspace != nullptr)
     {
         require_tensor(f.workspace, fn, "workspace", 1);
@@ -161,7 +169,7 @@ static void run_mxfp4(const char* fn, aiter_tensor_t* A, aiter_tensor_t* B, aite
     p.wgt_sf = scale_operand(B_scale, wire, fn, "B_scale");
     if(fused != nullptr)
     {
-        set_fused(p, A, out, *fused, fn);
+        set_fused(p, A, B, out, *fused, fn);
         for(const aiter_tensor_t* t : {B, A_scale, B_scale})
             require_same_device(A, t, fn, "an operand");
     }
@@ -341,7 +349,7 @@ static void run_mxfp8(const char* fn, int b_is_fp4, aiter_tensor_t* A, aiter_ten
     p.wgt_sf = scale_operand(ScaleB, SFW_G1250, fn, "ScaleB");
     if(fused != nullptr)
     {
-        set_fused(p, A, out, *fused, fn);
+        set_fused(p, A, B, out, *fused, fn);
         for(const aiter_tensor_t* t : {B, ScaleA, ScaleB})
             require_same_device(A, t, fn, "an operand");
     }
@@ -575,7 +583,7 @@ static void run_bf16(const char* fn, const aiter_tensor_t* A, const aiter_tensor
     p.beta   = 1.f;
     if(fused != nullptr)
     {
-        set_fused(p, A, out, *fused, fn);
+        set_fused(p, A, B, out, *fused, fn);
         require_same_device(A, B, fn, "B");
     }
     p.device = A->device_id;

@@ -92,6 +92,7 @@ RowParam row_param(const aiter_tensor_t* t, const char* fn, const char* name, lo
     require_tensor(t, fn, name, t->ndim == 1 ? 1 : 2);
     B200_CHECK(t->ptr != nullptr, fn, ": ", name, " has a null data pointer");
     const int dt       = float_type(t, fn, name);
+    require_rows(t, bytes_of(dt), fn, name);
     const long long w  = t->shape[t->ndim - 1];
     const bool one     = scalar != nullptr && t->ndim == 2 && w == 1 && n != 1;
     B200_CHECK(w == n || one, fn, ": ", name, " must have ", n, " columns (got ", w, ")");
@@ -439,6 +440,17 @@ extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_
             B200_CHECK(same_rows(prm.h, prm.x) || !overlap(sx, sh), fn, ": residual_out overlaps x");
             B200_CHECK(residual == nullptr || same_rows(prm.h, prm.res) || !overlap(span(prm.res, M, n), sh), fn, ": residual_out overlaps residual");
         }
+        // every row reads the parameters, and the scales are written beside the rows
+        for(const aiter_tensor_t* t : {weight, bias, gate, post_weight, post_bias, scales})
+        {
+            if(t == nullptr)
+                continue;
+            const int size = t == scales ? 1 : t->dtype_ == AITER_DTYPE_fp32 ? 4 : 2;
+            const bool one = t->ndim == 1;
+            const Span st{reinterpret_cast<uintptr_t>(t->ptr), one ? 0 : t->strides[0] * size, t->shape[t->ndim - 1] * size, one ? 1 : t->shape[0]};
+            B200_CHECK(!overlap(st, sy) && (residual_out == nullptr || !overlap(st, span(prm.h, M, n))), fn, ": an output overlaps a parameter or the scales");
+            B200_CHECK(t != scales || (!overlap(st, sx) && (residual == nullptr || !overlap(st, span(prm.res, M, n)))), fn, ": scales overlap an input");
+        }
         prm.post          = post_norm != 0;
         prm.layer         = norm;
         prm.res_scale     = residual_scale;
@@ -484,6 +496,11 @@ extern "C" int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* scale
         if(M == 0)
             return;
         B200_CHECK((y.dt <= OUT_F32 && same_rows(y, in)) || !overlap(span(in, M, n2), span(y, M, n)), fn, ": out overlaps the input (only the gate half may be overwritten in place)");
+        if(scales != nullptr)
+        {
+            const Span st{reinterpret_cast<uintptr_t>(scales->ptr), scales->strides[0], scales->shape[1], scales->shape[0]};
+            B200_CHECK(!overlap(st, span(in, M, n2)) && !overlap(st, span(y, M, n)), fn, ": scales overlap the input or out");
+        }
         prm.in     = in.ptr;
         prm.in_ld  = in.ld;
         prm.in_dt  = in.dt;

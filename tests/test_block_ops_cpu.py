@@ -89,6 +89,10 @@ def test_norm_refusals(ab):
         ({"residual_out": f((M, N), torch.float16, ptr=BASE + (3 << 20))}, "residual_out overlaps residual"),
         ({"residual_out": f((M, N), strides=(0, 1), ptr=far)}, "rows of residual_out overlap"),
         ({"out": f((M, N), strides=(N - 8, 1))}, "rows of out overlap"),
+        ({"residual": f((M, N), ptr=far + 1)}, "residual does not start on an element's boundary"),
+        ({"residual": f((M, N), strides=(-N, 1), ptr=far)}, "negative stride"),
+        ({"weight": f((N,), torch.float32, ptr=far + 2)}, "weight does not start on an element's boundary"),
+        ({"weight": f((N,), ptr=BASE + 64)}, "overlaps a parameter"),
     ]
     for over, match in cases:
         refuse(ab, name, norm_args(ab, **over), match)
@@ -136,6 +140,10 @@ def test_fused_gemm_refusals(ab):
         (dict(residual=f((M, N), torch.float16, ptr=BASE + (2 << 20))), "out overlaps residual"),
         (dict(residual=f((M, N), ptr=far, device=2)), "lives on device 2"),
         (dict(B=f((N, K + 8), ptr=far)), "disagree on K"),
+        (dict(out=f((M, N), ptr=BASE + 256)), "out overlaps an operand"),
+        (dict(out=f((M, N), ptr=BASE + (1 << 20))), "out overlaps an operand"),
+        (dict(bias=f((N,), ptr=BASE + (2 << 20) + 32)), "out overlaps bias"),
+        (dict(out=f((M, N), torch.float32, ptr=far + 2)), "out does not start on an element's boundary"),
         (dict(B=f((N, K), ptr=far, device=1)), "lives on device 1"),
         (dict(A=f((M, K), torch.float16, ptr=far)), "only bf16 inputs"),
         (dict(A=f((M, K), ptr=far, device=-1)), "must live on a GPU"),

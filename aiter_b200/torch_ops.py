@@ -13,8 +13,11 @@ aiter/ops/gemm_op_a4w4.py:125-144).
     torch.ops.aiter.gemm_a4w4o8(A, B, A_scale, B_scale, apreshuffle, global_A_scale, global_B_scale)   (fp8 [.., N], e8m0 [.., N/128])
     torch.ops.aiter.gemm_nvfp4(A, B, ScaleA, ScaleB, global_A_scale, global_B_scale, a_preshuffle)
     torch.ops.aiter.batched_gemm_bf16(XQ, WQ)
+    torch.ops.aiter.gemm_a16w16_fused(A, B, bias, activation, residual, otype)
+    torch.ops.aiter.gemm_a8w8_mxfp8_fused(A, B, ScaleA, ScaleB, bias, activation, residual, otype, a_preshuffle)
+    torch.ops.aiter.gemm_a4w4_fused(A, B, A_scale, B_scale, bias, activation, residual, otype, bpreshuffle)
 
-The first five and the last two return a new bf16 tensor.  The real implementations call the operators of this package (CUDA only).
+The first five, gemm_nvfp4 and batched_gemm_bf16 return a new bf16 tensor, the fused ones a new one of type otype.  The real implementations call the operators of this package (CUDA only).
 """
 from __future__ import annotations
 
@@ -23,7 +26,7 @@ from typing import Optional
 import torch
 from torch import Tensor
 
-from . import batched_gemm_op_bf16, dtypes, gemm_op_a4w4, gemm_op_a8w4, gemm_op_a8w8, tuned_gemm
+from . import batched_gemm_op_bf16, dtypes, gemm_op_a4w4, gemm_op_a8w4, gemm_op_a8w8, gemm_op_fused, tuned_gemm
 
 _NS = "aiter"
 
@@ -130,3 +133,38 @@ def batched_gemm_bf16(XQ: Tensor, WQ: Tensor) -> Tensor:
 @batched_gemm_bf16.register_fake
 def _(XQ, WQ):
     return XQ.new_empty((XQ.shape[0], XQ.shape[1], WQ.shape[1]), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::gemm_a16w16_fused", mutates_args=(), device_types="cuda")
+def gemm_a16w16_fused(A: Tensor, B: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
+                      residual: Optional[Tensor] = None, otype: Optional[torch.dtype] = None) -> Tensor:
+    return gemm_op_fused.gemm_a16w16_fused(A, B, bias, activation, residual, otype)
+
+
+@gemm_a16w16_fused.register_fake
+def _(A, B, bias=None, activation=None, residual=None, otype=None):
+    return A.new_empty((*A.shape[:-1], B.shape[0]), dtype=otype or A.dtype)
+
+
+@torch.library.custom_op(f"{_NS}::gemm_a8w8_mxfp8_fused", mutates_args=(), device_types="cuda")
+def gemm_a8w8_mxfp8_fused(A: Tensor, B: Tensor, ScaleA: Tensor, ScaleB: Tensor, bias: Optional[Tensor] = None,
+                          activation: Optional[str] = None, residual: Optional[Tensor] = None, otype: torch.dtype = torch.bfloat16,
+                          a_preshuffle: bool = True) -> Tensor:
+    return gemm_op_fused.gemm_a8w8_mxfp8_fused(A, B, ScaleA, ScaleB, bias, activation, residual, otype, a_preshuffle)
+
+
+@gemm_a8w8_mxfp8_fused.register_fake
+def _(A, B, ScaleA, ScaleB, bias=None, activation=None, residual=None, otype=torch.bfloat16, a_preshuffle=True):
+    return A.new_empty((*A.shape[:-1], B.shape[0]), dtype=otype)
+
+
+@torch.library.custom_op(f"{_NS}::gemm_a4w4_fused", mutates_args=(), device_types="cuda")
+def gemm_a4w4_fused(A: Tensor, B: Tensor, A_scale: Tensor, B_scale: Tensor, bias: Optional[Tensor] = None,
+                    activation: Optional[str] = None, residual: Optional[Tensor] = None, otype: torch.dtype = torch.bfloat16,
+                    bpreshuffle: bool = True) -> Tensor:
+    return gemm_op_fused.gemm_a4w4_fused(A, B, A_scale, B_scale, bias, activation, residual, otype, bpreshuffle)
+
+
+@gemm_a4w4_fused.register_fake
+def _(A, B, A_scale, B_scale, bias=None, activation=None, residual=None, otype=torch.bfloat16, bpreshuffle=True):
+    return A.new_empty((*A.shape[:-1], B.shape[0]), dtype=otype)

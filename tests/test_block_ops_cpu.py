@@ -198,3 +198,14 @@ def test_python_refusals(ab):
         ab.act_and_mul(x[:, :63])
     with pytest.raises(RuntimeError, match="must live on a GPU"):
         ab.gated_residual_norm(x, x)
+
+
+def test_fused_gemms_trace_on_the_meta_device(ab):
+    e = lambda *s, t=torch.bfloat16: torch.empty(*s, dtype=t, device="meta")  # noqa: E731
+    o = torch.ops.aiter.gemm_a16w16_fused(e(2, 7, 32), e(48, 32), e(48), "gelu", e(2, 7, 48))
+    assert o.shape == (2, 7, 48) and o.dtype == torch.bfloat16
+    assert torch.ops.aiter.gemm_a16w16_fused(e(7, 32), e(48, 32), otype=torch.float32).dtype == torch.float32
+    q, s = e(64, 128, t=torch.float8_e4m3fn), e(64, 4, t=torch.uint8)
+    assert torch.ops.aiter.gemm_a8w8_mxfp8_fused(q, q, s, s, None, "silu", None, torch.float16).dtype == torch.float16
+    p = e(64, 64, t=torch.uint8)
+    assert torch.ops.aiter.gemm_a4w4_fused(p, p, s, s).shape == (64, 64)

@@ -128,3 +128,58 @@ def test_broadcast_rows(ab):
             got, want = ab.gated_residual_norm(xs, rs, b[0].repeat(2)), ab.gated_residual_norm(xs.contiguous(), rs.contiguous(), b[0].repeat(2))
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert torch.equal(ab.act_and_mul(row.expand(m, 512)), ab.act_and_mul(row.repeat(m, 1)))
+
+
+def test_offsets_beyond_32_bits(ab):
+    """Rows so far apart that an element's offset does not fit 32 bits: every kernel of the norm and of the gated activation."""
+    g = torch.Generator().manual_seed(11)
+    buf = torch.empty(700 * (2**22 + 9), dtype=torch.bfloat16, device="cuda")
+    assert buf.numel() > 2**31
+    for m, n, pitch in ((700, 8192, 2**22 + 8), (700, 7001, 2**22 + 9), (700, 128, 2**22 + 8), (250, 8192, 2**23), (250, 1003, 2**23 + 1)):
+        view = torch.as_strided(buf, (m, n), (pitch, 1))
+        x, r, w = randn(g, m, n), randn(g, m, n), randn(g, n)
+        want_y, want_h, big_y, big_h = ref64(x, r, w)
+        view.copy_(x)
+        y, h = ab.gated_residual_norm(view, r, w)
+        check_values(y, want_y, big_y, "x far apart"), check_values(h, want_h, big_h, "x far apart")
+        view.copy_(r)
+        y, h = ab.gated_residual_norm(x, view, w, residual_out=view)
+        check_values(y, want_y, big_y, "residual far apart"), check_values(h, want_h, big_h, "residual far apart")
+        assert h is view
+        two = torch.as_strided(buf, (m, n // 2 * 2), (pitch, 1))
+        u, v = x[:, : n // 2].double(), x[:, n // 2 : n // 2 * 2].double()
+        two.copy_(x[:, : n // 2 * 2])
+        want = act64(u, "silu") * v
+        check_values(ab.act_and_mul(two), want, want.abs(), "input far apart")
+        out = torch.as_strided(buf, (m, n // 2), (pitch, 1), n)
+        ab.silu_and_mul(out, x[:, : n // 2 * 2])
+        check_values(out, want, want.abs(), "output far apart")
+
+
+def test_several_threads_at_once(ab):
+    """Four host threads, each on a stream of its own, run layers of different sizes at the same time."""
+    import threading
+
+    layers = [Layer(ab, kind, m) for kind, m in (("bf16", 40), ("mxfp8", 300), ("mxfp4", 1100), ("bf16", 1))]
+    want = [layer.run() for layer in layers]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    out = layers[i].run()
+                torch.cuda.current_stream().synchronize()
+            for k in (1, 2, 4, 5, 6):
+                assert torch.equal(out[k], want[i][k]), f"layer {i}, step {k}"
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(layers))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert ab.device_status(0) == (0, 0, 0, 0)

@@ -207,7 +207,7 @@ def test_norm_strides_leading_dimensions_and_in_place(ab):
     assert torch.equal(y2, y.view(15, 264)) and torch.equal(h2, h.view(15, 264)) and torch.equal(r2[:, 8:272], h2)
     assert (r2[:, :8] == 7).all() and (r2[:, 272:] == 7).all()
     assert torch.equal(wide[..., 528:], spare)
-    # rows that start on no 16-byte boundary take the element-wise path: same values up to the order of the sums
+    # rows that start on no 16-byte boundary (shifted groups): same values up to the order of the sums
     x3 = torch.empty(15, 271, dtype=torch.bfloat16, device="cuda")[:, 3:267]
     x3.copy_(x2)
     y3, _ = ab.gated_residual_norm(x3, residual.reshape(15, 264), w, gate=mod[:, 264:])

@@ -154,6 +154,15 @@ def test_strides_in_place_and_neighbours(ab, m):
     assert got.shape == (1, m, n) and torch.equal(got[0], p.run(residual=residual))
 
 
+def test_torch_ops_namespace(ab):
+    for kind in ("bf16", "mxfp8", "mxfp4"):
+        p = Problem(ab, kind, 70, 512, 256)
+        r, more = randn(1, 70, 512), [False] if kind == "mxfp8" else []
+        name = {"bf16": "gemm_a16w16_fused", "mxfp8": "gemm_a8w8_mxfp8_fused", "mxfp4": "gemm_a4w4_fused"}[kind]
+        got = getattr(torch.ops.aiter, name)(*p.args, None, "gelu", r, torch.float16, *more)
+        assert got.dtype == torch.float16 and torch.equal(got, p.run(activation="gelu", residual=r, otype=torch.float16))
+
+
 def test_shuffled_weight_and_empty_batch(ab):
     p = Problem(ab, "bf16", 40, 512, 256)
     bias = randn(1, 512)

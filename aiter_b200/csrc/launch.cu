@@ -4,6 +4,7 @@
 #include "launch.h"
 #include "gemm_persistent.cuh"
 #include "gemm_decode.cuh"
+#include "gemm_few_rows.cuh"
 #include "gemm_blockscale.cuh"
 
 #include <atomic>
@@ -1124,6 +1125,67 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
     }
 }
 
+// One to four rows of bf16 with a fused epilogue, unless the caller names a tile; false where the operands' addresses or order ask for
+// the other kernels.
+template <int M>
+static void launch_few_rows(const FewRowsParams& prm, int num_sms, cudaStream_t stream)
+{
+    // warps for a pair of columns: as many as fill the machine with 24 warps an SM, each with 512 elements of K at least
+    int ks = 1;
+    const long long groups = (prm.N + kFewRowsCols - 1) / kFewRowsCols;
+    while(ks < 8 && groups * ks < 24LL * num_sms && prm.K >= 1024u * ks)
+        ks *= 2;
+    cudaLaunchConfig_t lc{};
+    lc.gridDim  = dim3(static_cast<unsigned>((groups + 8 / ks - 1) / (8 / ks)), 1, 1);
+    lc.blockDim = dim3(256, 1, 1);
+    lc.stream   = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs    = attr;
+    lc.numAttrs = pdl_disabled() ? 0 : 1;
+    auto kernel = ks == 1 ? gemm_few_rows_kernel<M, 1> : ks == 2 ? gemm_few_rows_kernel<M, 2> : ks == 4 ? gemm_few_rows_kernel<M, 4> : gemm_few_rows_kernel<M, 8>;
+    B200_CUDA(cudaLaunchKernelEx(&lc, kernel, prm));
+    g_launches.fetch_add(1);
+}
+static bool try_launch_few_rows(const GemmProblem& prob, int num_sms)
+{
+    const KernelConfig& c = prob.cfg;
+    if(!prob.fused || prob.kind != PK_BF16 || prob.M > 4 || prob.batch != 1 || c.swap >= 0 || c.bn > 0 || c.cg > 0 || c.stages > 0 || c.log2_splitk >= 0)
+        return false;
+    // (us here / on tensor cores: 1 x 8192 x 8192 24.5 / 24.0; two rows 1024 x 8192 7.5 / 12.9, 2048 x 2048 5.3 / 6.8, 4096 x 4096 11.9 / 10.0;
+    // four rows 8.1 / 13.0, 5.8 / 6.8, 13.1 / 10.1)
+    if(prob.N * prob.K > (prob.M == 1 ? 48LL : 10LL) << 20)
+        return false;
+    auto rows16 = [](const Operand& o) { return o.mode == OPM_ROWMAJOR && (reinterpret_cast<uintptr_t>(o.ptr) & 15) == 0 && (o.rows == 1 || o.ld_bytes % 16 == 0); };
+    if(!rows16(prob.act) || !rows16(prob.wgt) || prob.N >= (1LL << 31) || prob.K >= (1LL << 31))
+        return false;
+    FewRowsParams prm{};
+    prm.a         = static_cast<const uint8_t*>(prob.act.ptr);
+    prm.a_ld      = prob.act.ld_bytes;
+    prm.b         = static_cast<const uint8_t*>(prob.wgt.ptr);
+    prm.b_ld      = prob.wgt.ld_bytes;
+    prm.bias      = prob.fused_bias;
+    prm.bias_mode = prob.fused_bias_mode;
+    prm.res       = prob.residual;
+    prm.res_ld    = prob.residual_ld;
+    prm.res_mode  = prob.residual_mode;
+    prm.out       = prob.out;
+    prm.out_ld    = prob.ldo;
+    prm.out_mode  = prob.out_mode;
+    prm.act       = prob.activation;
+    prm.N         = static_cast<unsigned>(prob.N);
+    prm.K         = static_cast<unsigned>(prob.K);
+    switch(prob.M)
+    {
+    case 1: launch_few_rows<1>(prm, num_sms, prob.stream); break;
+    case 2: launch_few_rows<2>(prm, num_sms, prob.stream); break;
+    case 3: launch_few_rows<3>(prm, num_sms, prob.stream); break;
+    default: launch_few_rows<4>(prm, num_sms, prob.stream); break;
+    }
+    return true;
+}
+
 size_t fused_workspace_bytes(long long M, long long N, long long K)
 {
     if(M < kScalePrepassMinM || K % 256 != 0 || K < (tall_problem(M, N) ? 1024 : kScalePrepassMinK) || relay_prepass_disabled())
@@ -1304,6 +1366,8 @@ static void launch_gemm_locked(const GemmProblem& prob)
     }
     DeviceState& st = (prob.scratch != nullptr) ? local_state : device_state(prob.device);
     require_healthy(st, prob.device);
+    if(try_launch_few_rows(prob, st.sm_count))
+        return;
 
     KernelConfig cfg = prob.cfg;
     const bool requant = (prob.out_mode == OUT_E2M1 || prob.out_mode == OUT_MXFP8);

@@ -90,7 +90,8 @@ def randn(seed, *shape, dtype=torch.bfloat16):
 # every kernel variant that the library's own choice reaches: few rows (one tile, several, K split), one-CTA tiles, pairs, odd sizes
 SHAPES = {
     "bf16": [(1, 128, 64), (1, 4096, 4096), (7, 40, 8), (16, 1001, 520), (33, 256, 1032), (64, 1024, 1024), (100, 512, 2048), (200, 1001, 72), (256, 4096, 512),
-             (257, 64, 1024), (333, 1001, 1160), (700, 24, 128), (600, 520, 4096), (1024, 4096, 256), (4096, 1160, 192), (2100, 2056, 64)],
+             (257, 64, 1024), (333, 1001, 1160), (700, 24, 128), (600, 520, 4096), (1024, 4096, 256), (4096, 1160, 192), (2100, 2056, 64),
+             (1, 76, 856), (2, 4096, 1032), (3, 1001, 520), (4, 333, 8), (4, 130, 16384), (2, 5, 24), (1, 1, 8), (3, 9000, 264), (4, 2048, 2048), (5, 1024, 4096)],
     "mxfp8": [(1, 256, 128), (16, 4096, 1024), (64, 528, 512), (130, 4096, 256), (300, 1040, 384), (1024, 2048, 512), (4100, 1152, 256)],
     "mxfp4": [(1, 256, 64), (32, 7168, 512), (64, 528, 320), (200, 1024, 1024), (300, 1040, 384), (1024, 2048, 512), (4100, 1152, 4096)],
 }
@@ -131,7 +132,7 @@ def test_named_tiles(ab, name):
     assert ab.device_status(0) == (0, 0, 0, 0)
 
 
-@pytest.mark.parametrize("m", [1, 5, 64, 300, 1024])
+@pytest.mark.parametrize("m", [1, 3, 5, 64, 300, 1024])
 def test_strides_in_place_and_neighbours(ab, m):
     """Outputs and residuals inside wider tensors, at pitches that do and do not allow tile copies; what lies around stays as it was."""
     n, k = 528, 256
@@ -191,7 +192,7 @@ def test_infinities_and_nan(ab):
 
 def test_other_stream_and_two_captured_graphs_at_once(ab):
     """Two graphs captured one after the other and replayed at the same time on two streams: they share no workspace."""
-    cases = [(Problem(ab, "bf16", 4, 1024, 4096), randn(1, 4, 1024)), (Problem(ab, "bf16", 300, 512, 8192), randn(2, 300, 512)),
+    cases = [(Problem(ab, "bf16", 4, 1024, 4096), randn(1, 4, 1024)), (Problem(ab, "bf16", 5, 1024, 4096), randn(4, 5, 1024)), (Problem(ab, "bf16", 300, 512, 8192), randn(2, 300, 512)),
              (Problem(ab, "mxfp4", 1024, 1024, 4096), randn(3, 1024, 1024))]
     for p, r in cases:
         want = p.run(activation="gelu", residual=r)

@@ -224,7 +224,14 @@ bool launch_stream(const NormParams& prm, StreamShape sh, int sms, cudaStream_t 
     sh.lay.param_off = sh.lay.stages * row;
     unsigned grid    = std::min(prm.M, static_cast<unsigned>(sms) * ctas);
     if(sh.flat)
+    {
+        // A CTA brings its parameters to shared memory first: with fewer than four rows for it the general kernel's shifted groups are ahead
+        // (us, here and there: 1000 x 1155 10 and 6.3, 400 x 3001 13.5 and 8.4, 1142 x 5287 41 and 26; with 5 to 18 rows 16384 x 301 27 and
+        // 31, 8200 x 1155 38 and 40, 8192 x 4097 50 and 76).
         grid = std::max(8u, grid / 8 * 8);
+        if(prm.M < 4 * grid)
+            return false;
+    }
     launch_smem(kernel, dim3(grid), dim3(sh.threads), static_cast<size_t>(sh.lay.stages) * row + sh.fixed, stream, prm, sh.lay);
     return true;
 }
@@ -268,9 +275,8 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
 {
     const unsigned n = prm.n;
     const int xd = prm.x.dt, rd = prm.res.ptr != nullptr ? prm.res.dt : (prm.h.ptr != nullptr ? prm.h.dt : xd);
-    // (rows on any address: up to about four million elements the general kernel's shifted groups are ahead - 1000 x 1155 6.3 us against
-    // 10, 400 x 3001 8.4 and 13.5, 8200 x 1155 40 and 38, 8192 x 4097 76 and 50 -, and so they are for short rows, 16384 x 203 17 and 22)
-    if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && (n < 256 || static_cast<unsigned long long>(prm.M) * n < (4u << 20))) || (prm.h.ptr != nullptr && prm.h.dt != rd))
+    // (short rows on any address: the general kernel's shifted groups, 16384 x 203 17 us against 22)
+    if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && n < 256) || (prm.h.ptr != nullptr && prm.h.dt != rd))
         return false;
     // one type for all parameters
     int pd          = -1;
@@ -287,7 +293,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     const int half = xd == OUT_F32 ? (rd == OUT_F32 ? OUT_BF16 : rd) : xd; // the call's 16-bit type
     if(pd < 0)
         pd = half;
-    if((xd != OUT_F32 && rd != OUT_F32 && xd != rd) || (xd == OUT_F32 && rd != OUT_F32) || (pd != OUT_F32 && pd != half))
+    if((xd != OUT_F32 && rd != OUT_F32 && xd != rd) || (pd != OUT_F32 && pd != half))
         return false;
     StreamShape sh{};
     unsigned cnt, elems = n;
@@ -324,7 +330,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     sh.lay.r_bytes = prm.res.ptr != nullptr ? elems * bytes_of(rd) : 0u;
     wait_report_targets(device, &sh.lay.report.status, &sh.lay.report.host_mirror);
     auto run = [&](auto x, auto r) {
-        constexpr int XD = decltype(x)::value, RD = decltype(r)::value, HD = XD == OUT_F32 ? OUT_BF16 : XD;
+        constexpr int XD = decltype(x)::value, RD = decltype(r)::value, HD = XD != OUT_F32 ? XD : RD != OUT_F32 ? RD : OUT_BF16;
         return pd == OUT_F32 ? launch_stream_shape<XD, RD, OUT_F32>(prm, cnt, sh, sms, stream) : launch_stream_shape<XD, RD, HD>(prm, cnt, sh, sms, stream);
     };
     using B = std::integral_constant<int, OUT_BF16>;
@@ -334,7 +340,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
         return rd == OUT_BF16 ? run(B{}, B{}) : run(B{}, F{});
     if(xd == OUT_F16)
         return rd == OUT_F16 ? run(H{}, H{}) : run(H{}, F{});
-    return run(F{}, F{});
+    return rd == OUT_BF16 ? run(F{}, B{}) : rd == OUT_F16 ? run(F{}, H{}) : run(F{}, F{});
 }
 
 void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaStream_t stream)

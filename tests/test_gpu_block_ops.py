@@ -109,7 +109,7 @@ CASES = [
     (5, 7, "fp16", "bf16", {"norm": "layer", "bias": True}),
     (2001, 37, "bf16", "fp32", {"norm": "layer", "bias": True, "post": True}),
     (1003, 99, "fp32", "bf16", {"post": True, "post_bias": True, "gate": "token"}),
-    (4000, 1155, "bf16", "fp32", {"norm": "layer", "affine": "sample4", "offset": 1.0, "bias": True, "gate": "sample4", "post": True}),
+    (4800, 1155, "bf16", "fp32", {"norm": "layer", "affine": "sample4", "offset": 1.0, "bias": True, "gate": "sample4", "post": True}),
     (700, 8000, "bf16", "bf16", {"post": True, "norm": "layer"}),
     (3, 8190, "bf16", "bf16", {"post": True, "post_bias": True}),
     # many rows: the streaming kernels, aligned and not, every width class
@@ -129,11 +129,16 @@ CASES = [
     (450, 8192, "bf16", "bf16", {"post": True, "gate": "channel16", "scale": 0.5, "post_bias": True}),
     (310, 9001, "bf16", "bf16", {"post": True}),
     (400, 512, "bf16", "fp16", {"gate": "channel"}),
-    (800, 7001, "fp16", "fp32", {"post": True, "norm": "layer", "post_bias": True, "bias": True}),
-    (4200, 1001, "fp32", "fp32", {"gate": "token", "affine": "sample4", "offset": 1.0}),
-    (9000, 513, "bf16", "bf16", {"norm": "layer", "gate": "sample4", "post": True, "scale": 0.5}),
+    (700, 4096, "fp32", "bf16", {"post": True, "gate": "channel16"}),
+    (5000, 128, "fp32", "fp16", {"norm": "layer", "bias": True}),
+    (444, 1152, "fp32", "fp16", {"gate": "token", "scale": 0.5}),
+    (6400, 1001, "fp32", "bf16", {"norm": "layer", "affine": "sample4", "offset": 1.0, "gate": "sample4", "bias": True}),
+    (320, 12288, "fp32", "bf16", {"post": True, "post_bias": True}),
+    (1300, 7001, "fp16", "fp32", {"post": True, "norm": "layer", "post_bias": True, "bias": True}),
+    (6400, 1001, "fp32", "fp32", {"gate": "token", "affine": "sample4", "offset": 1.0}),
+    (10000, 513, "bf16", "bf16", {"norm": "layer", "gate": "sample4", "post": True, "scale": 0.5}),
     (16400, 257, "bf16", None, {"gate": "channel", "bias": True}),
-    (700, 7999, "bf16", "bf16", {"post": True, "gate": "channel16"}),
+    (1300, 7999, "bf16", "bf16", {"post": True, "gate": "channel16"}),
 ]
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 

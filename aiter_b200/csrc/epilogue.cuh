@@ -228,8 +228,11 @@ __device__ __forceinline__ bool fused_tile(FusedWarp& f, const FusedParams& epi,
                 tma_store_2d_hint(map_out, f.slots + (f.seq & 1) * epi.slot_bytes, q_first * (out32 ? 4 : 2), row0, l2_evict_first_policy());
             else
                 tma_store_2d(map_out, f.slots + (f.seq & 1) * epi.slot_bytes, q_first * (out32 ? 4 : 2), row0);
-            bulk_commit_group();
         }
+        // A group for every step, empty where the step lies outside the output and stores nothing: "all groups but the last" then are
+        // the steps before the previous one, so that a slot is never written while the store of its last content still reads it.
+        if(lane == 0)
+            bulk_commit_group();
     }
     return true;
 }

@@ -1122,8 +1122,9 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                                 tma_store_2d(&map_out, epi_s + ebuf * 2048, q_first * 2, p_warp0);
                             else
                                 tma_store_2d(&map_out, epi_s + ebuf * 2048, p_warp0 * 2, q_first);
-                            bulk_commit_group();
                         }
+                        if(lane == 0)
+                            bulk_commit_group(); // (an empty group where nothing is stored: the wait above counts chunks)
                         ebuf ^= 1;
                     }
                     else if(p < prm.rows_p)
@@ -1367,10 +1368,9 @@ gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_c
                         fence_proxy_async_smem();
                         __syncwarp();
                         if(lane == 0 && p_warp0 < prm.rows_p && q_first < prm.rows_q)
-                        {
                             tma_store_2d(&map_out, epi_s + wbuf, q_first * 2, p_warp0);
-                            bulk_commit_group();
-                        }
+                        if(lane == 0)
+                            bulk_commit_group(); // (an empty group where nothing is stored: the wait above counts chunks)
                         if(prm.epi_bufs == 2)
                             wbuf ^= 4096u;
                     }

@@ -35,3 +35,20 @@ def test_fused_epilogue_without_a_residual(ab, kind, n, name, otype):
     got = repeats_agree(lambda: p.run(otype=otype, kernelName=name), f"{kind} {n} {name}")
     p.check(got, what=f"{kind} {n} {name}")
     assert ab.device_status(0) == (0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("name", ["tc5_256x192_n_s3", "tc5_256x256_n_s3", "tc5_128x192_n_s3", "tc5_128x96_n_s3", "tc5_128x224_n_s2", "tc5_128x128_t_s3", ""])
+@pytest.mark.parametrize("m,n", [(1280, 4096), (1280, 4096 + 64), (1296, 4096 + 16)])
+@pytest.mark.parametrize("kind", ["bf16", "mxfp8", "mxfp4"])
+def test_plain_epilogue(ab, kind, m, n, name):
+    p = Problem(ab, kind, m, n, 256)
+
+    def run():
+        if kind == "mxfp8":
+            return ab.gemm_a8w8_mxfp8(*p.args, a_preshuffle=False, kernelName=name)
+        out = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+        return ab.gemm_a16w16_asm(*p.args, out, kernelName=name) if kind == "bf16" else ab.gemm_a4w4_asm(*p.args, out, kernelName=name)
+
+    got = repeats_agree(run, f"{kind} {m} {n} {name}")
+    p.check(got, what=f"{kind} {m} {n} {name}")
+    assert ab.device_status(0) == (0, 0, 0, 0)

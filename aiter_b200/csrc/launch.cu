@@ -166,12 +166,38 @@ static std::mutex g_mutex;
 static std::map<int, DeviceState> g_devices;
 static std::atomic<unsigned long long> g_launches{0};
 
+// The set-up of a device allocates and copies, which the first call on it may do while some stream of the process is being captured:
+// this thread's calls are then not held against the capture (they belong to no stream of it), and what goes through a stream goes
+// through one of the set-up's own.
+struct SetupScope
+{
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaStream_t stream        = nullptr;
+    SetupScope()
+    {
+        B200_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+        if(e != cudaSuccess)
+        {
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            B200_CUDA(e);
+        }
+    }
+    ~SetupScope()
+    {
+        cudaStreamDestroy(stream);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    SetupScope(const SetupScope&) = delete;
+};
+
 static DeviceState& device_state(int device)
 {
     // caller holds g_mutex and has made `device` current
     auto it = g_devices.find(device);
     if(it != g_devices.end())
         return it->second;
+    SetupScope setup;
     DeviceState st;
     cudaDeviceProp prop;
     B200_CUDA(cudaGetDeviceProperties(&prop, device));
@@ -180,7 +206,7 @@ static DeviceState& device_state(int device)
     st.sm_count   = prop.multiProcessorCount;
     st.smem_optin = static_cast<int>(prop.sharedMemPerBlockOptin);
     B200_CUDA(cudaMalloc(&st.status, 4 * sizeof(unsigned int)));
-    B200_CUDA(cudaMemset(st.status, 0, 4 * sizeof(unsigned int)));
+    B200_CUDA(cudaMemsetAsync(st.status, 0, 4 * sizeof(unsigned int), setup.stream));
     // one pinned host word, mapped into the device: a kernel whose wait runs out stores its code there too, so
     // the next call on this device can refuse to launch without a device round trip
     void* host_word = nullptr;
@@ -194,7 +220,8 @@ static DeviceState& device_state(int device)
     }
     else
         cudaGetLastError();
-    B200_CUDA(cudaMemcpyToSymbol(c_wait_ctl, &st.wait_ctl, sizeof(WaitControl)));
+    B200_CUDA(cudaMemcpyToSymbolAsync(c_wait_ctl, &st.wait_ctl, sizeof(WaitControl), 0, cudaMemcpyHostToDevice, setup.stream));
+    B200_CUDA(cudaStreamSynchronize(setup.stream));
     return g_devices.emplace(device, st).first->second;
 }
 

@@ -89,14 +89,17 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
     p.ldo        = M == 1 ? (N + 7) / 8 * 8 : out->strides[0]; // (one row: any pitch, and one that allows a tensor map)
     p.fused      = true;
     p.activation = f.activation;
-    // the operands are read until the last tile has been written
-    for(const aiter_tensor_t* t : {first, B})
-    {
+    // the operands and their block scales are read until the last tile has been written
+    const Span so{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M};
+    auto span_of = [](const aiter_tensor_t* t) {
         const int size = t->dtype_ == AITER_DTYPE_bf16 || t->dtype_ == AITER_DTYPE_fp16 ? 2 : 1;
-        B200_CHECK(M == 0 || !overlap(Span{reinterpret_cast<uintptr_t>(t->ptr), t->strides[0] * size, t->shape[1] * size, t->shape[0]},
-                                      Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}),
-                   fn, ": out overlaps an operand");
-    }
+        return Span{reinterpret_cast<uintptr_t>(t->ptr), t->strides[0] * size, t->shape[1] * size, t->shape[0]};
+    };
+    auto span_of_scales = [](const ScaleOperand& s) { return Span{reinterpret_cast<uintptr_t>(s.ptr), 0, s.ptr == nullptr ? 0 : s.padded_rows * s.padded_cols, 1}; };
+    for(const aiter_tensor_t* t : {first, B})
+        B200_CHECK(!overlap(span_of(t), so), fn, ": out overlaps an operand");
+    for(const ScaleOperand* s : {&p.act_sf, &p.wgt_sf})
+        B200_CHECK(!overlap(span_of_scales(*s), so), fn, ": out overlaps the block scales");
     if(f.workspace != nullptr)
     {
         require_tensor(f.workspace, fn, "workspace", 1);
@@ -104,6 +107,21 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
         require_rows_contiguous(f.workspace, fn, "workspace");
         require_same_device(first, f.workspace, fn, "workspace");
         B200_CHECK((reinterpret_cast<uintptr_t>(f.workspace->ptr) & 15) == 0, fn, ": workspace must be 16-byte aligned");
+        // it is written before the GEMM reads anything
+        const Span sw{reinterpret_cast<uintptr_t>(f.workspace->ptr), 0, static_cast<long long>(f.workspace->numel_), 1};
+        for(const aiter_tensor_t* t : {first, B})
+            B200_CHECK(!overlap(span_of(t), sw), fn, ": workspace overlaps an operand");
+        for(const ScaleOperand* s : {&p.act_sf, &p.wgt_sf})
+            B200_CHECK(!overlap(span_of_scales(*s), sw), fn, ": workspace overlaps the block scales");
+        B200_CHECK(!overlap(so, sw), fn, ": workspace overlaps out");
+        for(const aiter_tensor_t* t : {f.bias, f.residual})
+        {
+            if(t == nullptr || t->ndim < 1 || t->ndim > 2) // (refused below)
+                continue;
+            const int size = t->dtype_ == AITER_DTYPE_fp32 ? 4 : 2, last = t->ndim - 1;
+            B200_CHECK(!overlap(Span{reinterpret_cast<uintptr_t>(t->ptr), last ? t->strides[0] * size : 0, t->shape[last] * size, last ? t->shape[0] : 1}, sw), fn,
+                       ": workspace overlaps bias or residual");
+        }
         p.workspace       = f.workspace->ptr;
         p.workspace_bytes = f.workspace->numel_;
     }
@@ -118,8 +136,7 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
         B200_CHECK(p.fused_bias_mode >= 0, fn, ": bias must be bf16, fp16 or fp32 (got ", dtype_name(f.bias->dtype_), ")");
         const int bb = p.fused_bias_mode == OUT_F32 ? 4 : 2;
         require_rows(f.bias, bb, fn, "bias");
-        B200_CHECK(M == 0 || !overlap(Span{reinterpret_cast<uintptr_t>(f.bias->ptr), 0, N * bb, 1}, Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}), fn,
-                   ": out overlaps bias");
+        B200_CHECK(!overlap(Span{reinterpret_cast<uintptr_t>(f.bias->ptr), 0, N * bb, 1}, so), fn, ": out overlaps bias");
     }
     if(f.residual != nullptr)
     {
@@ -136,9 +153,7 @@ static void set_fused(GemmProblem& p, const aiter_tensor_t* first, const aiter_t
         const int rb = p.residual_mode == OUT_F32 ? 4 : 2;
         require_rows(r, rb, fn, "residual");
         const bool same = r->ptr == out->ptr && p.residual_ld == p.ldo && p.residual_mode == p.out_mode;
-        B200_CHECK(M == 0 || same ||
-                       !overlap(Span{reinterpret_cast<uintptr_t>(r->ptr), p.residual_ld * rb, N * rb, M}, Span{reinterpret_cast<uintptr_t>(out->ptr), p.ldo * ob, N * ob, M}),
-                   fn, ": out overlaps residual");
+        B200_CHECK(same || !overlap(Span{reinterpret_cast<uintptr_t>(r->ptr), p.residual_ld * rb, N * rb, M}, so), fn, ": out overlaps residual");
     }
 }
 

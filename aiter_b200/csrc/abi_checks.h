@@ -67,6 +67,8 @@ struct Span
 // Whether two matrices share memory (rows of one pitch may interleave: two column slices of one tensor do not overlap)
 inline bool overlap(const Span& a, const Span& b)
 {
+    if(a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0)
+        return false;
     if(a.first + static_cast<uintptr_t>((a.rows - 1) * a.pitch + a.width) <= b.first || b.first + static_cast<uintptr_t>((b.rows - 1) * b.pitch + b.width) <= a.first)
         return false;
     if(a.pitch != b.pitch || a.pitch <= 0)

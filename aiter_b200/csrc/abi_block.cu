@@ -447,15 +447,19 @@ extern "C" int aiter_b200_gated_residual_norm(aiter_tensor_t* out, aiter_tensor_
             B200_CHECK(residual == nullptr || same_rows(prm.h, prm.res) || !overlap(span(prm.res, M, n), sh), fn, ": residual_out overlaps residual");
         }
         // every row reads the parameters, and the scales are written beside the rows
+        auto span_of = [&](const aiter_tensor_t* t) {
+            const int size = t == scales ? 1 : t->dtype_ == AITER_DTYPE_fp32 ? 4 : 2;
+            const bool one = t->ndim == 1;
+            return Span{reinterpret_cast<uintptr_t>(t->ptr), one ? 0 : t->strides[0] * size, t->shape[t->ndim - 1] * size, one ? 1 : t->shape[0]};
+        };
         for(const aiter_tensor_t* t : {weight, bias, gate, post_weight, post_bias, scales})
         {
             if(t == nullptr)
                 continue;
-            const int size = t == scales ? 1 : t->dtype_ == AITER_DTYPE_fp32 ? 4 : 2;
-            const bool one = t->ndim == 1;
-            const Span st{reinterpret_cast<uintptr_t>(t->ptr), one ? 0 : t->strides[0] * size, t->shape[t->ndim - 1] * size, one ? 1 : t->shape[0]};
+            const Span st = span_of(t);
             B200_CHECK(!overlap(st, sy) && (residual_out == nullptr || !overlap(st, span(prm.h, M, n))), fn, ": an output overlaps a parameter or the scales");
             B200_CHECK(t != scales || (!overlap(st, sx) && (residual == nullptr || !overlap(st, span(prm.res, M, n)))), fn, ": scales overlap an input");
+            B200_CHECK(t == scales || scales == nullptr || !overlap(st, span_of(scales)), fn, ": scales overlap a parameter");
         }
         prm.post          = post_norm != 0;
         prm.layer         = norm;

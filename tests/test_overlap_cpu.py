@@ -47,3 +47,14 @@ def test_fused_gemms_refuse_scales_and_workspaces_that_overlap(ab):
                       (far + 2 * MB + 256 * 8 - 16, "workspace overlaps the block scales"), (far + 3 * MB - 4080, "workspace overlaps the block scales"),
                       (far + 4 * MB, "workspace overlaps bias or residual"), (far + 5 * MB + out_bytes - 16, "workspace overlaps bias or residual")]:
         refuse(ab, "aiter_b200_gemm_a4w4_fused", mxfp4(ab, workspace=f((4096,), u8, ptr=at)), match)
+
+
+def test_norm_refuses_scales_over_a_parameter(ab):
+    f, far = lambda *a, **k: fake(ab, *a, **k), BASE + 32 * MB
+    at = far + 8 * MB
+    base = dict(out=f((M, N), torch.float8_e4m3fn, ptr=BASE), scales=f((M, N // 32), torch.uint8, ptr=at), residual_out=f((M, N), ptr=far), x=f((M, N), ptr=far + MB),
+                residual=f((M, N), ptr=far + 2 * MB), weight=None, bias=None, gate=None, post_weight=None, post_bias=None, residual_scale=1.0, weight_offset=0.0,
+                eps=1e-6, norm=1, post_norm=1, shuffle=0)
+    for name in ("weight", "bias", "gate", "post_weight", "post_bias"):
+        for p in (f((N,), ptr=at), f((N,), torch.float32, ptr=at - N * 4 + 16), f((2, N), ptr=at - 2 * N * 2 + 16)):
+            refuse(ab, "aiter_b200_gated_residual_norm", list({**base, name: p}.values()), "scales overlap a parameter")

@@ -259,8 +259,8 @@ def noalloc_status(device: int = 0):
 
 
 def debug_wait_control(device: int = 0, limit_ns: int = 1_000_000_000, withhold_scales: bool = False) -> None:
-    """Bound of the in-kernel waits on `device` and the switch that makes one producer issue nothing (tests of the
-    time-out path).  Call with no arguments to restore the defaults."""
+    """Bound of the in-kernel waits on `device` and the switch that makes a GEMM's scale producer and the row loads of a
+    streaming norm issue nothing (tests of the time-out path).  Call with no arguments to restore the defaults."""
     rc = _lib.aiter_b200_debug_wait_control(int(device), ctypes.c_ulonglong(int(limit_ns)), int(bool(withhold_scales)))
     if rc != 0:
         msg = _lib.aiter_get_last_error()

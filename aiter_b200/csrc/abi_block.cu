@@ -328,7 +328,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
     }
     sh.lay.x_bytes = elems * bytes_of(xd);
     sh.lay.r_bytes = prm.res.ptr != nullptr ? elems * bytes_of(rd) : 0u;
-    wait_report_targets(device, &sh.lay.report.status, &sh.lay.report.host_mirror);
+    sh.lay.report = wait_report(device);
     auto run = [&](auto x, auto r) {
         constexpr int XD = decltype(x)::value, RD = decltype(r)::value, HD = XD != OUT_F32 ? XD : RD != OUT_F32 ? RD : OUT_BF16;
         return pd == OUT_F32 ? launch_stream_shape<XD, RD, OUT_F32>(prm, cnt, sh, sms, stream) : launch_stream_shape<XD, RD, HD>(prm, cnt, sh, sms, stream);

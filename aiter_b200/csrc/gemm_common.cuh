@@ -41,8 +41,8 @@ struct WaitControl
 {
     unsigned long long limit_ns;  // wall-time bound of every in-kernel wait
     unsigned int* host_mirror;    // pinned, device-mapped host word that receives the first failure code (may be null)
-    unsigned int withhold_scales; // test hook: the raw-scale producer of the persistent kernel issues nothing, so
-                                  // the waits of the roles behind it run out after limit_ns
+    unsigned int withhold_scales; // test hook: the raw-scale producer of the persistent kernel and the row loads of the
+                                  // streaming norms issue nothing, so the waits behind them run out after limit_ns
 };
 static __constant__ WaitControl c_wait_ctl = {kWaitLimitNs, nullptr, 0u};
 
@@ -68,6 +68,8 @@ struct WaitReport
 {
     unsigned int* status;      // the device status record
     unsigned int* host_mirror; // pinned host word read before every launch (may be null)
+    unsigned long long limit_ns; // as in WaitControl
+    unsigned int withhold;       // test hook: issue no loads
 };
 __device__ __forceinline__ void report_timeout(const WaitReport& r, uint32_t code, uint32_t detail)
 {

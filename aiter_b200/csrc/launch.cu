@@ -291,7 +291,7 @@ int device_sm_count(int device)
     return n;
 }
 
-void wait_report_targets(int device, unsigned int** status, unsigned int** host_mirror)
+WaitReport wait_report(int device)
 {
     int prev = 0;
     B200_CUDA(cudaGetDevice(&prev));
@@ -302,8 +302,7 @@ void wait_report_targets(int device, unsigned int** status, unsigned int** host_
     if(prev != device)
         cudaSetDevice(prev);
     require_healthy(st, device);
-    *status      = st.status;
-    *host_mirror = st.wait_ctl.host_mirror;
+    return WaitReport{st.status, st.wait_ctl.host_mirror, st.wait_ctl.limit_ns, st.wait_ctl.withhold_scales};
 }
 
 void read_device_status(int device, unsigned int out_words[4])

@@ -156,14 +156,15 @@ void launch_blockscale(const BlockScaleProblem& prob);
 // "bs_fewrows" | "bs_128x128" | "bs_256x256" [+ "_k<n>"] -> (variant, log2 split); false when the name is not one of these
 bool parse_blockscale_name(const char* name, int& variant, int& log2_splitk);
 void read_device_status(int device, unsigned int out_words[4]);
-// Bound of every in-kernel wait on `device` (1 ms .. 10 s, default 1 s) and the test hook that makes the persistent
-// kernel's scale producer issue nothing, so that a wait runs out.  Synchronises the device.
+// Bound of every in-kernel wait on `device` (1 ms .. 10 s, default 1 s) and the test hook that makes the GEMM
+// kernels' scale producers and the streaming norms' row loads issue nothing, so that a wait runs out.  Synchronises the device.
 void set_wait_control(int device, unsigned long long limit_ns, int withhold_scales);
 unsigned long long launch_count();
 void count_launch(); // kernels launched outside launch.cu report themselves here
 int device_sm_count(int device);
-// Device status record and pinned mirror of a device, for kernels launched outside launch.cu; refuses while a record is pending
-void wait_report_targets(int device, unsigned int** status, unsigned int** host_mirror);
+struct WaitReport; // gemm_common.cuh
+// What the bounded waits of kernels launched outside launch.cu need of a device; refuses while a record is pending
+WaitReport wait_report(int device);
 bool programmatic_launch_enabled(); // launches carry the programmatic-serialization attribute
 
 } // namespace b200

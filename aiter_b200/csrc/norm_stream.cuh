@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float red[8][32]; // two sets of slots, for even and odd rows: one barrier a sum is enough
     __shared__ __align__(8) uint64_t full[4];
+    __shared__ volatile unsigned gave_up; // 1 + the row in which a thread's wait ran out
     const unsigned t = threadIdx.x, T = blockDim.x, n = prm.n;
     const bool has_res = prm.res.ptr != nullptr;
     const bool gate_one = prm.gate.ptr != nullptr && prm.gate_scalar;
@@ -159,6 +160,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
     const unsigned S = lay.stages, stage_bytes = lay.x_bytes + lay.r_bytes;
     if(t == 0)
     {
+        gave_up = 0;
         for(unsigned s = 0; s < S; ++s)
             mbar_init(smem_u32(&full[s]), 1);
         mbar_fence_init();
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
         if(has_res)
             bulk_load(dst + lay.x_bytes, static_cast<const uint8_t*>(prm.res.ptr) + static_cast<size_t>(row) * prm.res.ld * RS, lay.r_bytes, bar);
     };
-    if(t == 0)
+    if(t == 0 && lay.report.withhold == 0u)
         for(unsigned i = 0; i < min(S, rows); ++i)
             load(row0 + i, i);
     // the parameters' entries of the current row, until row `change`: indexes, since registers are what two CTAs an SM leave
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
     };
     auto entry = [&](const RowParam& q, unsigned e) { return static_cast<const uint8_t*>(q.ptr) + static_cast<size_t>(e) * q.ld * PS; };
     unsigned s = 0, phase = 0;
-    bool expired = false;
+    bool stopped = false;
     const unsigned col0 = t * 8, col_step = T * 8;
 #pragma unroll 1
     for(unsigned i = 0; i < rows; ++i)
@@ -208,14 +210,20 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
         const unsigned row = row0 + i;
         if(row >= change) // (the same for every thread)
             entries(row);
-        // (bounded, though a copy of valid memory always completes: on expiry the status record says that the output is incomplete)
-        if(!expired && !mbar_try_wait(smem_u32(&full[s]), phase))
+        // Bounded, though a copy of valid memory always completes.  A thread whose wait runs out stores no h and adds a NaN to the row's
+        // sum; a row with a NaN asks, behind the sum's barrier, whether that was the reason, and then the whole CTA stops there.  The
+        // status record says that the output is incomplete.
+        bool late = false; // this thread's wait ran out
+        if(!mbar_try_wait(smem_u32(&full[s]), phase))
         {
             const uint64_t t0 = global_timer_ns();
-            while(!expired && !mbar_try_wait_parked(smem_u32(&full[s]), phase, kParkNs))
-                expired = global_timer_ns() - t0 > kWaitLimitNs;
-            if(expired)
+            while(!late && !mbar_try_wait_parked(smem_u32(&full[s]), phase, kParkNs))
+                late = global_timer_ns() - t0 > lay.report.limit_ns;
+            if(late)
+            {
+                gave_up = i + 1;
                 report_timeout(lay.report, ST_TIMEOUT_ROWS, i);
+            }
         }
         const uint8_t* xs = smem + s * stage_bytes;
         const uint8_t* rs = xs + lay.x_bytes;
@@ -268,12 +276,17 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
                     for(int k = 0; k < P; ++k)
                         a = fma2(h[j][k], h[j][k], a);
             }
-            rstd = rsqrtf(row_sum(a.x + a.y, red, slot + 1) * prm.inv_n + prm.eps);
+            rstd = rsqrtf(row_sum(late ? __uint_as_float(0x7FFFFFFFu) : a.x + a.y, red, slot + 1) * prm.inv_n + prm.eps);
         };
         float mean = 0.f, rstd = 1.f;
         if(prm.post)
         {
             stats(0, mean, rstd);
+            if(rstd != rstd && gave_up == i + 1)
+            {
+                stopped = true;
+                break;
+            }
             const float2 a = make_float2(rstd, rstd);
             if(prm.layer)
             {
@@ -333,7 +346,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
                     for(int k = 0; k < P; ++k)
                         h[j][k] = make_float2(0.f, 0.f);
             }
-        if(prm.h.ptr != nullptr)
+        if(prm.h.ptr != nullptr && !late)
         {
             uint8_t* const hg = static_cast<uint8_t*>(prm.h.ptr) + static_cast<size_t>(row) * prm.h.ld * RS;
 #pragma unroll
@@ -345,8 +358,13 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
             }
         }
         stats(2, mean, rstd);
+        if(rstd != rstd && gave_up == i + 1)
+        {
+            stopped = true;
+            break;
+        }
         // every thread has read its part of the stage (the sum's barrier): a later row may land there
-        if(t == 0 && i + S < rows && !expired)
+        if(t == 0 && i + S < rows)
             load(row + S, s);
         if(++s == S)
         {
@@ -402,7 +420,7 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
                 fill_scale_padding(prm.sf, row, prm.M, n >> 5, t, T);
         }
     }
-    if(expired)
+    if(stopped)
     {
         // copies still in flight land before this CTA's shared memory is released (bounded)
         const uint64_t t0 = global_timer_ns();
@@ -423,6 +441,7 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float red[8][32];
     __shared__ __align__(8) uint64_t full[4];
+    __shared__ volatile unsigned gave_up; // 1 + the row in which a thread's wait ran out
     const unsigned t = threadIdx.x, T = blockDim.x, n = prm.n;
     const bool has_res  = prm.res.ptr != nullptr;
     const bool gate_one = prm.gate.ptr != nullptr && prm.gate_scalar;
@@ -436,6 +455,7 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
     const unsigned S = lay.stages, stage_bytes = lay.x_bytes + lay.r_bytes;
     if(t == 0)
     {
+        gave_up = 0;
         for(unsigned s = 0; s < S; ++s)
             mbar_init(smem_u32(&full[s]), 1);
         mbar_fence_init();
@@ -456,7 +476,7 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
         if(has_res)
             bulk_load(dst + lay.x_bytes + r0, static_cast<const uint8_t*>(prm.res.ptr) + (static_cast<size_t>(row) * prm.res.ld - e8) * RS + r0, rb, bar);
     };
-    if(t == 0)
+    if(t == 0 && lay.report.withhold == 0u)
         for(unsigned i = 0; i < min(S, rows); ++i)
             load(row_of(i), i);
     // the parameters of the current entries, element e of each at place e8 + e, until row `change`
@@ -500,20 +520,24 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
     const unsigned col0 = t * 8, col_step = T * 8;
     auto place = [&](int at) { return params + at * lay.param_pitch; };
     unsigned s = 0, phase = 0;
-    bool expired = false;
+    bool stopped = false;
 #pragma unroll 1
     for(unsigned i = 0; i < rows; ++i)
     {
         const unsigned row = row_of(i);
         if(row >= change) // (the same for every thread)
             entries(row);
-        if(!expired && !mbar_try_wait(smem_u32(&full[s]), phase))
+        bool late = false; // this thread's wait ran out
+        if(!mbar_try_wait(smem_u32(&full[s]), phase))
         {
             const uint64_t t0 = global_timer_ns();
-            while(!expired && !mbar_try_wait_parked(smem_u32(&full[s]), phase, kParkNs))
-                expired = global_timer_ns() - t0 > kWaitLimitNs;
-            if(expired)
+            while(!late && !mbar_try_wait_parked(smem_u32(&full[s]), phase, kParkNs))
+                late = global_timer_ns() - t0 > lay.report.limit_ns;
+            if(late)
+            {
+                gave_up = i + 1;
                 report_timeout(lay.report, ST_TIMEOUT_ROWS, i);
+            }
         }
         const uint8_t* xs = smem + s * stage_bytes;
         const uint8_t* rs = xs + lay.x_bytes;
@@ -584,7 +608,7 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
                     for(int k = 0; k < 4; ++k)
                         a = fma2(h[j][k], h[j][k], a);
             }
-            rstd = rsqrtf(row_sum(a.x + a.y, red, slot_ + 1) * prm.inv_n + prm.eps);
+            rstd = rsqrtf(row_sum(late ? __uint_as_float(0x7FFFFFFFu) : a.x + a.y, red, slot_ + 1) * prm.inv_n + prm.eps);
         };
         auto scale1 = [&](float f) {
 #pragma unroll
@@ -604,6 +628,11 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
         if(prm.post)
         {
             stats(0, mean, rstd);
+            if(rstd != rstd && gave_up == i + 1)
+            {
+                stopped = true;
+                break;
+            }
             if(prm.layer)
                 shift1(-mean);
             scale1(rstd);
@@ -648,11 +677,16 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
                     for_row(v, [&](int k) { store_out(p, 8 * v + k, (k & 1) ? h[j][k / 2].y : h[j][k / 2].x, DT); });
             }
         };
-        if(prm.h.ptr != nullptr)
+        if(prm.h.ptr != nullptr && !late)
             store(prm.h, std::integral_constant<int, RD>{});
         stats(2, mean, rstd);
+        if(rstd != rstd && gave_up == i + 1)
+        {
+            stopped = true;
+            break;
+        }
         // every thread has read its part of the stage (the sum's barrier): a later row may land there
-        if(t == 0 && i + S < rows && !expired)
+        if(t == 0 && i + S < rows)
             load(row_of(i + S), s);
         if(++s == S)
         {
@@ -673,7 +707,7 @@ __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_c
         else
             store(prm.y, std::integral_constant<int, OUT_F32>{});
     }
-    if(expired)
+    if(stopped)
     {
         const uint64_t t0 = global_timer_ns();
         while(global_timer_ns() - t0 < 200000ull) {}

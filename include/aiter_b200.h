@@ -257,9 +257,9 @@ AITER_B200_API int aiter_b200_act_and_mul(aiter_tensor_t* out, aiter_tensor_t* s
  * never polls still learns of an incomplete output at its next call. */
 AITER_B200_API int aiter_b200_device_status(int device, unsigned int out_words[4]);
 /* Test and diagnosis hook (no counterpart in the reference): the wall-time bound of every in-kernel wait on
- * `device`, 1 ms .. 10 s (default 1 s), and a switch that makes the scale producer of the MX GEMM kernel issue
- * nothing, so that the waits behind it run out after that bound, the kernel records its status and returns by
- * itself.  Used to exercise the time-out path without faulting or hanging anything.  Synchronises the device. */
+ * `device`, 1 ms .. 10 s (default 1 s), and a switch that makes the scale producer of the MX GEMM kernel and the
+ * row loads of the streaming norms issue nothing, so that the waits behind them run out after that bound, the kernel records its
+ * status and returns by itself.  Used to exercise the time-out path without faulting or hanging anything.  Synchronises the device. */
 AITER_B200_API int aiter_b200_debug_wait_control(int device, unsigned long long limit_ns, int withhold_scales);
 /* Human-readable list of the kernel configurations behind `kernelName`/`kernelId`. */
 AITER_B200_API const char* aiter_b200_kernel_list(void);

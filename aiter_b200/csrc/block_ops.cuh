@@ -665,6 +665,28 @@ __global__ void __launch_bounds__(CNT == 1 || SHIFT ? 1024 : 512) norm_rows_kern
         fill_scale_padding(prm.sf, row, prm.M, prm.n >> 5, t, T);
 }
 
+// A sum of any number of terms (Kahan, "Further remarks on reducing truncation errors", 1965): what an addition rounds off is carried
+// to the next one, so the error stays at 2^-23 of the sum of magnitudes however many terms there are.
+struct LongSum
+{
+    float sum = 0.f, lost = 0.f;
+    __device__ __forceinline__ void add(float v)
+    {
+        const float y = v - lost, t = sum + y, off = (t - sum) - y;
+        lost          = fabsf(off) <= 3.402823466e38f ? off : 0.f; // (an infinite sum stays one)
+        sum           = t;
+    }
+};
+// the values of a vector, added pairwise
+template <int VEC>
+__device__ __forceinline__ float pair_sum(const float (&v)[VEC])
+{
+    if(VEC == 1)
+        return v[0];
+    const int e = VEC == 1 ? 0 : 1;
+    return ((v[0] + v[e]) + (v[2 * e] + v[3 * e])) + ((v[4 * e] + v[5 * e]) + (v[6 * e] + v[7 * e]));
+}
+
 // Rows that do not fit the registers: a CTA goes over its row once per sum and once for the outputs, recomputing h each
 // time (the row comes from L2 after the first pass).
 template <int VEC>
@@ -725,30 +747,26 @@ __global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ 
         float m = 0.f;
         if(prm.layer)
         {
-            float s = 0.f;
+            LongSum s;
             for(unsigned col = t * VEC; col < n; col += T * VEC)
             {
                 float v[VEC];
                 load(col, v);
-#pragma unroll
-                for(int i = 0; i < VEC; ++i)
-                    s += v[i];
+                s.add(pair_sum(v));
             }
-            m = row_sum(s, red, slot) * prm.inv_n;
+            m = row_sum(s.sum, red, slot) * prm.inv_n;
         }
-        float s = 0.f;
+        LongSum s;
         for(unsigned col = t * VEC; col < n; col += T * VEC)
         {
             float v[VEC];
             load(col, v);
 #pragma unroll
             for(int i = 0; i < VEC; ++i)
-            {
-                const float d = v[i] - m;
-                s             = fmaf(d, d, s);
-            }
+                v[i] = (v[i] - m) * (v[i] - m);
+            s.add(pair_sum(v));
         }
-        const float q = row_sum(s, red, slot + 1) * prm.inv_n;
+        const float q = row_sum(s.sum, red, slot + 1) * prm.inv_n;
         mean          = m;
         rstd          = rsqrtf(q + prm.eps);
     };

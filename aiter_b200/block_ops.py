@@ -80,7 +80,8 @@ def gated_residual_norm(x: Tensor, residual: Tensor | None = None, weight: Tenso
 def act_and_mul(x: Tensor, activation: str = "silu", otype: torch.dtype | None = None, quant_dtype: torch.dtype | None = None,
                 shuffle=False):
     """y[.., j] = act(x[.., j]) * x[.., n + j] for x [.., 2n] (gate half first): the step between the two GEMMs of a gated layer.
-    activation: silu, gelu (erf), gelu_tanh or relu.  Returns y, or (y, y_scale) with quant_dtype fp4x2 / fp8: an MX operand, its
+    activation: silu, gelu (erf), gelu_tanh or relu, computed in fp32 (csrc/activation.cuh states the error; magnitudes of the activation
+    below 2^-119 may come out as 0).  Returns y, or (y, y_scale) with quant_dtype fp4x2 / fp8: an MX operand, its
     scales laid out by `shuffle` as per_1x32_mx_quant_hip does."""
     fn = "act_and_mul"
     act = activation_id(activation, fn)

@@ -6,6 +6,12 @@
 //   gelu_tanh  x / 2 * (1 + tanh u), u = sqrt(2 / pi) (x + 0.044715 x^3)  =  x / (1 + e^-2u)
 //
 // At -inf silu and the gelus give NaN (0 times infinity), as their formulas do.
+//
+// Error as evaluated, relative to the value: silu 2^-21 + |x| 2^-23, gelu 2^-19 + x^2 2^-23, gelu_tanh 2^-21 + |2u| 2^-22.  The first
+// term is the approximate reciprocal and power of two and the roundings around them.  The second is the power's argument, rounded to
+// 32 bits: it shows far out on the negative side, where the value itself is small (gelu at -5: 1.4e-6 of the value -1.4e-6).  Magnitudes below 2^-119 may
+// come out as 0, since both instructions flush (silu below x = -87.3, gelu -13.2, gelu_tanh -10.0).  Carrying the argument in two
+// floats would cost two to three instructions a value, and the 16-bit outputs of most calls would not show it.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -36,7 +42,8 @@ __device__ __forceinline__ float act_silu1(float x) { return x * rcp_approx(1.f 
 __device__ __forceinline__ float2 act_silu(float2 x) { return make_float2(act_silu1(x.x), act_silu1(x.y)); }
 // x Phi(x) = max(x, 0) - |x| Phi(-|x|), which cancels nowhere.  Phi(-a) = e^(-a^2 / 2) P(t), t = 1 / (1 + 0.305 a): the form of
 // Hastings' approximation of the error function (Abramowitz and Stegun 7.1.26) with eight terms, fitted here by weighted least
-// squares to a relative error of 1e-7 over 0 <= a <= 14.5, behind which the product is below the smallest float.
+// squares; the form's relative error over 0 <= a <= 14.5, in exact arithmetic, is 1e-7 (the roundings come on top, see above).  Behind
+// 14.5 the product is below the smallest float.
 __device__ __forceinline__ float2 act_gelu(float2 x)
 {
     const float2 a = make_float2(fabsf(x.x), fabsf(x.y));

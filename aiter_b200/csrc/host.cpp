@@ -14,24 +14,23 @@
 
 #include "../../include/aiter_b200.h"
 
+#include <limits>
+#include <type_traits>
+
 namespace {
 
 using Desc = aiter_tensor_t;
-using NormFn = int (*)(Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, float, float, float, int, int, int, void*);
-using ActFn  = int (*)(Desc*, Desc*, Desc*, int, int, void*);
-using Gemm16Fn = int (*)(Desc*, Desc*, Desc*, Desc*, Desc*, int, int, const char*, void*);
-using Gemm8Fn  = int (*)(Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, int, int, const char*, void*);
-using Gemm4Fn  = int (*)(Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, Desc*, int, int, const char*, void*);
-using WorkspaceFn = long long (*)(long long, long long, long long);
+// the library's functions, with the types that the public header declares
+#define ENTRY(name) decltype(&name)
 
 struct Bound
 {
-    NormFn norm;
-    ActFn act;
-    Gemm16Fn gemm16;
-    Gemm8Fn gemm8;
-    Gemm4Fn gemm4;
-    WorkspaceFn workspace;
+    ENTRY(aiter_b200_gated_residual_norm) norm;
+    ENTRY(aiter_b200_act_and_mul) act;
+    ENTRY(aiter_b200_gemm_a16w16_fused) gemm16;
+    ENTRY(aiter_b200_gemm_a8w8_mxfp8_fused) gemm8;
+    ENTRY(aiter_b200_gemm_a4w4_fused) gemm4;
+    ENTRY(aiter_b200_gemm_a4w4_fused_workspace) workspace;
     int dtypes[64]; // library's id of an ATen scalar type, -1: none
     at::ScalarType fp4x2, fp8, e8m0; // of MX operands and their scales
 } bound = {};
@@ -213,7 +212,10 @@ PyObject* gemm(PyObject*, PyObject* const* a, Py_ssize_t n)
     if(bits == 4 && A.size(0) >= 1024)
     {
         // tall problems re-lay the block scales once per call, in memory of this call's own (two captured graphs share none)
-        const long long bytes = bound.workspace(A.size(0), B.size(0), 2 * B.size(1));
+        // (sizes that no int holds are the library's to refuse)
+        constexpr int64_t most = std::numeric_limits<int>::max();
+        const bool fit         = A.size(0) <= most && B.size(0) <= most && B.size(1) <= most / 2;
+        const long long bytes  = fit ? bound.workspace(static_cast<int>(A.size(0)), static_cast<int>(B.size(0)), static_cast<int>(2 * B.size(1))) : 0;
         if(bytes > 0)
         {
             workspace = at::empty({static_cast<int64_t>(bytes)}, A.options().dtype(at::kByte));
@@ -243,12 +245,13 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
     count(n, 11);
-    bound.norm      = reinterpret_cast<NormFn>(address(a[0]));
-    bound.act       = reinterpret_cast<ActFn>(address(a[1]));
-    bound.gemm16    = reinterpret_cast<Gemm16Fn>(address(a[2]));
-    bound.gemm8     = reinterpret_cast<Gemm8Fn>(address(a[3]));
-    bound.gemm4     = reinterpret_cast<Gemm4Fn>(address(a[4]));
-    bound.workspace = reinterpret_cast<WorkspaceFn>(address(a[5]));
+    auto entry = [&](auto& function, int i) { function = reinterpret_cast<std::remove_reference_t<decltype(function)>>(address(a[i])); };
+    entry(bound.norm, 0);
+    entry(bound.act, 1);
+    entry(bound.gemm16, 2);
+    entry(bound.gemm8, 3);
+    entry(bound.gemm4, 4);
+    entry(bound.workspace, 5);
     for(int& id : bound.dtypes)
         id = -1;
     PyObject *key, *value;

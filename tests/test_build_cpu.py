@@ -21,3 +21,16 @@ def test_no_flag_trades_the_kernels_code_for_build_time():
     for flag in flags:
         name = flag.lstrip("-").split("=")[0]
         assert name not in ("split-compile", "split-compile-extended", "Ofast-compile", "maxrregcount", "use_fast_math", "G", "device-debug"), flag
+
+
+def test_the_extension_takes_the_librarys_function_types_from_its_header():
+    """A pointer type written out by hand can differ from the function behind it (three long long for three int) without a word from the
+    compiler, since the addresses arrive as integers."""
+    import re
+
+    with open(os.path.join(ROOT, "aiter_b200", "csrc", "host.cpp")) as f:
+        source = f.read()
+    assert not re.findall(r"using\s+\w+\s*=\s*[^;]*\(\*\)\s*\(", source), "a hand-written function pointer type"
+    header = open(os.path.join(ROOT, "include", "aiter_b200.h")).read()
+    names = re.findall(r"ENTRY\((aiter_b200_\w+)\)", source)
+    assert len(names) >= 6 and all(re.search(rf"\b{n}\(", header) for n in names)

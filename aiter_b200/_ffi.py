@@ -13,6 +13,7 @@ import importlib.machinery
 import importlib.util
 import os
 import struct
+import threading
 
 import torch
 
@@ -72,7 +73,8 @@ _lib.aiter_get_last_error.restype = ctypes.c_char_p
 _lib.aiter_b200_kernel_list.restype = ctypes.c_char_p
 _lib.aiter_b200_heuristic_name.restype = ctypes.c_char_p
 _lib.aiter_b200_launch_count.restype = ctypes.c_ulonglong
-_lib.aiter_b200_gemm_a4w4_fused_workspace.restype = ctypes.c_longlong
+if hasattr(_lib, "aiter_b200_gemm_a4w4_fused_workspace"):  # (a build from before the fused GEMMs has none)
+    _lib.aiter_b200_gemm_a4w4_fused_workspace.restype = ctypes.c_longlong
 assert _lib.aiter_ctypes_abi_version() == 2
 
 T, I, S, F = "tensor", "int", "str", "float"
@@ -205,20 +207,38 @@ def current_stream(device: int):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _load_host():
-    """The extension that allocates, fills descriptors and calls for the operators whose host time shows (see csrc/host.cpp)."""
-    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "_aiter_b200_host.so")
-    if not os.path.exists(path):
-        raise ImportError(f"{path} is missing: build it with `python aiter_b200/build.py`")
-    loader = importlib.machinery.ExtensionFileLoader("_aiter_b200_host", path)
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_aiter_b200_host", loader))
-    loader.exec_module(module)
-    names = ("gated_residual_norm", "act_and_mul", "gemm_a16w16_fused", "gemm_a8w8_mxfp8_fused", "gemm_a4w4_fused", "gemm_a4w4_fused_workspace")
-    module.bind(*(ctypes.cast(getattr(_lib, f"aiter_b200_{n}"), ctypes.c_void_p).value for n in names), dict(_DTYPE_IDS), aiter_dtype_id, fp4x2, fp8, fp8_e8m0)
-    return module
+HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "_aiter_b200_host.so")
+_HOST_ENTRIES = ("gated_residual_norm", "act_and_mul", "gemm_a16w16_fused", "gemm_a8w8_mxfp8_fused", "gemm_a4w4_fused", "gemm_a4w4_fused_workspace")
 
 
-host = _load_host()
+class _Host:
+    """The extension that allocates, fills descriptors and calls for the operators whose host time shows (see csrc/host.cpp).  It is loaded
+    with the first of them: the other operators need neither the extension nor a library that has these."""
+
+    _lock = threading.Lock()
+
+    def __getattr__(self, name):  # (only until the functions are there)
+        if name not in ("norm", "act", "gemm"):
+            raise AttributeError(name)
+        with self._lock:
+            if name not in self.__dict__:
+                self._load()
+        return self.__dict__[name]
+
+    def _load(self):
+        if not os.path.exists(HOST_PATH):
+            raise ImportError(f"{HOST_PATH} is missing: build it with `python aiter_b200/build.py`")
+        missing = [n for n in _HOST_ENTRIES if not hasattr(_lib, f"aiter_b200_{n}")]
+        if missing:
+            raise ImportError(f"{LIB_PATH} has no aiter_b200_{missing[0]}: it was built before this operator")
+        loader = importlib.machinery.ExtensionFileLoader("_aiter_b200_host", HOST_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_aiter_b200_host", loader))
+        loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(_lib, f"aiter_b200_{n}"), ctypes.c_void_p).value for n in _HOST_ENTRIES), dict(_DTYPE_IDS), aiter_dtype_id, fp4x2, fp8, fp8_e8m0)
+        self.__dict__.update(norm=module.norm, act=module.act, gemm=module.gemm)
+
+
+host = _Host()
 
 
 def call_host(name: str, function, *args):

@@ -275,7 +275,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
 {
     const unsigned n = prm.n;
     const int xd = prm.x.dt, rd = prm.res.ptr != nullptr ? prm.res.dt : (prm.h.ptr != nullptr ? prm.h.dt : xd);
-    // (short rows on any address: the general kernel's shifted groups, 16384 x 203 17 us against 22)
+    // (short rows on any address: the general kernel's shifted groups, 16384 x 203 16 us against 22)
     if(prm.M <= 2u * static_cast<unsigned>(sms) || (!aligned && n < 256) || (prm.h.ptr != nullptr && prm.h.dt != rd))
         return false;
     // one type for all parameters
@@ -304,8 +304,9 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
             return false;
         cnt        = n > 8192 ? 4 : n > 512 ? 2 : n > 256 ? 1 : 0; // (0: the short-row kernel)
         sh.threads = cnt == 0 ? 256 : ((n + 8 * cnt - 1) / (8 * cnt) + 31) / 32 * 32;
-        // The parameters are read through L1: several vectors of them want 100 KB of the SM's memory left to it (16384 x 8192 with
-        // three: 219 us with 192 KB of rows in flight, 198 with 128; with one: 173 and 191).
+        // The parameters are read through L1: several vectors of them want 100 KB of the SM's memory left to it (16384 x 8192, rms, with
+        // 192 KB of rows in flight and with 128: two norms and a gate 200 us and 184, a weight alone 191 with either.  A weight and a gate
+        // without the first norm go the other way, 173 and 194: the rule counts vectors, not norms).
         sh.budget = (params * n * param_bytes > 20u * 1024u ? 128u : 192u) * 1024u;
     }
     else
@@ -315,7 +316,7 @@ bool try_norm_stream(const NormParams& prm, bool aligned, int device, int sms, c
             return false;
         elems      = (n + 14) / 8 * 8; // (a row touches at most that many elements in whole groups)
         // two groups a thread, one where whole warps of them would leave more than 15 % of the lanes idle by comparison
-        // (8200 x 1155: 192 lanes for 146 groups 41 us, 160 lanes 35; 16384 x 1001, where both fit, 34 and 38)
+        // (8200 x 1155 with per-sample parameters: 192 lanes for 146 groups 41 us, 160 lanes 35; 16384 x 1001, where both fit, 34 and 38)
         auto warps = [&](unsigned c) { return ((elems / 8 + c - 1) / c + 31) / 32; };
         cnt        = n > 512 && 100 * warps(1) > 85 * 2 * warps(2) ? 2 : 1;
         if(warps(cnt) > 16)
@@ -359,7 +360,8 @@ void launch_norm(const NormParams& prm, bool aligned, int device, int sms, cudaS
     }
     // one group a thread where there are few rows (the shortest chain), up to four where the machine is full
     const bool few     = prm.M <= 2u * static_cast<unsigned>(sms);
-    // (SHIFT holds more registers a group: two at most, so that an SM keeps 32 warps; with four 4096 x 9001 141 us, with two 109)
+    // (SHIFT holds more registers a group: two at most, so that an SM keeps 32 warps, though under the 64 registers of that bound a thread
+    // spills 72 to 128 bytes; 4096 x 9001 126 us, four groups a thread took 30 % longer)
     const unsigned cnt = aligned ? (vecs > 1024 ? 4 : few ? 1 : vecs >= 1024 ? 4 : vecs >= 256 ? 2 : 1) : vecs > 1024 || (!few && vecs >= 256) ? 2 : 1;
     unsigned t         = ((vecs + cnt - 1) / cnt + 31) / 32 * 32;
     if(!aligned && vecs <= 16)

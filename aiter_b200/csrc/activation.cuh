@@ -34,7 +34,7 @@ __device__ __forceinline__ float ex2_approx(float x)
 }
 // Two values at a time.  Only gelu's polynomial uses the two-wide fp32 instructions of sm_100: for the short chains of silu and
 // gelu_tanh the moves into register pairs cost more than the issue slots they save (6 % of the gated activation's time on
-// 16384 x 12288), for gelu they save a little (1 %; in the GEMM's epilogue 39 -> 35 us on 4096 x 4096 x 1024).
+// 16384 x 12288), for gelu they save a little (1 %; in the GEMM's epilogue 39 -> 34 us on 4096 x 4096 x 1024).
 __device__ __forceinline__ float2 splat(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 rcp2(float2 x) { return make_float2(rcp_approx(x.x), rcp_approx(x.y)); }
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2_approx(x.x), ex2_approx(x.y)); }

@@ -501,7 +501,7 @@ __device__ __forceinline__ void affine(const NormParams& prm, Get&& get, size_t 
 // rows); more than one row per CTA only with at most a warp a row.  Bound by HBM for many rows (x, residual in, h, y out), by the chain load -
 // sum - load - store for one.  SHIFT: rows and parameters start on any element's address; the groups then begin on y's 16-byte
 // boundaries, the first and the last hold only some of the row, and the operands are shifted into place (one element at a time instead:
-// 6 x 3075 30 us against 3.8, 1142 x 5287 fp32 with a bf16 residual 146 against 25, 4096 x 9001 952 against 109).
+// 6 x 3075 30 us against 3.5, 1142 x 5287 fp32 with a bf16 residual 146 against 23, 4096 x 9001 952 against 126).
 template <int CNT, bool X32, bool R32, bool SHIFT>
 __global__ void __launch_bounds__(CNT == 1 || SHIFT ? 1024 : 512) norm_rows_kernel(const __grid_constant__ NormParams prm)
 {
@@ -688,7 +688,8 @@ __device__ __forceinline__ float pair_sum(const float (&v)[VEC])
 }
 
 // Rows that do not fit the registers: a CTA goes over its row once per sum and once for the outputs, recomputing h each
-// time (the row comes from L2 after the first pass).
+// time (the row comes from L2 after the first pass: 512 x 32768 56 us, of which 21 are its bytes at HBM's rate; rows on odd addresses
+// go one element at a time, 300 x 32001 118 us).
 template <int VEC>
 __global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ NormParams prm)
 {
@@ -811,7 +812,7 @@ struct ActMulParams
 };
 
 // Plain outputs: a thread takes U vectors of eight, 256 vectors apart, of the flat list of all rows' vectors; HBM-bound
-// (16384 x 12288: silu and gelu_tanh 175 us, 6.9 TB/s; gelu 202, whose arithmetic shows).  Compiled per activation: with all of them in
+// (16384 x 12288: relu 173 us, silu 177, gelu_tanh 180, 6.7 to 7.0 TB/s; gelu 205, whose arithmetic shows).  Compiled per activation: with all of them in
 // one kernel 190 and 207 us.
 template <bool X32, int ACT>
 __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ ActMulParams prm)
@@ -855,7 +856,7 @@ __global__ void __launch_bounds__(256) act_mul_kernel(const __grid_constant__ Ac
 }
 
 // Rows that start on any element's address: a thread's eight outputs begin on a 16-byte boundary of the output's row (its first and
-// last groups are partial), their operands are shifted into place (8192 x 1001 14.5 us, one element at a time 26).
+// last groups are partial), their operands are shifted into place (8192 x 1001 15.8 us, one element at a time 26).
 template <bool X32, int ACT>
 __global__ void __launch_bounds__(256) act_mul_shift_kernel(const __grid_constant__ ActMulParams prm)
 {

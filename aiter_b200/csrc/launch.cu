@@ -1025,9 +1025,11 @@ static bool fused_rows_aligned(const GemmProblem& prob)
 // bf16 with a fused epilogue, more than 64 rows.  Candidates are compared by a time estimate (units of 10 ns, `it` = K tiles of 64
 // elements) that was fitted to measurements of every tile by name on about 25 shapes (M = 100 .. 16384, N = 512 .. 8192, K = 512 ..
 // 8192): a start-up, and waves over the SMs times the time of a tile.  K is split inside a cluster only, one tile per cluster and
-// all clusters at once: 400 x 512 x 8192 43.8 (no split) -> 20.8 us; two waves of clusters are slower than none (300 x 1024 x 4096
-// in four slices 30.0, two 19.8, one 24.6 us).  Rows on odd addresses: weights on the 128-row slot, so that the lanes run along a
-// row of the output (4096 x 4097 x 1024: pairs 57.7 us, 128 x 256 tiles 64.5, row-major tiles 229).
+// all clusters at once: 400 x 512 x 8192 38.5 us (no split), 23.5 (two slices), 16.5 (four); two waves of clusters are slower than none
+// (300 x 1024 x 4096 in four slices 23.5, two 15.5, one 21.7 us; 333 x 1001 x 1160 on 64 rows in two slices 10.7, on 32 rows with K whole
+// 10.2).  Rows on odd addresses: weights on the 128-row slot, so that the lanes run along a row of the output (4096 x 4097 x 1024 with
+// gelu_tanh and a residual: pairs of 128 columns, which the estimate takes, 55 us, of 256 columns 48, 128 x 256 tiles 55, row-major
+// tiles 190).
 static void choose_fused_bf16(const GemmProblem& prob, int num_sms, KernelConfig& cfg)
 {
     const long long M = prob.M, N = prob.N, it = (prob.K + 63) / 64;
@@ -1078,9 +1080,10 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
         return;
     const long long M = prob.M, N = prob.N;
     // Tiles of 32 rows with the weights on the 128-row slot where they leave room for a K split over clusters: what a call with few
-    // tiles takes is its epilogue, which goes over a tile's rows 16 at a time, and one slice's K loop (us, tiles of 32 / what the
-    // rules below take, bf16, MXFP8, MXFP4: 76 x 464 x 512 6.4 / 8.8, 6.3 / 8.7, 6.0 / 8.0; 128 x 2048 x 2048 10.2 / 11.7, 9.9 / 11.1,
-    // 9.4 / 9.7; 128 x 1024 x 8192 15.4 / 20.3, 13.2 / 15.6, 12.0 / 13.0; not without that room: 76 x 4096 x 4096 22.2 / 18.5).
+    // tiles takes is its epilogue, which goes over a tile's rows 16 at a time, and one slice's K loop (us with a residual, tiles of 32 /
+    // tiles of 64 in four slices, bf16, MXFP8, MXFP4: 76 x 464 x 512 6.0 / 9.4, 5.5 / 9.3, 5.3 / 7.7; 128 x 2048 x 2048 10.2 / 11.7,
+    // 9.1 / 10.8, 8.8 / 10.3; 128 x 1024 x 8192 15.3 / 20.0, 12.5 / 15.5, 11.3 / 12.5; without that room 32 rows lose, bf16
+    // 76 x 4096 x 4096 22 / 18).
     if(M > 32 && M <= 600 && cfg.log2_splitk < 0)
     {
         const long long tiles = ((M + 31) / 32) * ((N + kTileP - 1) / kTileP);
@@ -1107,18 +1110,22 @@ static void choose_fused_config(const GemmProblem& prob, int num_sms, KernelConf
         return;
     if(!fused_rows_aligned(prob))
     {
-        // rows on odd addresses: see above
+        // rows on odd addresses: see above (silu and a residual, pairs of 256 columns / of 128 / 128 x 64 tiles, us: MXFP8 4096 x 4096 x 1024
+        // 45 / 47 / 73, MXFP4 42 / 44 / 69; small problems would take smaller tiles: MXFP8 1024 x 2048 x 512 12.8 / 10.2 / 12.3,
+        // 300 x 1040 x 384 15.5 / 9.9 / 7.4)
         cfg.swap = 1;
         cfg.cg   = 2;
         cfg.bn   = 256;
         return;
     }
     // MX tiles on CTA pairs: 256 columns leave TMEM no second accumulator beside the scale buffers, so the epilogue is exposed;
-    // 224 (MXFP8, four stages) or 192 have two.  Waves over the SM pairs x time per tile, fitted to 4096 x 7168 x K = 512 .. 8192
-    // (listed in 0.1 us, without activation, with silu, with a bf16 residual; the code counts in 0.01 us): MXFP8 256: 48 60 87 167 289,
-    // 65 76 104 170 300, 64 77 103 191 325; 224: 45 49 79 150 273, 63 67 87 165 312, 64 69 91 160 304; 192: 42 44 69 129 251,
-    // 56 59 74 151 292, 56 59 77 147 287; MXFP4 256: 47 50 67 98 156, 65 67 83 115 174, 64 66 82 114 177; 192: 44 46 58 77 133,
-    // 58 59 64 83 139, 58 58 64 84 146 (224 leaves MXFP4 two stages: 60 67 83 127 232 with silu).
+    // 224 (MXFP8, four stages) or 192 have two.  Waves over the SM pairs x time per tile.  The times of a tile on 4096 x 7168 x K = 512 .. 8192
+    // (in 0.1 us, without activation, with silu, with a bf16 residual; the code counts in 0.01 us): MXFP8 256: 46 58 85 143 265,
+    // 62 76 103 156 277, 63 75 101 157 285; 224: 42 49 78 141 270, 58 64 87 149 277, 63 70 89 151 280; 192: 37 42 68 122 235,
+    // 50 54 74 127 240, 51 56 74 130 242; MXFP4 256: 42 50 65 95 149, 61 65 82 113 167, 61 65 81 111 166; 192: 37 42 58 76 129,
+    // 50 54 58 86 139, 51 53 62 80 134 (224 leaves MXFP4 two stages).  The lines below were fitted to tiles that took up to 15 % longer; on
+    // these sizes they choose the fastest width or one within 3 %, but for MXFP8 at K = 512 (224 columns would be 6 to 10 % faster) and
+    // MXFP4 with silu at K = 8192 (256: 6 %).
     const long long pair_rows = (M + 2 * kTileP - 1) / (2 * kTileP);
     if(M >= 512 && N >= 192 && pair_rows * ((N + 255) / 256) >= 24)
     {
@@ -1179,8 +1186,8 @@ static bool try_launch_few_rows(const GemmProblem& prob, int num_sms)
     const KernelConfig& c = prob.cfg;
     if(!prob.fused || prob.kind != PK_BF16 || prob.M > 4 || prob.batch != 1 || c.swap >= 0 || c.bn > 0 || c.cg > 0 || c.stages > 0 || c.log2_splitk >= 0)
         return false;
-    // (us here / on tensor cores: 1 x 8192 x 8192 24.5 / 24.0; two rows 1024 x 8192 7.5 / 12.9, 2048 x 2048 5.3 / 6.8, 4096 x 4096 11.9 / 10.0;
-    // four rows 8.1 / 13.0, 5.8 / 6.8, 13.1 / 10.1)
+    // (us here / on tensor cores: 1 x 8192 x 8192 24.5 / 23.7; two rows 1024 x 8192 5.6 / 12.9, 2048 x 2048 5.2 / 6.6, 4096 x 4096 11.9 / 10.0;
+    // four rows 8.6 / 12.9, 5.8 / 6.6, 13.1 / 10.1)
     if(prob.N * prob.K > (prob.M == 1 ? 48LL : 10LL) << 20)
         return false;
     auto rows16 = [](const Operand& o) { return o.mode == OPM_ROWMAJOR && (reinterpret_cast<uintptr_t>(o.ptr) & 15) == 0 && (o.rows == 1 || o.ld_bytes % 16 == 0); };

@@ -1,10 +1,10 @@
 // gated_residual_norm for many rows: persistent CTAs that stream their rows through shared memory.
 //
 // The operator moves x and the residual in and h and y out, 8 bytes an element in 16-bit types, and is bound by HBM as long as
-// an SM always has some 50 KB of loads under way and spends less than about 25 instructions an element.  Hence: a CTA owns a
-// contiguous block of rows and keeps the next ones in flight with bulk copies (one thread, two instructions a row, no
-// registers), while the current row goes from shared memory to registers, through its one or two norms and out; a thread holds
-// 16 values, over which the fixed work of a row (its sums, addresses) is spread, and types are compile-time.
+// an SM always has some 50 KB of loads under way and spends few instructions an element (35 with both norms and a gate: 16384 x 8192
+// 184 us, 5.8 TB/s).  Hence: a CTA owns a contiguous block of rows and keeps the next ones in flight with bulk copies (one thread,
+// two instructions a row, no registers), while the current row goes from shared memory to registers, through its one or two norms
+// and out; a thread holds 16 values, over which the fixed work of a row (its sums, addresses) is spread, and types are compile-time.
 //
 // Rows of any width have a kernel of their own below, short rows another.
 #pragma once
@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(512, CNT <= 2 ? 2 : 1) norm_stream_kernel(cons
 // of a row only in part -, so every access of x, residual, h and y stays a 16-byte one.  A row's phase in its groups repeats every
 // eight rows: a CTA takes every eighth row of its block, and keeps the parameters in shared memory at that phase.  (One element a
 // lane at a time: 8192 x 4097 106 to 150 us, at about 100 instructions an element; parameters shifted into place by selects on
-// every row, 8200 x 1155 with three of them, 55 us.)
+// every row, 8200 x 1155 with three of them, 55 us.  As it stands: 8192 x 4097 54 us, 8200 x 1155 with three 40, at 77 instructions an
+// element - a thread holds eight values there, over which the row's two sums and its addresses are spread.)
 template <int XD, int RD, int PD, int CNT>
 __global__ void __launch_bounds__(512, 2) norm_stream_flat_kernel(const __grid_constant__ NormParams prm, const __grid_constant__ NormStreamLayout lay)
 {
